@@ -521,6 +521,187 @@ int vpa_release_blocks(const uint32_t* block_tables, int32_t block_table_stride,
                        uint32_t* free_ring_state, int32_t free_ring_capacity, int32_t num_rows,
                        void* stream);
 
+/*
+ * rotary_qk - rotary positions of one to four axes (time, height, width, ...)
+ * applied to the new rows of q and k, with the rows' RMS norms in front.
+ * The step between the projections and reshape_and_cache in the decoder
+ * layer (q_norm / k_norm, then the multi-axis rotation,
+ * vasr-models/src/model/thinker_text.rs:1041-1068; the reference's fused
+ * apply_rotary_qk, vasr-quant/src/lib.rs:83-89).
+ *
+ * query [num_tokens, num_heads, head_dim], key [num_tokens, num_kv_heads,
+ * head_dim], heads contiguous, token strides in elements; out_query /
+ * out_key likewise, and they may be query / key themselves (with the same
+ * stride). For a row x:
+ *   n = x * w / sqrt(mean(x^2) + norm_eps)   (w: query_norm / key_norm
+ *       [head_dim] of the row's type, or NULL: n = x)
+ *   a_i = positions[axes[i], token] * inv_freq[i]     i < rotary_dim / 2
+ *   (y_p, y_s) = (n_p cos a_i - n_s sin a_i, n_s cos a_i + n_p sin a_i)
+ * with the pairs (p, s) = (i, i + rotary_dim / 2), or (2i, 2i + 1) where
+ * `adjacent` is not 0; dims from rotary_dim on are n. Each value is rounded
+ * once, at the store; angles are formed and reduced in 64 bits.
+ * positions: [num_axes, num_tokens], int64 (positions_i64 != 0) or uint32,
+ * position_axis_stride elements between axes (0: all axes share one row).
+ * inv_freq: f64 [rotary_dim / 2], 16-byte aligned. axes: u8 [rotary_dim / 2],
+ * 4-byte aligned, each below num_axes (one past it counts as the last axis);
+ * NULL: all 0. num_axes 1 to 4. head_dim a multiple of 16 up to 256,
+ * rotary_dim a multiple of 16 up to head_dim (0: no rotation). Rows, norms and
+ * strides 16-byte aligned. dtype f32, f16 or bf16. num_tokens == 0 is a no-op.
+ */
+int vpa_rotary_qk(void* out_query, void* out_key, const void* query, const void* key,
+                  int64_t out_query_token_stride, int64_t out_key_token_stride,
+                  int64_t query_token_stride, int64_t key_token_stride, const void* positions,
+                  int64_t position_axis_stride, int32_t positions_i64, const void* inv_freq,
+                  const uint8_t* axes, int32_t num_axes, int32_t rotary_dim, int32_t adjacent,
+                  const void* query_norm, const void* key_norm, float norm_eps,
+                  int64_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                  int32_t dtype, void* stream);
+
+/*
+ * rotary_reshape_and_cache - vpa_rotary_qk of q and k followed by
+ * vpa_reshape_and_cache of k and v, in one launch: the rotated k goes from
+ * registers to the cache and is never written as rows. Arguments, layouts
+ * and errors as in those two; value [num_tokens, num_kv_heads, head_dim]
+ * with its token stride; out_query may be query. A rotated key is rounded
+ * once, to the cache's type (fp8: E4M3FN(y / *k_scale)). Tokens whose slot is
+ * negative or past the pool still get their rotated query. Slots of one call
+ * are distinct.
+ */
+int vpa_rotary_reshape_and_cache(
+    void* out_query, const void* query, const void* key, const void* value,
+    int64_t out_query_token_stride, int64_t query_token_stride, int64_t key_token_stride,
+    int64_t value_token_stride, const void* positions, int64_t position_axis_stride,
+    int32_t positions_i64, const void* inv_freq, const uint8_t* axes, int32_t num_axes,
+    int32_t rotary_dim, int32_t adjacent, const void* query_norm, const void* key_norm,
+    float norm_eps, const float* k_scale, const float* v_scale, void* key_cache,
+    void* value_cache, const int64_t* slot_mapping, int64_t num_tokens, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t num_blocks,
+    int64_t cache_block_stride, int64_t cache_head_stride, int32_t dtype, int32_t cache_dtype,
+    void* stream);
+
+/*
+ * Bytes of caller workspace vpa_paged_attention_weights needs. Depends only
+ * on the arguments; 0 where one of them is.
+ */
+size_t vpa_paged_attention_weights_workspace_size(int64_t total_query_rows, int32_t num_heads,
+                                                  int32_t max_context_len);
+
+/*
+ * paged_attention_weights - adds the attention weight that each cached token
+ * gets from the call's queries to running scores, by which a cache is cut
+ * (vpa_evict_kv_cache). No counterpart in the reference.
+ *
+ * query [total_query_rows, num_heads, head_dim] packed; sequence s owns rows
+ * cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 (n_s of them; NULL: row s
+ * alone) and its first L_s = context_lens[s] cached tokens, the rows' own
+ * included, as in vpa_chunked_prefill_paged_attention. For kv head j and
+ * token t < L_s
+ *   scores[s, j, t] += sum over its rows r and the query heads h of j of
+ *     exp(softmax_scale q[r, h] . K[s, j, t] - m) / sum_t' exp(...)
+ * over the tokens row r sees: all t < L_s, or with causal != 0 t <= r +
+ * L_s - n_s. A row that sees none adds nothing; block ids >= num_blocks are
+ * absent. Scores at and past L_s are not touched. scores f32 [num_seqs,
+ * num_kv_heads, >= max_context_len], strides in elements, tokens contiguous.
+ * One query per sequence is a decode step; the last rows of a prompt are the
+ * usual window before its cache is cut; the rows of drafted tokens fit too.
+ * A score's sum has a fixed order: results do not vary from call to call.
+ * Types, head dims and block sizes as the chunked prefill, any number of
+ * query heads per kv head. n_s and L_s are clamped to max_query_len and
+ * max_context_len, rows at or past total_query_rows are not read. workspace:
+ * vpa_paged_attention_weights_workspace_size bytes, 256-byte aligned; calls
+ * that run concurrently need one each.
+ */
+int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
+                                int64_t score_head_stride, const void* query,
+                                const float* k_scale, const void* key_cache,
+                                const uint32_t* block_tables, int32_t block_table_stride,
+                                const uint32_t* cu_seqlens_q, const uint32_t* context_lens,
+                                int32_t num_seqs, int32_t max_query_len,
+                                int32_t max_context_len, int64_t total_query_rows,
+                                float softmax_scale, int32_t causal, int32_t num_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                int64_t num_blocks, int64_t cache_block_stride,
+                                int64_t cache_head_stride, int32_t dtype, int32_t cache_dtype,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * evict_kv_cache - cuts every sequence's cache to `budget` tokens per kv head
+ * by accumulated attention weight, in place. No counterpart in the reference.
+ *
+ * A sequence of L = min(context_lens[s], max_context_len, its table) > budget
+ * tokens keeps, in each kv head j, its first keep_first tokens, its last
+ * keep_last, and of the others the ones with the highest scores[s, j, t], so
+ * that `budget` remain (equal scores: the lower index; NaN below every
+ * number). They move to positions 0 .. budget - 1 in their order, in
+ * key_cache, value_cache and scores; scores at budget .. L - 1 become 0.
+ * Every head keeps its own tokens: the block table stays common, and the
+ * sequence goes on as one of `budget` tokens (blocks past ceil(budget /
+ * block_size) may be released). Keys keep the rotation of the position they
+ * were appended at. Shorter sequences stay as they are.
+ *   new_context_lens[s] = min(L, budget)           (not context_lens itself)
+ *   kept[s, j, i]: old position of the token now at i, 0xffffffff past the
+ *   last; u32 [num_seqs, num_kv_heads, budget]
+ * budget >= 1, keep_first + keep_last <= budget. Cache geometry and types as
+ * vpa_reshape_and_cache; bytes are moved as they are. Blocks of different
+ * sequences, and columns of one, must be distinct (a cached prefix that
+ * sequences share cannot be evicted from one of them); tokens of block ids >=
+ * num_blocks are neither read nor written.
+ */
+int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
+                       int64_t score_seq_stride, int64_t score_head_stride,
+                       const uint32_t* block_tables, int32_t block_table_stride,
+                       const uint32_t* context_lens, uint32_t* new_context_lens,
+                       uint32_t* kept, int32_t num_seqs, int32_t max_context_len,
+                       int32_t budget, int32_t keep_first, int32_t keep_last,
+                       int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                       int64_t num_blocks, int64_t cache_block_stride,
+                       int64_t cache_head_stride, int32_t cache_dtype, void* stream);
+
+/*
+ * Bytes of caller workspace vpa_verify_draft_tokens needs. Depends only on the
+ * arguments; 0 where num_seqs or vocab is.
+ */
+size_t vpa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t max_drafts,
+                                              int32_t vocab);
+
+/*
+ * verify_draft_tokens - accepts or replaces drafted tokens by the target's
+ * logits, from given random numbers: the sampling counterpart of
+ * vpa_argmax_rows (the reference decodes greedily, one token per step,
+ * vasr-models/src/model/generation.rs:443-460).
+ *
+ * Sequence b has n = num_drafts[b] drafts (NULL: max_drafts; larger ones
+ * count as max_drafts) draft_ids[b, 0 .. n - 1]. target_logits [num_seqs,
+ * max_drafts + 1, vocab]: row i follows draft i - 1. draft_logits [num_seqs,
+ * max_drafts, vocab]: the distributions the drafts were drawn from, or NULL
+ * (drafts that were looked up: probability 1). With T = temperature[b]
+ * (NULL: 1) > 0, p_i = softmax(target_i / T), q_i = softmax(draft_i / T):
+ *   draft i is accepted while accept_u[b, i] * q_i(x_i) < p_i(x_i);
+ *   the first one that is not is replaced by a draw from max(p_i - q_i, 0)
+ *   scaled to sum 1 (from p_i where that is 0 everywhere); if all n are
+ *   accepted, a draw from p_n follows.
+ * A draw is the first v with cumsum(r)[v] > sample_u[b] * sum(r), summed in
+ * f64. T <= 0 or NaN: draft i is accepted if it is the first maximum of row i,
+ * and the row's first maximum replaces it or follows. Logits of -inf and NaN
+ * have probability 0; a row of nothing else gives id 0. Ids >= vocab are
+ * never accepted.
+ *   out_ids[b, 0 .. c - 1], c = out_count[b] = accepted + 1: the emitted
+ *   tokens; 0xffffffff behind them (u32 [num_seqs, max_drafts + 1])
+ * max_drafts 0 samples one token per sequence; at most 64. accept_u f32
+ * [num_seqs, max_drafts] and sample_u f32 [num_seqs], in [0, 1). Logits f32,
+ * f16 or bf16, strides in elements, vocab contiguous. workspace:
+ * vpa_verify_draft_tokens_workspace_size bytes, 256-byte aligned; calls that
+ * run concurrently need one each.
+ */
+int vpa_verify_draft_tokens(uint32_t* out_ids, uint32_t* out_count, const void* target_logits,
+                            int64_t target_seq_stride, int64_t target_row_stride,
+                            const void* draft_logits, int64_t draft_seq_stride,
+                            int64_t draft_row_stride, const uint32_t* draft_ids,
+                            const uint32_t* num_drafts, const float* temperature,
+                            const float* accept_u, const float* sample_u, int32_t num_seqs,
+                            int32_t max_drafts, int32_t vocab, int32_t dtype, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

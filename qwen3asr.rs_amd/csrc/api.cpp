@@ -843,4 +843,333 @@ int vpa_release_blocks(const uint32_t* block_tables, int32_t block_table_stride,
                                               static_cast<hipStream_t>(stream)));
 }
 
+namespace {
+
+// Checks of the rows, norms, positions and tables shared by the rotary ops.
+int check_rotary(const char* op, const RotaryRows& a, const RotaryArgs& r, int32_t dtype) {
+  if (!is_float_dtype(dtype))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: unsupported dtype %s", op, dtype_name(dtype));
+  if (a.num_tokens < 0 || a.num_heads <= 0 || a.num_kv_heads <= 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_tokens=%lld num_heads=%d num_kv_heads=%d", op,
+                (long long)a.num_tokens, a.num_heads, a.num_kv_heads);
+  if (a.head_dim <= 0 || a.head_dim % 16 != 0 || a.head_dim > 256)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: head_dim=%d must be a multiple of 16 up to 256", op,
+                a.head_dim);
+  if (r.rotary_dim < 0 || r.rotary_dim % 16 != 0 || r.rotary_dim > a.head_dim)
+    return fail(VPA_ERR_UNSUPPORTED,
+                "%s: rotary_dim=%d must be a multiple of 16 up to head_dim=%d", op, r.rotary_dim,
+                a.head_dim);
+  if (r.num_axes < 1 || r.num_axes > kRotaryMaxAxes)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_axes=%d must be 1 to %d", op, r.num_axes,
+                kRotaryMaxAxes);
+  if (!(a.eps >= 0.f) || a.eps > 3.0e38f)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: norm_eps must be finite and >= 0, got %g", op,
+                (double)a.eps);
+  if (a.num_tokens == 0) return VPA_OK;
+  if (r.axis_stride != 0 && r.axis_stride < a.num_tokens)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: position axis stride %lld smaller than num_tokens=%lld", op,
+                (long long)r.axis_stride, (long long)a.num_tokens);
+  if (a.q == nullptr || a.k == nullptr || a.out_q == nullptr || r.positions == nullptr ||
+      (r.rotary_dim > 0 && r.inv_freq == nullptr))
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: query, key, outputs, positions and inv_freq must be non-null", op);
+  const int64_t q_row = (int64_t)a.num_heads * a.head_dim;
+  const int64_t k_row = (int64_t)a.num_kv_heads * a.head_dim;
+  if (a.q_stride < q_row || a.out_q_stride < q_row || a.k_stride < k_row ||
+      (a.out_k != nullptr && a.out_k_stride < k_row))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: token strides smaller than a token's rows", op);
+  if ((a.out_q == a.q && a.out_q_stride != a.q_stride) ||
+      (a.out_k == a.k && a.out_k_stride != a.k_stride))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: in place needs equal token strides", op);
+  const int eb = dtype_bytes(dtype);
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.out_q) || !aligned16(a.out_k) ||
+      !aligned16(a.q_norm) || !aligned16(a.k_norm) || (a.q_stride * eb) % 16 != 0 ||
+      (a.k_stride * eb) % 16 != 0 || (a.out_q_stride * eb) % 16 != 0 ||
+      (a.out_k != nullptr && (a.out_k_stride * eb) % 16 != 0))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: rows and norms must be 16-byte aligned", op);
+  if (!aligned16(r.inv_freq) || (reinterpret_cast<uintptr_t>(r.axes) & 3u) != 0 ||
+      (reinterpret_cast<uintptr_t>(r.positions) & (r.positions_i64 ? 7u : 3u)) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: inv_freq must be 16-byte, axes 4-byte and positions element aligned", op);
+  // one 256-lane workgroup per (token, kv head) or 32 lanes per head row at
+  // most, on a 1D grid whose lane count must fit in 32 bits
+  if (a.num_tokens > (int64_t)0xffffff / ((int64_t)a.num_heads + a.num_kv_heads))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: too many tokens for one launch: %lld", op,
+                (long long)a.num_tokens);
+  return VPA_OK;
+}
+
+}  // namespace
+
+int vpa_rotary_qk(void* out_query, void* out_key, const void* query, const void* key,
+                  int64_t out_query_token_stride, int64_t out_key_token_stride,
+                  int64_t query_token_stride, int64_t key_token_stride, const void* positions,
+                  int64_t position_axis_stride, int32_t positions_i64, const void* inv_freq,
+                  const uint8_t* axes, int32_t num_axes, int32_t rotary_dim, int32_t adjacent,
+                  const void* query_norm, const void* key_norm, float norm_eps,
+                  int64_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                  int32_t dtype, void* stream) {
+  clear_error();
+  const char* op = "rotary_qk";
+  const RotaryRows a{query, key, query_token_stride, key_token_stride, out_query, out_key,
+                     out_query_token_stride, out_key_token_stride, query_norm, key_norm, norm_eps,
+                     num_tokens, num_heads, num_kv_heads, head_dim};
+  const RotaryArgs r{positions, position_axis_stride, static_cast<const double*>(inv_freq), axes,
+                     num_axes, rotary_dim, positions_i64 != 0, adjacent != 0};
+  const int rc = check_rotary(op, a, r, dtype);
+  if (rc != VPA_OK) return rc;
+  if (num_tokens == 0) return VPA_OK;
+  if (out_key == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: out_key must be non-null", op);
+  return hip_status(op, launch_rotary_qk(dtype, a, r, static_cast<hipStream_t>(stream)));
+}
+
+int vpa_rotary_reshape_and_cache(
+    void* out_query, const void* query, const void* key, const void* value,
+    int64_t out_query_token_stride, int64_t query_token_stride, int64_t key_token_stride,
+    int64_t value_token_stride, const void* positions, int64_t position_axis_stride,
+    int32_t positions_i64, const void* inv_freq, const uint8_t* axes, int32_t num_axes,
+    int32_t rotary_dim, int32_t adjacent, const void* query_norm, const void* key_norm,
+    float norm_eps, const float* k_scale, const float* v_scale, void* key_cache,
+    void* value_cache, const int64_t* slot_mapping, int64_t num_tokens, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t num_blocks,
+    int64_t cache_block_stride, int64_t cache_head_stride, int32_t dtype, int32_t cache_dtype,
+    void* stream) {
+  clear_error();
+  const char* op = "rotary_reshape_and_cache";
+  const RotaryRows a{query, key, query_token_stride, key_token_stride, out_query, nullptr,
+                     out_query_token_stride, 0, query_norm, key_norm, norm_eps, num_tokens,
+                     num_heads, num_kv_heads, head_dim};
+  const RotaryArgs r{positions, position_axis_stride, static_cast<const double*>(inv_freq), axes,
+                     num_axes, rotary_dim, positions_i64 != 0, adjacent != 0};
+  int rc = check_rotary(op, a, r, dtype);
+  if (rc != VPA_OK) return rc;
+  if (dtype != cache_dtype && cache_dtype != VPA_DTYPE_FP8_E4M3)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: cache dtype %s differs from input dtype %s", op,
+                dtype_name(cache_dtype), dtype_name(dtype));
+  rc = check_cache(op, cache_dtype, num_kv_heads, head_dim, block_size, num_blocks,
+                   cache_block_stride, cache_head_stride, key_cache, value_cache);
+  if (rc != VPA_OK) return rc;
+  rc = check_scales(op, cache_dtype, k_scale, v_scale);
+  if (rc != VPA_OK) return rc;
+  if (num_heads % num_kv_heads != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_heads=%d not a multiple of num_kv_heads=%d",
+                op, num_heads, num_kv_heads);
+  if (num_tokens == 0) return VPA_OK;
+  if (value == nullptr || slot_mapping == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: value and slot_mapping must be non-null", op);
+  if (value_token_stride < (int64_t)num_kv_heads * head_dim)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: value token stride %lld smaller than a token's row",
+                op, (long long)value_token_stride);
+  if (!aligned16(value) || (value_token_stride * dtype_bytes(dtype)) % 16 != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: value rows must be 16-byte aligned", op);
+  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
+                    cache_head_stride};
+  const RotaryCache c{value, value_token_stride, key_cache, value_cache, slot_mapping, k_scale,
+                      v_scale};
+  return hip_status(op, launch_rotary_cache(dtype, cache_dtype, a, r, c, g,
+                                            static_cast<hipStream_t>(stream)));
+}
+
+size_t vpa_paged_attention_weights_workspace_size(int64_t total_query_rows, int32_t num_heads,
+                                                  int32_t max_context_len) {
+  if (total_query_rows <= 0 || num_heads <= 0 || max_context_len <= 0) return 0;
+  return weights_workspace_bytes(total_query_rows, num_heads, max_context_len);
+}
+
+int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
+                                int64_t score_head_stride, const void* query,
+                                const float* k_scale, const void* key_cache,
+                                const uint32_t* block_tables, int32_t block_table_stride,
+                                const uint32_t* cu_seqlens_q, const uint32_t* context_lens,
+                                int32_t num_seqs, int32_t max_query_len,
+                                int32_t max_context_len, int64_t total_query_rows,
+                                float softmax_scale, int32_t causal, int32_t num_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                int64_t num_blocks, int64_t cache_block_stride,
+                                int64_t cache_head_stride, int32_t dtype, int32_t cache_dtype,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* op = "paged_attention_weights";
+  if (!is_float_dtype(dtype))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: unsupported query dtype %s", op, dtype_name(dtype));
+  if (dtype != cache_dtype && cache_dtype != VPA_DTYPE_FP8_E4M3)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: cache dtype %s differs from query dtype %s", op,
+                dtype_name(cache_dtype), dtype_name(dtype));
+  int rc = check_cache(op, cache_dtype, num_kv_heads, head_dim, block_size, num_blocks,
+                       cache_block_stride, cache_head_stride, key_cache, key_cache);
+  if (rc != VPA_OK) return rc;
+  if (cache_dtype == VPA_DTYPE_FP8_E4M3 &&
+      (k_scale == nullptr || (reinterpret_cast<uintptr_t>(k_scale) & 3u) != 0))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: an fp8 cache needs a 4-byte aligned k_scale", op);
+  if (num_seqs < 0 || num_heads <= 0 || max_query_len < 0 || max_context_len < 0 ||
+      total_query_rows < 0 || block_table_stride < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_seqs=%d num_heads=%d max_query_len=%d max_context_len=%d "
+                "total_query_rows=%lld block_table_stride=%d",
+                op, num_seqs, num_heads, max_query_len, max_context_len,
+                (long long)total_query_rows, block_table_stride);
+  if (num_heads % num_kv_heads != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_heads=%d not a multiple of num_kv_heads=%d",
+                op, num_heads, num_kv_heads);
+  if (num_seqs == 0 || max_query_len == 0 || max_context_len == 0 || total_query_rows == 0)
+    return VPA_OK;
+  if (num_seqs > 65535 || num_kv_heads > 65535)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_seqs=%d and num_kv_heads=%d must not exceed 65535",
+                op, num_seqs, num_kv_heads);
+  if (max_context_len > (1 << 28))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: max_context_len=%d exceeds %d", op, max_context_len,
+                1 << 28);
+  {
+    const int64_t chunks = ((int64_t)max_context_len + kWeightsChunk - 1) / kWeightsChunk;
+    const int64_t row_groups = ((int64_t)max_query_len * (num_heads / num_kv_heads) + 15) / 16;
+    // (256-lane workgroups: the grid's lane count must fit in 32 bits)
+    if (row_groups > 0xffffff || chunks * row_groups > 0xffffff / num_kv_heads)
+      return fail(VPA_ERR_UNSUPPORTED, "%s: too many rows and tokens for one launch", op);
+  }
+  if (scores == nullptr || query == nullptr || block_tables == nullptr || context_lens == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: scores, query, block_tables and context_lens must be non-null", op);
+  if (!aligned16(query) || (reinterpret_cast<uintptr_t>(scores) & 3u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: misaligned query or scores", op);
+  if ((int64_t)block_table_stride * block_size < max_context_len)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: block_table_stride=%d too small for max_context_len=%d (block_size=%d)", op,
+                block_table_stride, max_context_len, block_size);
+  if (score_head_stride < max_context_len || score_seq_stride < score_head_stride * num_kv_heads)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: score strides (seq=%lld head=%lld) overlap for max_context_len=%d", op,
+                (long long)score_seq_stride, (long long)score_head_stride, max_context_len);
+  const size_t need = weights_workspace_bytes(total_query_rows, num_heads, max_context_len);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(VPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", op, need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", op);
+  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
+                    cache_head_stride};
+  const WeightsArgs w{query, key_cache, k_scale, block_tables, block_table_stride, cu_seqlens_q,
+                      context_lens, softmax_scale, causal, num_seqs, max_query_len,
+                      max_context_len, total_query_rows, num_heads, scores, score_seq_stride,
+                      score_head_stride, workspace};
+  return hip_status(op, launch_attention_weights(dtype, cache_dtype, w, g,
+                                                 static_cast<hipStream_t>(stream)));
+}
+
+int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
+                       int64_t score_seq_stride, int64_t score_head_stride,
+                       const uint32_t* block_tables, int32_t block_table_stride,
+                       const uint32_t* context_lens, uint32_t* new_context_lens,
+                       uint32_t* kept, int32_t num_seqs, int32_t max_context_len,
+                       int32_t budget, int32_t keep_first, int32_t keep_last,
+                       int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                       int64_t num_blocks, int64_t cache_block_stride,
+                       int64_t cache_head_stride, int32_t cache_dtype, void* stream) {
+  clear_error();
+  const char* op = "evict_kv_cache";
+  int rc = check_cache(op, cache_dtype, num_kv_heads, head_dim, block_size, num_blocks,
+                       cache_block_stride, cache_head_stride, key_cache, value_cache);
+  if (rc != VPA_OK) return rc;
+  if (num_seqs < 0 || max_context_len < 0 || block_table_stride < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_seqs=%d max_context_len=%d block_table_stride=%d", op, num_seqs,
+                max_context_len, block_table_stride);
+  if (budget < 1 || keep_first < 0 || keep_last < 0 || (int64_t)keep_first + keep_last > budget)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: budget=%d must be positive and hold keep_first=%d + keep_last=%d", op, budget,
+                keep_first, keep_last);
+  if (num_seqs == 0) return VPA_OK;
+  // (up to 64 workgroups of 256 lanes each: the grid's lane count must fit in
+  // 32 bits)
+  if ((int64_t)num_seqs * num_kv_heads >= ((int64_t)1 << 18))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_seqs=%d times num_kv_heads=%d reaches 2^18", op,
+                num_seqs, num_kv_heads);
+  if (max_context_len > (1 << 30) || budget > (1 << 30))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: max_context_len=%d or budget=%d exceeds 2^30", op,
+                max_context_len, budget);
+  if (scores == nullptr || block_tables == nullptr || context_lens == nullptr ||
+      new_context_lens == nullptr || kept == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: scores, block_tables, context_lens, new_context_lens and kept must be non-null",
+                op);
+  if (new_context_lens == context_lens)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: new_context_lens must not be context_lens", op);
+  if ((int64_t)block_table_stride * block_size < max_context_len)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: block_table_stride=%d too small for max_context_len=%d (block_size=%d)", op,
+                block_table_stride, max_context_len, block_size);
+  if (score_head_stride < max_context_len || score_seq_stride < score_head_stride * num_kv_heads)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: score strides (seq=%lld head=%lld) overlap for max_context_len=%d", op,
+                (long long)score_seq_stride, (long long)score_head_stride, max_context_len);
+  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
+                    cache_head_stride};
+  const EvictArgs e{key_cache, value_cache, scores, score_seq_stride, score_head_stride,
+                    block_tables, block_table_stride, context_lens, max_context_len, num_seqs,
+                    budget, keep_first, keep_last, new_context_lens, kept};
+  return hip_status(op, launch_evict(cache_dtype, e, g, static_cast<hipStream_t>(stream)));
+}
+
+size_t vpa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t max_drafts,
+                                              int32_t vocab) {
+  if (num_seqs <= 0 || max_drafts < 0 || vocab <= 0) return 0;
+  return verify_workspace_bytes(num_seqs, max_drafts, vocab);
+}
+
+int vpa_verify_draft_tokens(uint32_t* out_ids, uint32_t* out_count, const void* target_logits,
+                            int64_t target_seq_stride, int64_t target_row_stride,
+                            const void* draft_logits, int64_t draft_seq_stride,
+                            int64_t draft_row_stride, const uint32_t* draft_ids,
+                            const uint32_t* num_drafts, const float* temperature,
+                            const float* accept_u, const float* sample_u, int32_t num_seqs,
+                            int32_t max_drafts, int32_t vocab, int32_t dtype, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* op = "verify_draft_tokens";
+  if (!is_float_dtype(dtype))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: unsupported logits dtype %s", op, dtype_name(dtype));
+  if (num_seqs < 0 || max_drafts < 0 || vocab < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: bad sizes num_seqs=%d max_drafts=%d vocab=%d", op,
+                num_seqs, max_drafts, vocab);
+  if (max_drafts > kVerifyMaxDrafts)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: max_drafts=%d exceeds %d", op, max_drafts,
+                kVerifyMaxDrafts);
+  if (num_seqs == 0) return VPA_OK;
+  if (vocab == 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: a draw from empty rows (vocab = 0)", op);
+  if (num_seqs > 65535 || vocab > (1 << 30))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_seqs=%d exceeds 65535 or vocab=%d 2^30", op,
+                num_seqs, vocab);
+  // (256-lane workgroups: the grid's lane count must fit in 32 bits)
+  if ((int64_t)num_seqs * (2 * max_drafts + 1) * (((int64_t)vocab + 4095) / 4096) > 0xffffff)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: too many logits for one launch", op);
+  if (out_ids == nullptr || out_count == nullptr || target_logits == nullptr ||
+      sample_u == nullptr || (max_drafts > 0 && (draft_ids == nullptr || accept_u == nullptr)))
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: outputs, target_logits, draft_ids, accept_u and sample_u must be non-null",
+                op);
+  // (rows may repeat through a zero stride: they are only read)
+  if (target_row_stride < 0 || target_seq_stride < 0 || draft_row_stride < 0 ||
+      draft_seq_stride < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: negative strides", op);
+  const uintptr_t eb = (uintptr_t)dtype_bytes(dtype);
+  if (reinterpret_cast<uintptr_t>(target_logits) % eb != 0 ||
+      reinterpret_cast<uintptr_t>(draft_logits) % eb != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: misaligned logits", op);
+  const size_t need = verify_workspace_bytes(num_seqs, max_drafts, vocab);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(VPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", op, need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", op);
+  // no drafts: the drafter's logits have no rows
+  const void* draft = max_drafts > 0 ? draft_logits : nullptr;
+  const VerifyArgs v{target_logits, target_seq_stride, target_row_stride, draft, draft_seq_stride,
+                     draft_row_stride, draft_ids, num_drafts, temperature, accept_u, sample_u,
+                     num_seqs, max_drafts, vocab, out_ids, out_count, workspace};
+  return hip_status(op, launch_verify(dtype, v, static_cast<hipStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -271,6 +271,112 @@ hipError_t launch_prefill_vector(int dtype, int cache_dtype, void* out, const vo
                                  const float* k_scale, const float* v_scale,
                                  hipStream_t stream);
 
+// Rotary positions (rotary_kernels.hip): the angle of pair i is
+// positions[axes[i]][token] * inv_freq[i]; axes null: one axis.
+constexpr int kRotaryMaxAxes = 4;
+struct RotaryArgs {
+  const void* positions;  // [num_axes, tokens], i64 or u32
+  int64_t axis_stride;    // elements
+  const double* inv_freq;
+  const uint8_t* axes;
+  int32_t num_axes;
+  int32_t rotary_dim;
+  bool positions_i64;
+  bool adjacent;
+};
+// The rows of one call: q and k as they come (heads contiguous, token strides
+// in elements), where the rotated ones go, and the norms' weights (or null).
+struct RotaryRows {
+  const void* q;
+  const void* k;
+  int64_t q_stride, k_stride;
+  void* out_q;
+  void* out_k;
+  int64_t out_q_stride, out_k_stride;
+  const void* q_norm;
+  const void* k_norm;
+  float eps;
+  int64_t num_tokens;
+  int32_t num_heads, num_kv_heads, head_dim;
+};
+// Where the second form's k and v rows go.
+struct RotaryCache {
+  const void* v;
+  int64_t v_stride;
+  void* key_cache;
+  void* value_cache;
+  const int64_t* slot_mapping;
+  const float* k_scale;
+  const float* v_scale;
+};
+hipError_t launch_rotary_qk(int dtype, const RotaryRows& a, const RotaryArgs& r,
+                            hipStream_t stream);
+hipError_t launch_rotary_cache(int dtype, int cache_dtype, const RotaryRows& a,
+                               const RotaryArgs& r, const RotaryCache& k, const CacheGeom& g,
+                               hipStream_t stream);
+
+// Attention weights of cached tokens (weights_kernels.hip). The workspace
+// holds every row's logits and, per chunk of kWeightsChunk tokens, its
+// maximum and sum.
+constexpr int kWeightsChunk = 256;
+struct WeightsArgs {
+  const void* query;
+  const void* key_cache;
+  const float* k_scale;
+  const uint32_t* block_tables;
+  int32_t block_table_stride;
+  const uint32_t* cu_seqlens_q;  // null: one row per sequence
+  const uint32_t* context_lens;
+  float scale;
+  int32_t causal;
+  int32_t num_seqs, max_query_len, max_ctx;
+  int64_t total_rows;
+  int32_t num_heads;
+  float* scores;
+  int64_t score_seq_stride, score_head_stride;
+  void* workspace;
+};
+size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx);
+hipError_t launch_attention_weights(int dtype, int cache_dtype, const WeightsArgs& a,
+                                    const CacheGeom& g, hipStream_t stream);
+
+// Eviction (evict_kernels.hip).
+struct EvictArgs {
+  void* key_cache;
+  void* value_cache;
+  float* scores;
+  int64_t score_seq_stride, score_head_stride;
+  const uint32_t* block_tables;
+  int32_t block_table_stride;
+  const uint32_t* context_lens;
+  int32_t max_ctx, num_seqs;
+  int32_t budget, keep_first, keep_last;
+  uint32_t* new_lens;
+  uint32_t* kept;  // [num_seqs, num_kv_heads, budget]
+};
+hipError_t launch_evict(int cache_dtype, const EvictArgs& a, const CacheGeom& g,
+                        hipStream_t stream);
+
+// Draft verification (verify_kernels.hip).
+struct VerifyArgs {
+  const void* target;  // [num_seqs, max_drafts + 1, vocab]
+  int64_t target_seq_stride, target_row_stride;
+  const void* draft;  // [num_seqs, max_drafts, vocab] or null
+  int64_t draft_seq_stride, draft_row_stride;
+  const uint32_t* draft_ids;   // [num_seqs, max_drafts]
+  const uint32_t* num_drafts;  // [num_seqs] or null
+  const float* temperature;    // [num_seqs] or null (1)
+  const float* accept_u;       // [num_seqs, max_drafts]
+  const float* sample_u;       // [num_seqs]
+  int32_t num_seqs, max_drafts, vocab;
+  uint32_t* out_ids;    // [num_seqs, max_drafts + 1]
+  uint32_t* out_count;  // [num_seqs]
+  void* workspace;
+};
+constexpr int kVerifyMaxDrafts = 64;
+size_t verify_workspace_bytes(int32_t num_seqs, int32_t max_drafts, int32_t vocab);
+hipError_t launch_verify(int dtype, const VerifyArgs& a, hipStream_t stream);
+
 // True when the MFMA prefill kernel is compiled for this combination.
 bool prefill_supported(int dtype, int cache_dtype, int head_dim, int block_size, int group);
 

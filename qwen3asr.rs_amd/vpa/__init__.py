@@ -20,8 +20,15 @@ from .ops import (  # noqa: F401
     reshape_and_cache,
     reshape_and_cache_paged_attention,
 )
+from .eviction import (  # noqa: F401
+    evict_kv_cache,
+    paged_attention_weights,
+    paged_attention_weights_workspace,
+)
 from .graph import DecodeGraphCache  # noqa: F401
+from .rotary import rotary_frequencies, rotary_qk, rotary_reshape_and_cache  # noqa: F401
 from .step import DeviceDecodeStep  # noqa: F401
+from .verify import verify_draft_tokens, verify_draft_tokens_workspace  # noqa: F401
 
 __all__ = [
     "DecodeGraphCache",
@@ -31,12 +38,20 @@ __all__ = [
     "VpaError",
     "argmax_token_ids_from_logits",
     "cache_geometry",
+    "evict_kv_cache",
     "gather_kv_cache",
     "paged_attention",
     "paged_attention_plan",
+    "paged_attention_weights",
+    "paged_attention_weights_workspace",
     "paged_cache_read",
     "paged_attention_varlen_prefill",
     "paged_attention_workspace",
     "reshape_and_cache",
     "reshape_and_cache_paged_attention",
+    "rotary_frequencies",
+    "rotary_qk",
+    "rotary_reshape_and_cache",
+    "verify_draft_tokens",
+    "verify_draft_tokens_workspace",
 ]

@@ -75,6 +75,23 @@ SIGNATURES = {
     "vpa_decode_step_metadata": (ctypes.c_int, [
         _p, _i32, _p, _p, _p, _p, _p, _i32, _i32, _p, _p, _p, _i32, _p]),
     "vpa_release_blocks": (ctypes.c_int, [_p, _i32, _p, _p, _p, _p, _i32, _i32, _p]),
+    "vpa_rotary_qk": (ctypes.c_int, [
+        _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _p, _p,
+        _f32, _i64, _i32, _i32, _i32, _i32, _p]),
+    "vpa_rotary_reshape_and_cache": (ctypes.c_int, [
+        _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _p, _p,
+        _f32, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _p]),
+    "vpa_paged_attention_weights_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "vpa_paged_attention_weights": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i64, _f32, _i32, _i32,
+        _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _p, _sz, _p]),
+    "vpa_evict_kv_cache": (ctypes.c_int, [
+        _p, _p, _p, _i64, _i64, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+        _i32, _i64, _i64, _i64, _i32, _p]),
+    "vpa_verify_draft_tokens_workspace_size": (_sz, [_i32, _i32, _i32]),
+    "vpa_verify_draft_tokens": (ctypes.c_int, [
+        _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p,
+        _sz, _p]),
     # include/vpa_host.h
     "vpa_bytes_per_paged_block": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _p]),
     "vpa_pool_blocks_for_context": (ctypes.c_int, [_i64, _i32, _p]),

@@ -20,6 +20,7 @@ launch, as the reference returns ``Err(candle_core::Error::Msg)``.
 
 from __future__ import annotations
 
+import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -58,6 +59,14 @@ def _stream(t: torch.Tensor) -> int:
     if _raw_stream is None or not t.is_cuda:
         return torch.cuda.current_stream(t.device).cuda_stream  # raises: not a GPU
     return _raw_stream(t.get_device())
+
+
+def _on_device_of(t: torch.Tensor):
+    """Makes t's GPU the current one where it is not (launches go to the current
+    device)."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -518,6 +527,20 @@ class DeviceBlockAllocator:
             self.slot_mapping.data_ptr(), self.context_lens.data_ptr(), self.status.data_ptr(),
             self.batch, _stream(self.block_tables)))
         return self.slot_mapping, self.context_lens
+
+    def trim(self, num_tokens: torch.Tensor) -> None:
+        """Rows hold num_tokens[r] tokens from here on (u32 [batch], at most what
+        they held): the next step appends there, and the blocks past them go
+        back (trim_request_to_num_tokens, paged_cache_runtime.rs:320-340). For rows
+        whose drafted tokens were rejected or whose cache was cut."""
+        if num_tokens.dtype != torch.uint32 or num_tokens.shape != (self.batch,):
+            raise _err(f"num_tokens must be u32 [{self.batch}], got {num_tokens.dtype} "
+                       f"{tuple(num_tokens.shape)}")
+        self.positions.copy_(num_tokens)
+        bs = self.block_size
+        # (u32 arithmetic through the bits: torch has none of its own)
+        keep = (num_tokens.view(torch.int32).long() + (bs - 1)) // bs
+        self.release(keep.to(torch.int32).view(torch.uint32))
 
     def release(self, keep_blocks: torch.Tensor) -> None:
         """Rows keep their first keep_blocks[r] blocks (u32 [batch]), the rest go back."""
