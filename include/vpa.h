@@ -625,6 +625,13 @@ int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Bytes of caller workspace vpa_evict_kv_cache needs. Depends only on the
+ * arguments; 0 where one of them is.
+ */
+size_t vpa_evict_kv_cache_workspace_size(int32_t num_seqs, int32_t num_kv_heads,
+                                         int32_t max_context_len, int32_t block_size);
+
+/*
  * evict_kv_cache - cuts every sequence's cache to `budget` tokens per kv head
  * by accumulated attention weight, in place. No counterpart in the reference.
  *
@@ -645,7 +652,9 @@ int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
  * vpa_reshape_and_cache; bytes are moved as they are. Blocks of different
  * sequences, and columns of one, must be distinct (a cached prefix that
  * sequences share cannot be evicted from one of them); tokens of block ids >=
- * num_blocks are neither read nor written.
+ * num_blocks are neither read nor written, and the place one would move to
+ * keeps what it holds. workspace: vpa_evict_kv_cache_workspace_size bytes,
+ * 256-byte aligned; calls that run concurrently need one each.
  */
 int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
                        int64_t score_seq_stride, int64_t score_head_stride,
@@ -655,7 +664,8 @@ int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
                        int32_t budget, int32_t keep_first, int32_t keep_last,
                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                        int64_t num_blocks, int64_t cache_block_stride,
-                       int64_t cache_head_stride, int32_t cache_dtype, void* stream);
+                       int64_t cache_head_stride, int32_t cache_dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /*
  * Bytes of caller workspace vpa_verify_draft_tokens needs. Depends only on the

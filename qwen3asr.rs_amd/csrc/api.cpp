@@ -1058,6 +1058,12 @@ int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
                                                  static_cast<hipStream_t>(stream)));
 }
 
+size_t vpa_evict_kv_cache_workspace_size(int32_t num_seqs, int32_t num_kv_heads,
+                                         int32_t max_context_len, int32_t block_size) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || max_context_len <= 0 || block_size <= 0) return 0;
+  return evict_workspace_bytes(num_seqs, num_kv_heads, max_context_len, block_size);
+}
+
 int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
                        int64_t score_seq_stride, int64_t score_head_stride,
                        const uint32_t* block_tables, int32_t block_table_stride,
@@ -1066,7 +1072,8 @@ int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
                        int32_t budget, int32_t keep_first, int32_t keep_last,
                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                        int64_t num_blocks, int64_t cache_block_stride,
-                       int64_t cache_head_stride, int32_t cache_dtype, void* stream) {
+                       int64_t cache_head_stride, int32_t cache_dtype, void* workspace,
+                       size_t workspace_bytes, void* stream) {
   clear_error();
   const char* op = "evict_kv_cache";
   int rc = check_cache(op, cache_dtype, num_kv_heads, head_dim, block_size, num_blocks,
@@ -1106,10 +1113,18 @@ int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
                 (long long)score_seq_stride, (long long)score_head_stride, max_context_len);
   const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
                     cache_head_stride};
+  const size_t need =
+      vpa_evict_kv_cache_workspace_size(num_seqs, num_kv_heads, max_context_len, block_size);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(VPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", op, need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", op);
   const EvictArgs e{key_cache, value_cache, scores, score_seq_stride, score_head_stride,
                     block_tables, block_table_stride, context_lens, max_context_len, num_seqs,
                     budget, keep_first, keep_last, new_context_lens, kept};
-  return hip_status(op, launch_evict(cache_dtype, e, g, static_cast<hipStream_t>(stream)));
+  return hip_status(op, launch_evict(cache_dtype, e, workspace, g,
+                                     static_cast<hipStream_t>(stream)));
 }
 
 size_t vpa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t max_drafts,

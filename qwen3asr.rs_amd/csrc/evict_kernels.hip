@@ -32,8 +32,6 @@
 namespace vpa {
 namespace {
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kBins = 2048;
 constexpr uint32_t kNone = 0xffffffffu;
 
@@ -51,6 +49,7 @@ __device__ __forceinline__ int context_of(const EvictArgs& a, int s, int bs) {
 
 // Inclusive sum over the workgroup's threads before and with this one, and the
 // total. Every thread calls it; s_w is free again after the next barrier.
+template <int kWaves>
 __device__ __forceinline__ int group_scan(int v, int* s_w, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int in = wave_scan_i32(v);
@@ -59,7 +58,7 @@ __device__ __forceinline__ int group_scan(int v, int* s_w, int& total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kSelWaves; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     const int n = s_w[w];
     before += w < wave ? n : 0;
     total += n;
@@ -67,24 +66,60 @@ __device__ __forceinline__ int group_scan(int v, int* s_w, int& total) {
   return before + in;
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a,
-                                                                   int32_t num_kv_heads, int32_t bs) {
+// Items of a chunk held by a thread: wave w has tokens w * 64 * R + 64 i + lane of
+// the chunk's kThreads * R, so a wave's tokens are one run.
+constexpr int kItems = 16;
+
+// One workgroup per (sequence, kv head). A row of up to 16 tokens per thread is
+// read once and stays in registers for the three digits and the final walk; a
+// longer one is read chunk by chunk in each of the four passes.
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int32_t num_kv_heads,
+                                                                int32_t bs_log2) {
+  const int bs = 1 << bs_log2;
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kChunk = kThreads * kItems;
+  constexpr int kPer = kBins / kThreads;  // bins per thread
   __shared__ int s_hist[kBins];
-  __shared__ int s_w[2][kSelWaves];
+  __shared__ int s_w[2][kWaves];
   __shared__ int s_digit, s_rank;
   const int j = (int)(blockIdx.x % (uint32_t)num_kv_heads);
   const int s = (int)(blockIdx.x / (uint32_t)num_kv_heads);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int L = context_of(a, s, bs);
-  uint32_t* kept = a.kept + ((int64_t)s * num_kv_heads + j) * a.budget;
+  const int64_t pair = (int64_t)s * num_kv_heads + j;
+  uint32_t* kept = a.kept + pair * a.budget;
   if (j == 0 && tid == 0) a.new_lens[s] = (uint32_t)min(L, a.budget);
   if (L <= a.budget) {  // nothing to evict
-    for (int i = tid; i < a.budget; i += kSelThreads) kept[i] = i < L ? (uint32_t)i : kNone;
+    for (int i = tid; i < a.budget; i += kThreads) kept[i] = i < L ? (uint32_t)i : kNone;
     return;
   }
   float* score = a.scores + s * a.score_seq_stride + j * a.score_head_stride;
+  uint2* columns = a.columns + pair * a.max_columns;
   const int lo = a.keep_first, hi = L - a.keep_last;  // lo < hi: budget >= first + last
   const int want = a.budget - a.keep_first - a.keep_last;
+  const int chunks = (L + kChunk - 1) / kChunk;
+  // items per thread of a chunk
+  auto items_of = [&](int c) { return (min(L - c * kChunk, kChunk) + kThreads - 1) / kThreads; };
+  float f[kItems];
+  uint32_t inside, middle;  // bit i: item i is one of the sequence's tokens; of its middle
+  auto load_chunk = [&](int c) {
+    const int R = items_of(c), t0 = c * kChunk + wave * 64 * R + lane;
+    inside = middle = 0u;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int t = t0 + 64 * i;
+      const bool in = i < R && t < L;
+      f[i] = 0.f;
+      if (in) f[i] = score[t];
+      inside |= (uint32_t)in << i;
+      middle |= (uint32_t)(in && t >= lo && t < hi) << i;
+    }
+    // (opaque, so that the bits stay bits: as comparisons kept from pass to pass
+    // they would not fit the scalar registers)
+    asm volatile("" : "+v"(inside), "+v"(middle));
+  };
+  load_chunk(0);
 
   // threshold: `prefix` is the pattern of the want-th highest score of the
   // middle, `rank` how many scores equal to it are kept
@@ -97,78 +132,175 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a,
       const int bits = pass < 2 ? 11 : 10;
       const uint32_t seen = pass == 0 ? 0u : 0xffffffffu << shift;
       shift -= bits;
-      for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
+      for (int i = tid; i < kBins; i += kThreads) s_hist[i] = 0;
       __syncthreads();
-      for (int t = lo + tid; t < hi; t += kSelThreads) {
-        const uint32_t key = score_key(score[t]);
-        if ((key & seen) == prefix) atomicAdd(&s_hist[(key >> shift) & ((1u << bits) - 1)], 1);
+      for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) load_chunk(c);
+        const int R = items_of(c);
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          if (i >= R) continue;  // (uniform)
+          const uint32_t key = score_key(f[i]);
+          if (((middle >> i) & 1u) && (key & seen) == prefix)
+            atomicAdd(&s_hist[(key >> shift) & ((1u << bits) - 1)], 1);
+        }
       }
       __syncthreads();
-      // bins from the highest down, two per thread; the one where the count
+      // bins from the highest down, kPer per thread; the one where the count
       // reaches `rank`
-      const int b = kBins - 1 - 2 * tid;
-      const int n0 = s_hist[b], n1 = s_hist[b - 1];
+      const int b = kBins - 1 - kPer * tid;
+      int n[kPer], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        n[i] = s_hist[b - i];
+        mine += n[i];
+      }
       int total;
-      const int upto = group_scan(n0 + n1, s_w[0], total);
-      const int before = upto - n0 - n1;
+      const int upto = group_scan<kWaves>(mine, s_w[0], total);
+      int before = upto - mine;
       if (before < rank && rank <= upto) {
-        const bool second = rank > before + n0;
-        s_digit = second ? b - 1 : b;
-        s_rank = rank - before - (second ? n0 : 0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (before < rank && rank <= before + n[i]) {
+            s_digit = b - i;
+            s_rank = rank - before;
+          }
+          before += n[i];
+        }
       }
       __syncthreads();
       prefix |= (uint32_t)s_digit << shift;
       rank = s_rank;
-      __syncthreads();
     }
   }
-  // one walk in order: kept indices and scores, a stretch of 1024 tokens read
-  // before its part is written (at or before it)
+  // in token order: kept indices, moved scores, and each table column's kept
+  // tokens for the move. Every score of a chunk is read (waited for) before the
+  // barrier, every write lies at or before the chunk's tokens.
   int done = 0, equal = 0;
-  for (int t0 = 0; t0 < L; t0 += kSelThreads) {
-    const int t = t0 + tid;
-    const float f = t < L ? score[t] : 0.f;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // read before the barriers below
-    const bool middle = t >= lo && t < hi;
-    const uint32_t key = score_key(f);
-    const bool eq = want > 0 && middle && key == prefix;
-    int eq_total, total;
-    const int eq_rank = equal + group_scan(eq ? 1 : 0, s_w[0], eq_total);  // 1-based
-    const bool keep = t < L && (!middle || (want > 0 && (key > prefix || (eq && eq_rank <= rank))));
-    const int pos = done + group_scan(keep ? 1 : 0, s_w[1], total) - 1;
-    // (the wait above and group_scan's barriers stand between every thread's
-    // read of its score and the writes below)
-    if (keep && pos < a.budget) {
-      kept[pos] = (uint32_t)t;
-      score[pos] = f;
+  for (int c = 0; c < chunks; ++c) {
+    if (chunks > 1) {
+      __syncthreads();  // (the previous chunk's counts are read)
+      load_chunk(c);
     }
-    equal += eq_total;
-    done += total;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int R = items_of(c), t0 = c * kChunk + wave * 64 * R + lane;
+    // bit i: token i of the thread is kept whatever its place among equals; is
+    // one of the equals
+    uint32_t above = 0, ties = 0;
+    int n_above = 0, n_ties = 0;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t key = score_key(f[i]);
+      above |= (uint32_t)(want > 0 && key > prefix) << i;
+      ties |= (uint32_t)(want > 0 && key == prefix) << i;
+    }
+    above = (above & middle) | (inside & ~middle);
+    ties &= middle;
+    asm volatile("" : "+v"(above), "+v"(ties));
+    n_above = wave_sum_i32(__builtin_popcount(above));
+    n_ties = wave_sum_i32(__builtin_popcount(ties));
+    if (lane == 0) {
+      s_w[0][wave] = n_above;
+      s_w[1][wave] = n_ties;
+    }
     __syncthreads();
+    int eq = equal, kept_before = done;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const int na = s_w[0][w], nt = s_w[1][w];
+      // of a wave's ties those that are among the first `rank` stay
+      const int take = min(max(rank - equal, 0), nt);
+      if (w < wave) {
+        eq += nt;
+        kept_before += na + take;
+      }
+      equal += nt;
+      done += na + take;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (i >= R) continue;  // (uniform)
+      const int t = t0 + 64 * i;
+      const uint64_t tie = __ballot((ties >> i) & 1u);
+      const bool tie_kept = ((ties >> i) & 1u) && eq + __builtin_popcountll(tie & below) < rank;
+      const bool mine = ((above >> i) & 1u) || tie_kept;
+      const uint64_t keep = __ballot(mine);
+      const int pos = kept_before + __builtin_popcountll(keep & below);
+      if (mine && pos < a.budget) {
+        kept[pos] = (uint32_t)t;
+        score[pos] = f[i];
+      }
+      if ((lane & (bs - 1)) == 0 && t < L) {
+        const uint32_t full = 0xffffffffu >> (32 - bs), mask = (uint32_t)(keep >> lane) & full;
+        columns[t >> bs_log2] = make_uint2(mask, (uint32_t)pos);
+        // the first column that loses a token: what lies before it stays in place
+        if (mask != full && pos == t) a.first_column[pair] = (uint32_t)(t >> bs_log2);
+      }
+      eq += __builtin_popcountll(tie);
+      kept_before += __builtin_popcountll(keep);
+      __builtin_amdgcn_sched_barrier(0);  // (one item's lane masks at a time fit the scalar registers)
+    }
   }
-  for (int t = a.budget + tid; t < L; t += kSelThreads) score[t] = 0.f;
+  __syncthreads();
+  for (int t = a.budget + tid; t < L; t += kThreads) score[t] = 0.f;
 }
 
-constexpr int kMoveThreads = 256;
-
-// Waits until this wave's loads have arrived, then for the workgroup's other
-// waves: no store after it can overtake a load before it.
-__device__ __forceinline__ void loads_done_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// Workgroup barrier for data exchanged through LDS: the wave's global loads and
+// stores stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// One workgroup per (sequence, kv head, K or V, group of `dims` dims): moves
-// those dims of every kept token, kStretch tokens at a time.
-// E: cache element (moved as it is).
-template <typename E, int BS>
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(
-    EvictArgs a, int32_t num_kv_heads, int32_t head_dim, int32_t dims, int64_t num_blocks,
-    int64_t block_stride, int64_t head_stride) {
-  constexpr int X = 16 / (int)sizeof(E);
-  constexpr int kStretch = 256;
-  const int groups = head_dim / dims;
+// One workgroup per (sequence, kv head, K or V, group of DG dims): DG dims of a
+// cache block are one run of DG * BS elements in the key tile (whole chunks) and
+// in the value tile (whole rows) alike. The workgroup walks the table's columns in
+// batches: it reads the runs of a batch's columns that have kept tokens, 16
+// bytes per lane, into LDS as they lie, then gathers from there, 16 bytes at a
+// time, what goes to each destination block, and writes runs of whole vectors
+// (single elements of a value row only where a batch ends inside a vector). A
+// column's kept tokens come from the selection as a bit mask and the place of the
+// first; from them the batch makes a list of where each place's token lies in
+// LDS, common to all its dims, so a gathered element costs one LDS read. (Putting
+// each token's elements from registers to their places instead takes a
+// predicated LDS write for every element that is read, kept or not: 330 us for 64
+// sequences of 600 to 4096 tokens, 8 heads of 128 dims in 16 bits, cut to 1024
+// tokens; 197 us so.) Reading whole columns costs nothing: a value row's 32-byte
+// sector holds 16 tokens. The next two batches' runs are in flight while one is
+// written: they lie behind everything that is written (a place is at or before
+// the token that moves to it). Columns before the first evicted token stay.
+// E: cache element, moved as it is; BS tokens per block; NV vectors per thread and
+// batch.
+template <typename E, int BS, int DG, int kThreads, int NV>
+__global__ __launch_bounds__(kThreads) void evict_move_kernel(
+    EvictArgs a, int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks, int64_t block_stride,
+    int64_t head_stride) {
+  constexpr int EB = (int)sizeof(E);
+  constexpr int X = 16 / EB;
+  constexpr int VPB = DG * BS / X;            // 16-byte vectors of a block's run
+  constexpr int kCols = kThreads * NV / VPB;  // columns of a batch
+  constexpr int kTok = kCols * BS;            // tokens of a batch
+  // a wave's vectors lie in one column (and its units in one block): its index,
+  // and the addresses made from it, stay in scalar registers
+  constexpr bool kUniform = VPB % 64 == 0;
+  // A run in LDS. Value rows are read at one token by lanes of different rows, so
+  // 8 bytes of padding follow every 256: rows that would share a bank do not.
+  constexpr int kRunBytes = VPB * 16 + (VPB + 15) / 16 * 8;
+  constexpr int RUN = (kRunBytes + 15) / 16 * 16 / EB;
+  constexpr int U = BS < X ? BS : X;          // tokens of a value unit
+  constexpr int kInfo = 512;  // columns whose masks, places and blocks wait in LDS
+  static_assert(DG % X == 0 && kThreads * NV % VPB == 0 && kCols >= 1 && kInfo % (2 * kCols) == 0,
+                "whole chunks, columns and pairs of batches");
+  __shared__ __align__(16) E s_run[kCols * RUN];
+  __shared__ __align__(16) uint32_t s_src[kTok + 2 * U];  // of each place: its token's byte in s_run
+  __shared__ uint2 s_col[kInfo];                          // {mask, place of the first kept token}
+  // offsets (elements) of the blocks of the columns and of the places, -1: absent
+  __shared__ int64_t s_from[kInfo], s_to[kInfo + 1];
+  __shared__ int s_p1, s_absent[2];
+  const int groups = head_dim / DG;
   uint32_t w = blockIdx.x;
   const int dg = (int)(w % (uint32_t)groups);
   w /= (uint32_t)groups;
@@ -176,73 +308,209 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(
   w >>= 1;
   const int j = (int)(w % (uint32_t)num_kv_heads);
   const int s = (int)(w / (uint32_t)num_kv_heads);
+  const int64_t pair = (int64_t)s * num_kv_heads + j;
+  const uint2* columns = a.columns + pair * a.max_columns;
+  const uint32_t* table = a.block_tables + (int64_t)s * a.block_table_stride;
+  auto offset_of = [&](int c) {
+    const uint32_t b = table[c];
+    return (int64_t)b < num_blocks ? (int64_t)b * block_stride : (int64_t)-1;
+  };
+  // Where all columns fit, they are read together with the length (one round
+  // trip before the first data, not three; what lies past the context is not
+  // used); else window by window.
+  const bool whole = a.max_columns <= kInfo;
+  if (whole)
+    for (int i = threadIdx.x; i < a.max_columns; i += kThreads) {
+      s_col[i] = columns[i];
+      s_from[i] = offset_of(i);
+    }
+  const int c_begin = (int)a.first_column[pair];
   const int L = context_of(a, s, BS);
   if (L <= a.budget) return;
-  const uint32_t* kept = a.kept + ((int64_t)s * num_kv_heads + j) * a.budget;
-  const uint32_t* table = a.block_tables + (int64_t)s * a.block_table_stride;
-  E* cache = static_cast<E*>(value ? a.value_cache : a.key_cache) + j * head_stride;
-  const int d0 = dg * dims;
-  const int i_thr = threadIdx.x;  // token of the stretch
-  for (int i0 = 0; i0 < a.budget; i0 += kStretch) {
-    const int n = min(kStretch, a.budget - i0);
-    if (kept[i0 + n - 1] == (uint32_t)(i0 + n - 1)) continue;  // all in place
-    const int i = i0 + i_thr;
-    const uint32_t src = i_thr < n ? kept[i] : kNone;
-    // a token whose block is not one of the pool's (a table entry past it) is
-    // neither read nor written
-    const bool live = i_thr < n && src < (uint32_t)L;
-    const uint32_t sb = live ? table[src / BS] : kNone, db = live ? table[i / BS] : kNone;
-    const bool from = (int64_t)sb < num_blocks && live, to = from && (int64_t)db < num_blocks;
-    const E* ps = cache + (from ? (int64_t)sb : 0) * block_stride;
-    E* pd = cache + (to ? (int64_t)db : 0) * block_stride;
-    if (!value) {
-      for (int d = 0; d < dims; d += 4 * X) {
-        uint4 u[4] = {};
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (to && d + q * X < dims)
-            u[q] = *reinterpret_cast<const uint4*>(ps + (d0 + d + q * X) * BS + (src % BS) * X);
-        loads_done_barrier();
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (to && d + q * X < dims)
-            *reinterpret_cast<uint4*>(pd + (d0 + d + q * X) * BS + (i % BS) * X) = u[q];
+  E* cache = static_cast<E*>(value ? a.value_cache : a.key_cache) + j * head_stride +
+             (int64_t)dg * DG * BS;
+  const int tid = threadIdx.x;
+  const int c_end = (L + BS - 1) / BS;
+
+  auto row_at = [](int row) { return row * BS + row * BS * EB / 256 * (8 / EB); };  // in a run
+  auto uniform64 = [](int64_t v) {
+    if constexpr (kUniform)
+      return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+    else return v;
+  };
+  auto uniform = [](int v) {
+    if constexpr (kUniform) return __builtin_amdgcn_readfirstlane(v);
+    else return v;
+  };
+  if (tid < 2) s_absent[tid] = 0;
+  int flip = 0, p0 = c_begin * BS;  // (nothing before c_begin moves)
+  for (int sc = whole ? 0 : c_begin; sc < c_end; sc += kInfo) {
+    const int n = min(kInfo, c_end - sc), to0 = whole ? 0 : p0 / BS;
+    const int64_t* places = whole ? s_from : s_to;  // blocks from place to0 * BS on
+    if (!whole) {
+      __syncthreads();
+      for (int i = tid; i <= n; i += kThreads) {
+        if (i < n) {
+          s_col[i] = columns[sc + i];
+          s_from[i] = offset_of(sc + i);
+        }
+        s_to[i] = to0 + i < c_end ? offset_of(to0 + i) : -1;
       }
-    } else {
-      for (int d = 0; d < dims; d += 16) {
-        E u[16] = {};
+    }
+    __syncthreads();
+    // (a column whose block is not one of the pool's is neither read nor moved)
+    auto load_data = [&](uint4(&u)[NV], int c0) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-          if (to && d + q < dims) u[q] = ps[(d0 + d + q) * BS + src % BS];
-        loads_done_barrier();
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-          if (to && d + q < dims) pd[(d0 + d + q) * BS + i % BS] = u[q];
+      for (int k = 0; k < NV; ++k) {
+        const int c = uniform(c0 + (k * kThreads + tid) / VPB);
+        u[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (c < n && uniform((int)s_col[c].x) != 0) {
+          const int64_t at = uniform64(s_from[c]);
+          if (at >= 0)
+            u[k] = load_stream(reinterpret_cast<const uint4*>(cache + at) + (k * kThreads + tid) % VPB);
+        }
       }
+    };
+    auto batch = [&](uint4(&u)[NV], int c0) {
+      const int c_last = min(c0 + kCols, n) - 1;
+      const int aligned = p0 / U * U;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = k * kThreads + tid, v = q % VPB;
+        if (!value) {
+          *reinterpret_cast<uint4*>(s_run + q / VPB * RUN + v * X) = u[k];
+        } else {
+          uint2* to = reinterpret_cast<uint2*>(reinterpret_cast<char*>(s_run + q / VPB * RUN) +
+                                               v * 16 + v / 16 * 8);
+          to[0] = make_uint2(u[k].x, u[k].y);
+          to[1] = make_uint2(u[k].z, u[k].w);
+        }
+      }
+      for (int i = tid; i < kTok; i += kThreads) {
+        const int off = i % BS, c = c0 + i / BS;
+        if (c > c_last) break;
+        const uint2 col = s_col[c];
+        if ((col.x >> off) & 1u) {
+          const bool there = s_from[c] >= 0;
+          s_src[(int)col.y + __builtin_popcount(col.x & ((1u << off) - 1u)) - aligned] =
+              there ? (uint32_t)(i / BS * RUN + (value ? off : off * X)) * EB : kNone;
+          if (!there) s_absent[flip] = 1;
+        }
+        if (c == c_last && off == 0) s_p1 = (int)col.y + __builtin_popcount(col.x);
+      }
+      lds_barrier();  // the batch is read and lies in LDS
+      const int p1 = s_p1;
+      const bool all_there = s_absent[flip] == 0;
+      load_data(u, c0 + 2 * kCols);
+      if (tid == 0) s_absent[flip ^ 1] = 0;
+      const int b0 = p0 / BS, nb = p1 > p0 ? (p1 - 1) / BS - b0 + 1 : 0;
+      if (!value) {
+        for (int q = tid; q < nb * VPB; q += kThreads) {
+          const int i = uniform(q / VPB), v = q % VPB, p = (b0 + i) * BS + v % BS;
+          const int64_t to = uniform64(places[b0 + i - to0]);
+          if (to < 0 || p < p0 || p >= p1) continue;
+          const uint32_t src = s_src[p - aligned];
+          if (src == kNone) continue;
+          *(reinterpret_cast<uint4*>(cache + to) + v) = *reinterpret_cast<const uint4*>(
+              reinterpret_cast<const char*>(s_run) + src + v / BS * (BS * 16));
+        }
+      } else {
+        constexpr int SEG = BS / U, UPB = DG * SEG;  // units of a row and of a block
+        for (int q = tid; q < nb * UPB; q += kThreads) {
+          const int i = uniform(q / UPB), v = q % UPB, row = v / SEG;
+          const int p = (b0 + i) * BS + v % SEG * U;
+          const int64_t at = uniform64(places[b0 + i - to0]);
+          if (at < 0 || p + U <= p0 || p >= p1) continue;
+          E* to = cache + at + v * U;
+          const char* from = reinterpret_cast<const char*>(s_run + row_at(row));
+          const uint32_t* src = s_src + (p - aligned);
+          if (p >= p0 && p + U <= p1 && all_there) {
+            union {
+              uint4 v4;
+              uint2 v2;
+              E e[X];
+            } out;
+#pragma unroll
+            for (int e = 0; e < U; ++e) out.e[e] = *reinterpret_cast<const E*>(from + src[e]);
+            if constexpr (U == X) *reinterpret_cast<uint4*>(to) = out.v4;
+            else *reinterpret_cast<uint2*>(to) = out.v2;
+          } else {
+            for (int e = 0; e < U; ++e)
+              if (p + e >= p0 && p + e < p1 && src[e] != kNone)
+                to[e] = *reinterpret_cast<const E*>(from + src[e]);
+          }
+        }
+      }
+      p0 = p1;
+      flip ^= 1;
+      lds_barrier();  // (LDS is read)
+    };
+    uint4 even[NV], odd[NV];
+    const int first = whole ? c_begin : 0;
+    load_data(even, first);
+    load_data(odd, first + kCols);
+    for (int c0 = first; c0 < n; c0 += 2 * kCols) {
+      batch(even, c0);
+      if (c0 + kCols < n) batch(odd, c0 + kCols);
     }
   }
 }
 
+template <typename E, int BS, int DG, int kThreads, int NV>
+hipError_t move_launch(const EvictArgs& a, const CacheGeom& g, hipStream_t stream) {
+  const int64_t grid = (int64_t)a.num_seqs * g.num_kv_heads * 2 * (g.head_dim / DG);
+  hipLaunchKernelGGL((evict_move_kernel<E, BS, DG, kThreads, NV>), dim3((uint32_t)grid),
+                     dim3(kThreads), 0, stream, a, g.num_kv_heads, g.head_dim, g.num_blocks,
+                     g.block_stride, g.head_stride);
+  return hipGetLastError();
+}
+
+template <typename E, int BS>
+hipError_t move_bs(const EvictArgs& a, const CacheGeom& g, hipStream_t stream) {
+  constexpr int kThin = 16 / (int)sizeof(E) > 8 ? 16 : 8;
+  // groups of 32 dims unless they leave compute units idle: one sequence of 8192
+  // tokens cut to 4096 takes 18 us in groups of 8 (256 workgroups), 64 sequences
+  // of 600 to 4096 cut to 1024 take 197 us in groups of 32, 214 in groups of 8
+  const int64_t wide = (int64_t)a.num_seqs * g.num_kv_heads * 2 * (g.head_dim / 32);
+  return wide >= 1024 ? move_launch<E, BS, 32, 512, 4>(a, g, stream)
+                      : move_launch<E, BS, kThin, 512, 4>(a, g, stream);
+}
+
 template <typename E>
 hipError_t move_typed(const EvictArgs& a, const CacheGeom& g, hipStream_t stream) {
-  constexpr int X = 16 / (int)sizeof(E);
-  const int dims = g.head_dim % 32 == 0 ? 32 : std::max(16, X);
-  const int64_t grid =
-      (int64_t)a.num_seqs * g.num_kv_heads * 2 * (g.head_dim / dims);
-  const auto k = g.block_size == 8    ? evict_move_kernel<E, 8>
-                 : g.block_size == 16 ? evict_move_kernel<E, 16>
-                                      : evict_move_kernel<E, 32>;
-  hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(kMoveThreads), 0, stream, a, g.num_kv_heads,
-                     g.head_dim, dims, g.num_blocks, g.block_stride, g.head_stride);
-  return hipGetLastError();
+  switch (g.block_size) {
+    case 8: return move_bs<E, 8>(a, g, stream);
+    case 16: return move_bs<E, 16>(a, g, stream);
+    case 32: return move_bs<E, 32>(a, g, stream);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-hipError_t launch_evict(int cache_dtype, const EvictArgs& a, const CacheGeom& g,
-                        hipStream_t stream) {
-  hipLaunchKernelGGL(evict_select_kernel, dim3((uint32_t)((int64_t)a.num_seqs * g.num_kv_heads)),
-                     dim3(kSelThreads), 0, stream, a, g.num_kv_heads, g.block_size);
+size_t evict_workspace_bytes(int32_t num_seqs, int32_t num_kv_heads, int32_t max_ctx,
+                             int32_t block_size) {
+  const size_t pairs = (size_t)num_seqs * num_kv_heads;
+  return pairs * ((max_ctx + block_size - 1) / block_size) * sizeof(uint2) +
+         pairs * sizeof(uint32_t);
+}
+
+hipError_t launch_evict(int cache_dtype, const EvictArgs& args, void* workspace,
+                        const CacheGeom& g, hipStream_t stream) {
+  EvictArgs a = args;
+  const int64_t pairs = (int64_t)a.num_seqs * g.num_kv_heads;
+  a.max_columns = (a.max_ctx + g.block_size - 1) / g.block_size;
+  a.columns = static_cast<uint2*>(workspace);
+  a.first_column = reinterpret_cast<uint32_t*>(a.columns + pairs * a.max_columns);
+  const int bs_log2 = __builtin_ctz((unsigned)g.block_size);
+  // 16 scores per thread in registers
+  if (a.max_ctx <= 256 * kItems)
+    hipLaunchKernelGGL(evict_select_kernel<256>, dim3((uint32_t)pairs), dim3(256), 0, stream, a,
+                       g.num_kv_heads, bs_log2);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<1024>, dim3((uint32_t)pairs), dim3(1024), 0, stream, a,
+                       g.num_kv_heads, bs_log2);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (cache_dtype == VPA_DTYPE_F32) return move_typed<uint32_t>(a, g, stream);

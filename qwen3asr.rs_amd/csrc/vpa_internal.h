@@ -353,9 +353,17 @@ struct EvictArgs {
   int32_t budget, keep_first, keep_last;
   uint32_t* new_lens;
   uint32_t* kept;  // [num_seqs, num_kv_heads, budget]
+  // in the workspace: [num_seqs, num_kv_heads, max_columns] of each table column
+  // that a cut sequence's context reaches, the kept tokens {mask, place of the
+  // first}, and [num_seqs, num_kv_heads] the first column that loses one
+  uint2* columns = nullptr;
+  uint32_t* first_column = nullptr;
+  int32_t max_columns = 0;
 };
-hipError_t launch_evict(int cache_dtype, const EvictArgs& a, const CacheGeom& g,
-                        hipStream_t stream);
+size_t evict_workspace_bytes(int32_t num_seqs, int32_t num_kv_heads, int32_t max_ctx,
+                             int32_t block_size);
+hipError_t launch_evict(int cache_dtype, const EvictArgs& args, void* workspace,
+                        const CacheGeom& g, hipStream_t stream);
 
 // Draft verification (verify_kernels.hip).
 struct VerifyArgs {

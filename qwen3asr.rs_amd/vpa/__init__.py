@@ -22,6 +22,7 @@ from .ops import (  # noqa: F401
 )
 from .eviction import (  # noqa: F401
     evict_kv_cache,
+    evict_kv_cache_workspace,
     paged_attention_weights,
     paged_attention_weights_workspace,
 )
@@ -39,6 +40,7 @@ __all__ = [
     "argmax_token_ids_from_logits",
     "cache_geometry",
     "evict_kv_cache",
+    "evict_kv_cache_workspace",
     "gather_kv_cache",
     "paged_attention",
     "paged_attention_plan",

@@ -87,7 +87,8 @@ SIGNATURES = {
         _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _p, _sz, _p]),
     "vpa_evict_kv_cache": (ctypes.c_int, [
         _p, _p, _p, _i64, _i64, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
-        _i32, _i64, _i64, _i64, _i32, _p]),
+        _i32, _i64, _i64, _i64, _i32, _p, _sz, _p]),
+    "vpa_evict_kv_cache_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
     "vpa_verify_draft_tokens_workspace_size": (_sz, [_i32, _i32, _i32]),
     "vpa_verify_draft_tokens": (ctypes.c_int, [
         _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p,

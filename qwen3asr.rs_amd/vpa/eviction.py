@@ -105,12 +105,21 @@ def paged_attention_weights(q: torch.Tensor, key_cache: torch.Tensor,
     return scores
 
 
+def evict_kv_cache_workspace(num_seqs: int, num_kv_heads: int, max_context_len: int,
+                             block_size: int, device) -> Optional[torch.Tensor]:
+    """Caller-side workspace of ``evict_kv_cache`` (None when not needed)."""
+    n = _lib.load().vpa_evict_kv_cache_workspace_size(num_seqs, num_kv_heads, max_context_len,
+                                                      block_size)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
 def evict_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: torch.Tensor,
                    block_tables: torch.Tensor, context_lens: torch.Tensor, budget: int, *,
                    keep_first: int = 0, keep_last: int = 0,
                    max_context_len: Optional[int] = None,
                    new_context_lens: Optional[torch.Tensor] = None,
-                   kept: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                   kept: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Cuts each sequence of more than ``budget`` tokens to ``budget`` per kv head:
     its first ``keep_first``, its last ``keep_last`` and the others with the
     highest ``scores`` [B, KVH, width] (equal ones: the earlier) stay, moved to the
@@ -121,7 +130,7 @@ def evict_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: t
     ceil(new_context_lens / block_size) may then be given back
     (``DeviceBlockAllocator.trim``)."""
     _require_device(key_cache, value_cache, scores, block_tables, context_lens, new_context_lens,
-                    kept)
+                    kept, workspace)
     nb, kvh, d, bs, bstride, hstride = cache_geometry(key_cache, value_cache)
     b = _check_tables(block_tables, context_lens)
     if max_context_len is None:
@@ -139,10 +148,13 @@ def evict_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: t
     block_tables = block_tables.contiguous()
     context_lens = context_lens.contiguous()
     with _on_device_of(scores):
+        if workspace is None:
+            workspace = evict_kv_cache_workspace(b, kvh, int(max_context_len), bs, scores.device)
         check(_lib.load().vpa_evict_kv_cache(
             key_cache.data_ptr(), value_cache.data_ptr(), scores.data_ptr(), seq_stride,
             head_stride, block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(),
             new_context_lens.data_ptr(), kept.data_ptr(), b, int(max_context_len), int(budget),
             int(keep_first), int(keep_last), kvh, d, bs, nb, bstride, hstride,
-            dtype_code(key_cache.dtype), _stream(scores)))
+            dtype_code(key_cache.dtype), _ptr(workspace),
+            0 if workspace is None else workspace.nbytes, _stream(scores)))
     return new_context_lens, kept

@@ -115,10 +115,16 @@ def test_weights_workspace_covers_rows_and_chunks():
 
 EV = dict(kc=P, vc=P, sc=P, ss=8 * 512, sh=512, bt=P, bts=32, cl=P, new=2 * P, kept=P, n=4, mc=500,
           budget=64, first=4, last=8, kvh=8, d=128, bs=16, nb=200, bst=8 * 2048, hst=2048, cdtype=BF16,
-          stream=None)
+          ws=P, wsb=1 << 20, stream=None)
+
+
+def ews_bytes(n, kvh, ctx, bs):
+    return _lib.load().vpa_evict_kv_cache_workspace_size(n, kvh, ctx, bs)
 
 
 @pytest.mark.parametrize("over,code,needle", [
+    (dict(ws=None), WS, "bytes needed"), (dict(wsb=ews_bytes(4, 8, 500, 16) - 1), WS, "bytes needed"),
+    (dict(ws=P + 64), INV, "256-byte"),
     (dict(cdtype=7), UNS, "dtype"), (dict(d=80), UNS, "no kernel"), (dict(n=-1), INV, "num_seqs"),
     (dict(budget=0), INV, "budget"), (dict(budget=-3), INV, "budget"), (dict(first=-1), INV, "budget"),
     (dict(last=-1), INV, "budget"), (dict(first=60, last=5), INV, "budget"),
