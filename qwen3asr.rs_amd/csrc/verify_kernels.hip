@@ -27,6 +27,7 @@
 // first; only where drafts have logits), draw (the segment, then the place in
 // it).
 
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -42,58 +43,66 @@ constexpr int kThreads = 256;
 constexpr int kSeg = 4096;  // logits of a segment: 16 per thread
 constexpr int kPer = kSeg / kThreads;
 constexpr int kMaxDrafts = kVerifyMaxDrafts;
-
-enum Mode : int32_t {
-  kDone = 0,      // the last token is known (greedy)
-  kPlain = 1,     // drawn from the target row
-  kResidual = 2,  // from max(p - q, 0)
-  kExcluded = 3,  // from the target row without the drafted token
-};
-struct Pick {
-  int32_t row;   // accepted drafts, and the target row that is drawn from
-  int32_t mode;
-  float max_p, max_q;
-  uint32_t drafted;  // the rejected draft
-};
+constexpr int kMaxRows = 2 * kMaxDrafts + 1;
+constexpr uint32_t kNone = 0xffffffffu;
 
 struct Buffers {
-  float2* stats;     // [target rows then draft rows][segments] {max, sum}
-  uint32_t* best;    // [target rows][segments] first maximum
-  Pick* picks;       // [num_seqs]
-  double2* sums;     // [num_seqs][segments] of the target row and the draft row
-  double* rest;      // [num_seqs][segments] of what is drawn from
+  // [target rows then draft rows][segments]: maximum, and the sum of weights
+  // against it (greedy: the first maximum's index, as bits)
+  float* max;
+  double* sum;
+  double* rest;  // [num_seqs][segments] of max(p - q, 0)
   int32_t segs;
 };
 
-// e^x for x <= 0 in f64 (0 below -708 and for NaN): x = n ln 2 + r, Taylor sum
-// of e^r to r^13 (|r| <= 0.35: 0.35^14 / 14! < 2^-57).
-__device__ __forceinline__ double exp_nonpos(double x) {
-  if (!(x > -708.0)) return 0.0;
-  const double n = __builtin_rint(x * 1.44269504088896340736);
-  double r = __builtin_fma(n, -0.69314718055994530942, x);
-  r = __builtin_fma(n, -2.3190468138462995584e-17, r);
-  double p = 1.0 / 6227020800.0;
-  p = __builtin_fma(p, r, 1.0 / 479001600.0);
-  p = __builtin_fma(p, r, 1.0 / 39916800.0);
-  p = __builtin_fma(p, r, 1.0 / 3628800.0);
-  p = __builtin_fma(p, r, 1.0 / 362880.0);
-  p = __builtin_fma(p, r, 1.0 / 40320.0);
-  p = __builtin_fma(p, r, 1.0 / 5040.0);
-  p = __builtin_fma(p, r, 1.0 / 720.0);
-  p = __builtin_fma(p, r, 1.0 / 120.0);
-  p = __builtin_fma(p, r, 1.0 / 24.0);
-  p = __builtin_fma(p, r, 1.0 / 6.0);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  return __builtin_bit_cast(double, __builtin_bit_cast(int64_t, p) + ((int64_t)n << 52));
+// 2^t for 0 >= t > -2^31 in f64, 0 below -1074: t = n + f, and for 2^f,
+// |f| <= 1/2, the polynomial 1 + f g(f) with g through the 9 Chebyshev nodes of
+// (2^f - 1) / f: within 4e-14 of the value. A draw among 150 000 tokens then has
+// about one chance in 10^8 to see a border on its wrong side.
+__device__ __forceinline__ double exp2_nonpos(double t) {
+  const double n = __builtin_rint(t);
+  const double f = t - n;
+  double p = 1.02031210633917290e-07;
+  p = __builtin_fma(p, f, 1.32552248786688168e-06);
+  p = __builtin_fma(p, f, 1.52526868462677196e-05);
+  p = __builtin_fma(p, f, 1.54034558524538382e-04);
+  p = __builtin_fma(p, f, 1.33335581790431116e-03);
+  p = __builtin_fma(p, f, 9.61812915940255843e-03);
+  p = __builtin_fma(p, f, 5.55041086647604237e-02);
+  p = __builtin_fma(p, f, 2.40226506958129887e-01);
+  p = __builtin_fma(p, f, 6.93147180559945286e-01);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
 }
-// Weight of a logit l against the maximum m: e^((l - m) / T), 1 at the maximum
+// The weights e^((l - m) / T) of logits l against a maximum m: 1 at the maximum
 // (also an infinite one), 0 for -inf and NaN.
-__device__ __forceinline__ double weight64(float l, float m, double inv_t) {
-  if (l == m) return l == -INFINITY ? 0.0 : 1.0;
-  return exp_nonpos(((double)l - (double)m) * inv_t);
-}
+struct Scale {
+  double c;  // log2 e / T
+  double m64;
+  float m;
+  float floor;  // logits below it, and NaN, count as it: an exponent below every f64
+  bool odd;     // (uniform) the maximum is infinite or the lowest number: only its equals weigh
+  __device__ __forceinline__ Scale(float max, float temp)
+      // (T above 1e30 as 1e30: a masked logit's weight stays 0)
+      : c(fmax(1.44269504088896340736 / (double)temp, 1e-30)),
+        m64((double)max),
+        m(max),
+        floor(fmaxf(fminf(max - 2000.f * temp, below(max)), -FLT_MAX)),
+        odd(!(max > -FLT_MAX && max < INFINITY)) {}
+  // the next number below a finite one
+  static __device__ __forceinline__ float below(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return __uint_as_float(v > 0.f ? u - 1u : v < 0.f ? u + 1u : 0x80000001u);
+  }
+  __device__ __forceinline__ double plain(float l) const {
+    // (the difference first: logits of the lowest value have products whose
+    // rounding alone would be a huge exponent)
+    return exp2_nonpos(((double)fmaxf(l, floor) - m64) * c);
+  }
+  __device__ __forceinline__ double weight(float l) const {
+    return odd ? (l == m && l > -INFINITY ? 1.0 : 0.0) : plain(l);
+  }
+};
 
 __device__ __forceinline__ float seq_temperature(const VerifyArgs& a, int b) {
   return a.temperature == nullptr ? 1.f : a.temperature[b];
@@ -102,6 +111,14 @@ __device__ __forceinline__ int seq_drafts(const VerifyArgs& a, int b) {
   return a.num_drafts == nullptr ? a.max_drafts
                                  : (int)min(a.num_drafts[b], (uint32_t)a.max_drafts);
 }
+template <typename T>
+__device__ __forceinline__ const T* target_row(const VerifyArgs& a, int b, int i) {
+  return static_cast<const T*>(a.target) + b * a.target_seq_stride + i * a.target_row_stride;
+}
+template <typename T>
+__device__ __forceinline__ const T* draft_row(const VerifyArgs& a, int b, int i) {
+  return static_cast<const T*>(a.draft) + b * a.draft_seq_stride + i * a.draft_row_stride;
+}
 
 // The thread's 16 logits of a segment, -inf past the row: vector q = tid + 256 i
 // of the segment, so element e of it is logit seg * 4096 + q * X + e.
@@ -109,12 +126,18 @@ template <typename T>
 __device__ __forceinline__ void load_segment(const T* row, int seg, int vocab, bool vec_ok,
                                              float (&f)[kPer]) {
   constexpr int X = pack_x<T>();
+  uint4 u[kPer / X];
+#pragma unroll
+  for (int i = 0; i < kPer / X; ++i) {
+    const int at = seg * kSeg + ((int)threadIdx.x + kThreads * i) * X;
+    u[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (vec_ok && at + X <= vocab) u[i] = load_stream(reinterpret_cast<const uint4*>(row + at));
+  }
 #pragma unroll
   for (int i = 0; i < kPer / X; ++i) {
     const int at = seg * kSeg + ((int)threadIdx.x + kThreads * i) * X;
     if (vec_ok && at + X <= vocab) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + at);
-      const T* e = reinterpret_cast<const T*>(&u);
+      const T* e = reinterpret_cast<const T*>(&u[i]);
 #pragma unroll
       for (int k = 0; k < X; ++k) f[i * X + k] = load_as_f32(e + k);
     } else {
@@ -130,13 +153,32 @@ __device__ __forceinline__ int segment_index(int seg, int k) {  // logit of f[k]
   return seg * kSeg + ((int)threadIdx.x + kThreads * (k / X)) * X + k % X;
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-  return v;
+template <int kCtrl>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, kCtrl, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), kCtrl, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
-// Sum over the workgroup, in every thread; s4 is free again after the next
-// barrier.
+// Sum over each row of 16 lanes, in every lane of it.
+__device__ __forceinline__ double row16_sum_f64(double v) {
+  v += dpp_f64<kDppQuadXor1>(v);
+  v += dpp_f64<kDppQuadXor2>(v);
+  v += dpp_f64<kDppRowHalfMirror>(v);
+  return v + dpp_f64<kDppRowMirror>(v);
+}
+__device__ __forceinline__ double readlane_f64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v = row16_sum_f64(v);
+  return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
+}
+// Sum over the workgroup's first four waves, in every thread; s4 is free again
+// after the next barrier.
 __device__ __forceinline__ double group_sum_f64(double v, double* s4) {
   v = wave_sum_f64(v);
   if ((threadIdx.x & 63) == 0) s4[threadIdx.x >> 6] = v;
@@ -144,12 +186,21 @@ __device__ __forceinline__ double group_sum_f64(double v, double* s4) {
   return (s4[0] + s4[1]) + (s4[2] + s4[3]);
 }
 
+// (greater value, lower index) over the workgroup
+struct Best {
+  float v;
+  uint32_t i;
+};
+__device__ __forceinline__ void take_best(Best& a, float v, uint32_t i) {
+  if (v > a.v || (v == a.v && i < a.i)) a = {v, i};
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a, Buffers w,
                                                                 bool vec_ok) {
   __shared__ float s_m[4];
   __shared__ uint32_t s_i[4];
-  __shared__ float s_s[4];
+  __shared__ double s_s[4];
   const int rows_t = a.num_seqs * (a.max_drafts + 1);
   const int r = (int)(blockIdx.x / (uint32_t)w.segs);
   const int seg = (int)(blockIdx.x - (uint32_t)r * (uint32_t)w.segs);
@@ -157,383 +208,441 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a, Bu
   const int per = is_target ? a.max_drafts + 1 : a.max_drafts;
   const int rr = is_target ? r : r - rows_t;
   const int b = rr / per, i = rr - b * per;
-  if (i >= seq_drafts(a, b) + (is_target ? 1 : 0)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float temp = seq_temperature(a, b);
   const bool greedy = !(temp > 0.f);
-  if (greedy && !is_target) return;
-  const T* row = is_target ? static_cast<const T*>(a.target) + b * a.target_seq_stride +
-                                 i * a.target_row_stride
-                           : static_cast<const T*>(a.draft) + b * a.draft_seq_stride +
-                                 i * a.draft_row_stride;
+  if (i >= seq_drafts(a, b) + (is_target ? 1 : 0) || (greedy && !is_target)) return;
   float f[kPer];
-  load_segment<T>(row, seg, a.vocab, vec_ok, f);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float mx = -INFINITY;
-  uint32_t at = 0xffffffffu;
+  load_segment<T>(is_target ? target_row<T>(a, b, i) : draft_row<T>(a, b, i), seg, a.vocab, vec_ok,
+                  f);
+  const int64_t at = (int64_t)r * w.segs + seg;
+  if (greedy) {
+    Best best{-INFINITY, kNone};
 #pragma unroll
-  for (int k = 0; k < kPer; ++k)
-    if (f[k] > mx) {  // (indices ascend with k; a NaN is never greater)
-      mx = f[k];
-      at = (uint32_t)segment_index<T>(seg, k);
-    }
+    for (int k = 0; k < kPer; ++k)  // (indices ascend with k; a NaN is never greater)
+      if (f[k] > best.v) best = {f[k], (uint32_t)segment_index<T>(seg, k)};
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const float om = __shfl_xor(mx, m, 64);
-    const uint32_t oi = __shfl_xor(at, m, 64);
-    if (om > mx || (om == mx && oi < at)) {
-      mx = om;
-      at = oi;
+    for (int m = 1; m < 64; m <<= 1)
+      take_best(best, __shfl_xor(best.v, m, 64), __shfl_xor(best.i, m, 64));
+    if (lane == 0) {
+      s_m[wave] = best.v;
+      s_i[wave] = best.i;
     }
-  }
-  if (lane == 0) {
-    s_m[wave] = mx;
-    s_i[wave] = at;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int v = 0; v < 4; ++v)
-    if (s_m[v] > mx || (s_m[v] == mx && s_i[v] < at)) {
-      mx = s_m[v];
-      at = s_i[v];
-    }
-  float sum = 0.f;
-  if (!greedy) {
-    const float c = fminf(1.44269504f / temp, 3.0e38f);  // (finite: 0 * c is 0 at the maximum)
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const float x = (f[k] - mx) * c;
-      const float e = mx == INFINITY ? (f[k] == mx ? 1.f : 0.f) : __builtin_amdgcn_exp2f(x);
-      sum += x == x || mx == INFINITY ? e : 0.f;
-    }
-    sum = wave_sum_dpp(sum);
-    if (lane == 0) s_s[wave] = sum;
     __syncthreads();
-    sum = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
+    if (threadIdx.x == 0) {
+      for (int v = 1; v < 4; ++v) take_best(best, s_m[v], s_i[v]);
+      w.max[at] = best.v;
+      w.sum[at] = __builtin_bit_cast(double, (uint64_t)best.i);
+    }
+    return;
   }
+  float mx = f[0];
+#pragma unroll
+  for (int k = 1; k < kPer; ++k) mx = fmaxf(mx, f[k]);  // (a NaN loses)
+  mx = fmaxf(mx, -INFINITY);
+  mx = wave_max_dpp(mx);
+  if (lane == 0) s_m[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const Scale sc(mx, temp);
+  double s0 = 0.0, s1 = 0.0;
+  if (sc.odd) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s0 += sc.weight(f[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) {
+      s0 += sc.plain(f[k]);
+      s1 += sc.plain(f[k + 1]);
+    }
+  }
+  const double sum = group_sum_f64(s0 + s1, s_s);
   if (threadIdx.x == 0) {
-    w.stats[(int64_t)r * w.segs + seg] = make_float2(mx, sum);
-    if (is_target) w.best[(int64_t)r * w.segs + seg] = at;
+    w.max[at] = mx;
+    w.sum[at] = sum;
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a, Buffers w) {
-  __shared__ float s_max[2 * kMaxDrafts + 1];
-  __shared__ double s_sum[2 * kMaxDrafts + 1];
-  __shared__ uint32_t s_best[kMaxDrafts + 1];
-  const int b = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// What became of a sequence's drafts.
+struct Pick {
+  int took;          // accepted drafts, and the target row that is drawn from
+  bool greedy;       // the last token is `best`, nothing is drawn
+  bool rejected;     // the row's draft was: drawn from what is left of the row without it
+  uint32_t drafted;  // that draft
+  uint32_t best;
+  float max_p, max_q;
+  double sum_p, sum_q;  // totals of the row's weights, and of its draft row's
+};
+struct PickShared {
+  float max[kMaxRows];
+  double sum[kMaxRows];
+  uint32_t best[kMaxDrafts + 1];
+  uint64_t good;
+};
+
+// Merges the segments of the sequence's rows, LPR lanes (16 or 64) a row, and tests
+// its drafts; called by the whole workgroup of kGroup threads, the result in
+// every thread.
+template <typename T, int kGroup, int LPR>
+__device__ __forceinline__ Pick pick_row(const VerifyArgs& a, const Buffers& w, int b,
+                                         PickShared& sh) {
+  constexpr int kHeld = 64 / LPR;  // segments a lane holds: the first 64 are read once
   const int K = a.max_drafts, n = seq_drafts(a, b);
   const float temp = seq_temperature(a, b);
   const bool greedy = !(temp > 0.f);
-  const double inv_t = 1.0 / (double)temp;
-  const int rows = n + 1 + (greedy || a.draft == nullptr ? 0 : n);
-  for (int q = wave; q < rows; q += 4) {  // a wave merges a row's segments
+  const bool have_q = !greedy && a.draft != nullptr;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the drafts' own logits, read ahead of the merge
+  uint32_t x = kNone;
+  float lx = -INFINITY, lq = -INFINITY, au = 0.f;
+  if (wave == 0 && lane < n) {
+    x = a.draft_ids[(int64_t)b * K + lane];
+    if (!greedy && x < (uint32_t)a.vocab) {
+      lx = load_as_f32(target_row<T>(a, b, lane) + x);
+      if (have_q) lq = load_as_f32(draft_row<T>(a, b, lane) + x);
+      au = a.accept_u[(int64_t)b * K + lane];
+    }
+  }
+  const int rows = n + 1 + (have_q ? n : 0);
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += kGroup / LPR) {
+    const int q = r0 + (int)threadIdx.x / LPR, part = (int)threadIdx.x % LPR;
     const bool is_target = q <= n;
-    const int64_t r = is_target ? (int64_t)b * (K + 1) + q
-                                : (int64_t)a.num_seqs * (K + 1) + (int64_t)b * K + (q - n - 1);
-    const float2* st = w.stats + r * w.segs;
-    float mx = -INFINITY;
-    uint32_t at = 0xffffffffu;
-    for (int g = lane; g < w.segs; g += 64) {
-      const float v = st[g].x;
-      const uint32_t i = is_target ? w.best[r * w.segs + g] : 0u;
-      if (v > mx || (v == mx && i < at)) {
-        mx = v;
-        at = i;
-      }
-    }
+    const int64_t at = ((is_target ? (int64_t)b * (K + 1) + q
+                                   : (int64_t)a.num_seqs * (K + 1) + (int64_t)b * K + (q - n - 1))) *
+                       w.segs;
+    const int segs = q < rows ? w.segs : 0;
+    float v[kHeld], mx = -INFINITY;
+    double held[kHeld], sum = 0.0;
+    uint32_t best = kNone;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const float om = __shfl_xor(mx, m, 64);
-      const uint32_t oi = __shfl_xor(at, m, 64);
-      if (om > mx || (om == mx && oi < at)) {
-        mx = om;
-        at = oi;
+    for (int u = 0; u < kHeld; ++u) {
+      const int g = part + LPR * u;
+      v[u] = -INFINITY;
+      held[u] = 0.0;
+      if (g < segs) {
+        v[u] = w.max[at + g];
+        held[u] = w.sum[at + g];
       }
     }
-    double sum = 0.0;
-    if (!greedy)
-      for (int g = lane; g < w.segs; g += 64) sum += (double)st[g].y * weight64(st[g].x, mx, inv_t);
-    sum = wave_sum_f64(sum);
-    if (lane == 0) {
-      s_max[is_target ? q : K + q - n] = mx;
-      s_sum[is_target ? q : K + q - n] = sum;
-      if (is_target) s_best[q] = at;
+    auto take = [&](float value, double stat) {
+      if (greedy) {
+        const uint32_t i = (uint32_t)__builtin_bit_cast(uint64_t, stat);
+        if (value > mx || (value == mx && i < best)) {
+          mx = value;
+          best = i;
+        }
+      } else {
+        mx = fmaxf(mx, value);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (part + LPR * u < segs) take(v[u], held[u]);
+    for (int g = part + 64; g < segs; g += LPR) take(w.max[at + g], greedy ? w.sum[at + g] : 0.0);
+    if (greedy) {
+#pragma unroll
+      for (int m = 1; m < LPR; m <<= 1) {
+        const float om = __shfl_xor(mx, m, 64);
+        const uint32_t oi = __shfl_xor(best, m, 64);
+        if (om > mx || (om == mx && oi < best)) {
+          mx = om;
+          best = oi;
+        }
+      }
+    } else {
+      mx = fmaxf(mx, dpp<kDppQuadXor1>(mx));
+      mx = fmaxf(mx, dpp<kDppQuadXor2>(mx));
+      mx = fmaxf(mx, dpp<kDppRowHalfMirror>(mx));
+      mx = fmaxf(mx, dpp<kDppRowMirror>(mx));
+      if constexpr (LPR == 64)
+        mx = fmaxf(fmaxf(readlane_f(mx, 0), readlane_f(mx, 16)),
+                   fmaxf(readlane_f(mx, 32), readlane_f(mx, 48)));
+      const Scale sc(mx, temp);
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if (v[u] != -INFINITY) sum += held[u] * sc.weight(v[u]);
+      for (int g = part + 64; g < segs; g += LPR) {
+        const float value = w.max[at + g];
+        if (value != -INFINITY) sum += w.sum[at + g] * sc.weight(value);
+      }
+      sum = row16_sum_f64(sum);
+      if constexpr (LPR == 64)
+        sum = (readlane_f64(sum, 0) + readlane_f64(sum, 16)) +
+              (readlane_f64(sum, 32) + readlane_f64(sum, 48));
+    }
+    if (q < rows && part == 0) {
+      sh.max[q] = mx;
+      sh.sum[q] = sum;
+      if (is_target) sh.best[q] = best;
     }
   }
   __syncthreads();
-  if (wave != 0) return;
-  // lane i tests draft i
-  bool good = false;
-  uint32_t x = 0xffffffffu;
-  if (lane < n) {
-    x = a.draft_ids[(int64_t)b * K + lane];
-    if (greedy) {
-      good = s_best[lane] == x;
-    } else if (x < (uint32_t)a.vocab) {
-      const T* tr = static_cast<const T*>(a.target) + b * a.target_seq_stride +
-                    lane * a.target_row_stride;
-      const double px = weight64(load_as_f32(tr + x), s_max[lane], inv_t) / s_sum[lane];
-      double qx = 1.0;
-      if (a.draft != nullptr) {
-        const T* dr = static_cast<const T*>(a.draft) + b * a.draft_seq_stride +
-                      lane * a.draft_row_stride;
-        const double sum = s_sum[K + 1 + lane];  // 0: no logit with any weight
-        qx = sum > 0.0 ? weight64(load_as_f32(dr + x), s_max[K + 1 + lane], inv_t) / sum : 0.0;
+  if (wave == 0) {  // lane i tests draft i
+    bool good = false;
+    if (lane < n) {
+      if (greedy) {
+        good = sh.best[lane] == x;
+      } else if (x < (uint32_t)a.vocab) {
+        const double px = Scale(sh.max[lane], temp).weight(lx) / sh.sum[lane];
+        double qx = 1.0;
+        if (have_q) {
+          const double sum = sh.sum[n + 1 + lane];  // 0: no logit with any weight
+          qx = sum > 0.0 ? Scale(sh.max[n + 1 + lane], temp).weight(lq) / sum : 0.0;
+        }
+        good = (double)au * qx < px;
       }
-      good = (double)a.accept_u[(int64_t)b * K + lane] * qx < px;
     }
+    const uint64_t mask = __ballot(good);
+    if (lane == 0) sh.good = mask;
   }
-  const uint64_t mask = __ballot(good);
-  const int took = ~mask == 0 ? 64 : __builtin_ctzll(~mask);  // at most n
-  uint32_t* out = a.out_ids + (int64_t)b * (K + 1);
-  for (int i = lane; i <= K; i += 64) {
-    const uint32_t id = i < took ? a.draft_ids[(int64_t)b * K + i] : 0xffffffffu;
-    if (i != took) out[i] = id;
-  }
-  if (lane != 0) return;
-  a.out_count[b] = (uint32_t)took + 1u;
+  __syncthreads();
   Pick p;
-  p.row = took;
-  p.max_p = s_max[took];
-  p.max_q = 0.f;
-  p.drafted = 0xffffffffu;
-  p.mode = kPlain;
-  if (greedy) {
-    p.mode = kDone;
-    const uint32_t id = s_best[took];
-    out[took] = id == 0xffffffffu ? 0u : id;  // a row with no number: 0, as the argmax gives
-  } else if (took < n) {
-    p.drafted = a.draft_ids[(int64_t)b * K + took];
-    p.mode = a.draft == nullptr ? kExcluded : kResidual;
-    if (a.draft != nullptr) p.max_q = s_max[K + 1 + took];
-  }
-  w.picks[b] = p;
+  p.took = ~sh.good == 0 ? 64 : __builtin_ctzll(~sh.good);  // at most n
+  p.greedy = greedy;
+  p.rejected = p.took < n;
+  p.drafted = p.rejected ? a.draft_ids[(int64_t)b * K + p.took] : kNone;
+  p.best = sh.best[p.took];
+  p.max_p = sh.max[p.took];
+  p.sum_p = sh.sum[p.took];
+  const int q = p.rejected && have_q ? n + 1 + p.took : p.took;
+  p.max_q = sh.max[q];
+  p.sum_q = sh.sum[q];
+  return p;
 }
 
-// The row a sequence draws from, and its draft row.
-template <typename T>
-__device__ __forceinline__ const T* picked_target(const VerifyArgs& a, int b, const Pick& p) {
-  return static_cast<const T*>(a.target) + b * a.target_seq_stride + p.row * a.target_row_stride;
-}
-template <typename T>
-__device__ __forceinline__ const T* picked_draft(const VerifyArgs& a, int b, const Pick& p) {
-  return static_cast<const T*>(a.draft) + b * a.draft_seq_stride + p.row * a.draft_row_stride;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Buffers w,
-                                                               bool vec_ok) {
-  __shared__ double s4[2][4];
-  const int seg = blockIdx.x, b = blockIdx.y;
-  const Pick p = w.picks[b];
-  if (p.mode == kDone) return;
-  const double inv_t = 1.0 / (double)seq_temperature(a, b);
-  float f[kPer];
-  load_segment<T>(picked_target<T>(a, b, p), seg, a.vocab, vec_ok, f);
-  double sp = 0.0, sq = 0.0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k)
-    if (p.mode != kExcluded || (uint32_t)segment_index<T>(seg, k) != p.drafted)
-      sp += weight64(f[k], p.max_p, inv_t);
-  sp = group_sum_f64(sp, s4[0]);
-  if (p.mode == kResidual) {
-    load_segment<T>(picked_draft<T>(a, b, p), seg, a.vocab, vec_ok, f);
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) sq += weight64(f[k], p.max_q, inv_t);
-    sq = group_sum_f64(sq, s4[1]);
-  }
-  if (threadIdx.x == 0) {
-    w.sums[(int64_t)b * w.segs + seg] = make_double2(sp, sq);
-    w.rest[(int64_t)b * w.segs + seg] = sp;  // what is drawn from, but for kResidual
-  }
-}
-
-// Totals over the segments of a sequence, in a fixed order, in every thread.
-__device__ __forceinline__ double2 total_sums(const Buffers& w, int b, double (*s4)[4]) {
-  double sp = 0.0, sq = 0.0;
-  for (int g = threadIdx.x; g < w.segs; g += kThreads) {
-    const double2 v = w.sums[(int64_t)b * w.segs + g];
-    sp += v.x;
-    sq += v.y;
-  }
-  const double tp = group_sum_f64(sp, s4[0]);
-  return make_double2(tp, group_sum_f64(sq, s4[1]));
-}
-
-// What logit (l of the target, d of the draft) weighs in max(p - q, 0). Both
+// What a logit (l of the target, d of the draft) weighs in max(p - q, 0). Both
 // products are rounded (not fused into the difference), so that equal
 // probabilities leave exactly 0.
-__device__ __forceinline__ double residual(float l, float d, const Pick& p, double inv_t,
-                                           double inv_p, double inv_q) {
+__device__ __forceinline__ double residual(double wp, double wq, double inv_p, double inv_q) {
 #pragma clang fp contract(off)
-  const double r = weight64(l, p.max_p, inv_t) * inv_p - weight64(d, p.max_q, inv_t) * inv_q;
+  const double r = wp * inv_p - wq * inv_q;
   return r > 0.0 ? r : 0.0;
 }
+__device__ __forceinline__ double inverse(double sum) { return sum > 0.0 ? 1.0 / sum : 0.0; }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a, Buffers w,
                                                                bool vec_ok) {
-  __shared__ double s4[3][4];
+  __shared__ PickShared sh;
+  __shared__ double s4[4];
   const int seg = blockIdx.x, b = blockIdx.y;
-  const Pick p = w.picks[b];
-  if (p.mode != kResidual) return;
-  const double inv_t = 1.0 / (double)seq_temperature(a, b);
+  const Pick p = pick_row<T, kThreads, 16>(a, w, b, sh);
+  if (p.greedy || !p.rejected) return;
+  const float temp = seq_temperature(a, b);
   float f[kPer], d[kPer];
-  load_segment<T>(picked_target<T>(a, b, p), seg, a.vocab, vec_ok, f);
-  load_segment<T>(picked_draft<T>(a, b, p), seg, a.vocab, vec_ok, d);
-  const double2 t = total_sums(w, b, s4);
-  const double inv_p = t.x > 0.0 ? 1.0 / t.x : 0.0, inv_q = t.y > 0.0 ? 1.0 / t.y : 0.0;
+  load_segment<T>(target_row<T>(a, b, p.took), seg, a.vocab, vec_ok, f);
+  load_segment<T>(draft_row<T>(a, b, p.took), seg, a.vocab, vec_ok, d);
+  const Scale sp(p.max_p, temp), sq(p.max_q, temp);
+  const double inv_p = inverse(p.sum_p), inv_q = inverse(p.sum_q);
   double r = 0.0;
+  if (sp.odd || sq.odd) {
+#pragma unroll 1
+    for (int k = 0; k < kPer; ++k)
+      r += residual(sp.weight(f[k]), sq.weight(d[k]), inv_p, inv_q);
+  } else {
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) r += residual(f[k], d[k], p, inv_t, inv_p, inv_q);
-  r = group_sum_f64(r, s4[2]);
+    for (int k = 0; k < kPer; ++k)
+      r += residual(sp.plain(f[k]), sq.plain(d[k]), inv_p, inv_q);
+  }
+  r = group_sum_f64(r, s4);
   if (threadIdx.x == 0) w.rest[(int64_t)b * w.segs + seg] = r;
 }
 
+constexpr int kDrawThreads = 1024;
+constexpr int kDrawWaves = kDrawThreads / 64;
+
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double dpp_add_f64(double v) {  // 0 from lanes that are not there
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, kRows, 0xf, kRows == 0xf);
+  const uint32_t hi =
+      __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, kRows, 0xf, kRows == 0xf);
+  return v + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 // Inclusive prefix sum over the workgroup's threads in their order.
-__device__ __forceinline__ double group_scan_f64(double v, double* s4, double& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double o = __shfl_up(v, m, 64);
-    if (lane >= m) v += o;
-  }
-  if (lane == 63) s4[wave] = v;
+__device__ __forceinline__ double group_scan_f64(double v, double* s_w, double& total) {
+  const int wave = threadIdx.x >> 6;
+  v = dpp_add_f64<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v = dpp_add_f64<0x112, 0xf>(v);
+  v = dpp_add_f64<0x114, 0xf>(v);
+  v = dpp_add_f64<0x118, 0xf>(v);
+  v = dpp_add_f64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3, :31 into 2 and 3
+  v = dpp_add_f64<0x143, 0xc>(v);
+  if ((threadIdx.x & 63) == 63) s_w[wave] = v;
   __syncthreads();
   double before = 0.0;
+  total = 0.0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) before += i < wave ? s4[i] : 0.0;
-  total = ((s4[0] + s4[1]) + s4[2]) + s4[3];
+  for (int i = 0; i < kDrawWaves; ++i) {
+    before += i < wave ? s_w[i] : 0.0;
+    total += s_w[i];
+  }
   return before + v;
 }
-
-// First thread-ordered place of the workgroup where a value in `mine` is set
-// (kNone where no thread has one): minimum over threads.
-__device__ __forceinline__ uint32_t group_min(uint32_t v, uint32_t* s) {
+// The lowest `first` and the highest `last` (kNone: none; last counted from 1) of
+// the workgroup.
+__device__ __forceinline__ void group_first_last(uint32_t& first, uint32_t& last, uint2* s_w) {
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v = min(v, (uint32_t)__shfl_xor(v, m, 64));
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  for (int m = 1; m < 64; m <<= 1) {
+    first = min(first, (uint32_t)__shfl_xor(first, m, 64));
+    last = max(last, (uint32_t)__shfl_xor(last, m, 64));
+  }
+  if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = make_uint2(first, last);
   __syncthreads();
-  return min(min(s[0], s[1]), min(s[2], s[3]));
+#pragma unroll
+  for (int i = 0; i < kDrawWaves; ++i) {
+    first = min(first, s_w[i].x);
+    last = max(last, s_w[i].y);
+  }
+}
+
+// Four logits from `at` on, -inf past the row.
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, int at, int vocab, bool vec_ok, float (&f)[4]) {
+  if (vec_ok && at + 4 <= vocab) {
+    uint32_t u[4];
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(row + at);
+    else *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(row + at);
+    const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = load_as_f32(e + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = at + k < vocab ? load_as_f32(row + at + k) : -INFINITY;
+  }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a, Buffers w) {
-  __shared__ double s4[6][4];
-  __shared__ uint32_t s_u[4][4];
-  __shared__ double s_target, s_before;
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a, Buffers w,
+                                                                   bool vec_ok) {
+  static_assert(kSeg == 4 * kDrawThreads, "four logits a thread");
+  __shared__ PickShared sh;
+  __shared__ double s_w[4][kDrawWaves];
+  __shared__ uint2 s_u[2][kDrawWaves];
+  __shared__ double s_before;
   __shared__ int s_seg;
-  constexpr uint32_t kNone = 0xffffffffu;
   const int b = blockIdx.x, tid = threadIdx.x;
-  Pick p = w.picks[b];
-  if (p.mode == kDone) return;
-  uint32_t* out = a.out_ids + (int64_t)b * (a.max_drafts + 1) + p.row;
-  const double inv_t = 1.0 / (double)seq_temperature(a, b);
-  const double2 t = total_sums(w, b, s4);
-  // the segments' sums, scanned in order by chunks of 256 of them
-  double rest_total = 0.0;
-  for (int g = tid; g < w.segs; g += kThreads) rest_total += w.rest[(int64_t)b * w.segs + g];
-  rest_total = group_sum_f64(rest_total, s4[2]);
-  const bool fall_back = p.mode == kResidual && !(rest_total > 0.0);
-  // p equals q (every difference rounds to nothing): draw from p
-  if (fall_back) p.mode = kPlain;
-  const double total = fall_back ? t.x : rest_total;
-  if (!(total > 0.0)) {  // no logit with any weight, or only the drafted one
-    if (tid == 0)
-      *out = p.mode == kExcluded && p.drafted < (uint32_t)a.vocab &&
-                     weight64(load_as_f32(picked_target<T>(a, b, p) + p.drafted), p.max_p, inv_t) > 0.0
-                 ? p.drafted
-                 : 0u;
+  const int K = a.max_drafts;
+  const Pick p = pick_row<T, kDrawThreads, 64>(a, w, b, sh);
+  uint32_t* out = a.out_ids + (int64_t)b * (K + 1);
+  for (int i = tid; i <= K; i += kDrawThreads)
+    if (i != p.took) out[i] = i < p.took ? a.draft_ids[(int64_t)b * K + i] : kNone;
+  if (tid == 0) a.out_count[b] = (uint32_t)p.took + 1u;
+  out += p.took;
+  if (p.greedy) {  // a row with no number: 0, as the argmax gives
+    if (tid == 0) *out = p.best == kNone ? 0u : p.best;
     return;
   }
-  const double target = (double)a.sample_u[b] * total;
-  // the segment: the first whose running sum passes the target; each thread
-  // has a run of segments
-  {
-    const int per = (w.segs + kThreads - 1) / kThreads;
-    const int g0 = min(tid * per, w.segs), g1 = min(g0 + per, w.segs);
-    auto seg_sum = [&](int g) {
-      const int64_t at = (int64_t)b * w.segs + g;
-      return fall_back ? w.sums[at].x : w.rest[at];
-    };
-    double mine = 0.0;
-    for (int g = g0; g < g1; ++g) mine += seg_sum(g);
-    double all;
-    const double upto = group_scan_f64(mine, s4[4], all);
-    const uint32_t first = group_min(mine > 0.0 && upto > target ? (uint32_t)tid : kNone, s_u[2]);
-    const uint32_t last = kNone - group_min(mine > 0.0 ? kNone - (uint32_t)tid : kNone, s_u[3]);
-    if ((uint32_t)tid == (first != kNone ? first : last)) {  // (rounding: the last with any weight)
-      double run = upto - mine, start = run;
-      int found = g0;
-      for (int g = g0; g < g1; ++g) {
-        const double v = seg_sum(g);
-        if (v > 0.0) {
-          found = g;
-          start = run;
-        }
-        run += v;
-        if (run > target) break;
-      }
-      s_seg = found;
-      s_before = start;
-      s_target = target;
+  const float temp = seq_temperature(a, b);
+  const Scale sp(p.max_p, temp), sq(p.max_q, temp);
+  const double inv_p = inverse(p.sum_p), inv_q = inverse(p.sum_q);
+  const T* rt = target_row<T>(a, b, p.took);
+  // drawn from the residual; or, of a drafter without logits, from the row without
+  // the draft; or from the whole row
+  bool residuals = p.rejected && a.draft != nullptr;
+  const int without = p.rejected && a.draft == nullptr && p.drafted < (uint32_t)a.vocab
+                          ? (int)p.drafted
+                          : -1;
+  const T* rd = residuals ? draft_row<T>(a, b, p.took) : rt;
+  float f[4], d[4] = {};
+  double r[4];
+  // the weights drawn from of the thread's four logits of segment seg, their sum
+  auto weigh = [&](int seg) {
+    const int at = seg * kSeg + tid * 4;
+    load4<T>(rt, at, a.vocab, vec_ok, f);
+    if (residuals) load4<T>(rd, at, a.vocab, vec_ok, d);
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      r[k] = at + k == without ? 0.0 : sp.weight(f[k]);
+      if (residuals) r[k] = residual(r[k], sq.weight(d[k]), inv_p, inv_q);
+      sum += r[k];
     }
+    return sum;
+  };
+  // the drafted token's segment without it (summed again: a difference would keep
+  // the rounding of its sum)
+  double rest_of_draft = 0.0;
+  if (without >= 0) {
+    double all;
+    group_scan_f64(weigh(without / kSeg), s_w[0], all);
+    rest_of_draft = all;
+  }
+  const int per = (w.segs + kDrawThreads - 1) / kDrawThreads;
+  const int g0 = min(tid * per, w.segs), g1 = min(g0 + per, w.segs);
+  const int64_t row_at = ((int64_t)b * (K + 1) + p.took) * w.segs;
+  auto segment_sum = [&](int g) {
+    if (residuals) return w.rest[(int64_t)b * w.segs + g];
+    if (without >= 0 && g == without / kSeg) return rest_of_draft;
+    const float m = w.max[row_at + g];
+    return m == -INFINITY ? 0.0 : w.sum[row_at + g] * sp.weight(m);
+  };
+  double mine, upto, total;
+#pragma unroll 1
+  for (int round = 1;; ++round) {
+    mine = 0.0;
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) mine += segment_sum(g);
+    upto = group_scan_f64(mine, s_w[round], total);
+    if (!residuals || total > 0.0) break;
+    residuals = false;  // p equals q: drawn from p
+  }
+  if (!(total > 0.0)) {  // no logit with any weight, or only the drafted one
+    if (tid == 0)
+      *out = without >= 0 && sp.weight(load_as_f32(rt + without)) > 0.0 ? (uint32_t)without : 0u;
+    return;
+  }
+  // the segment: the first whose running sum passes the target
+  const double target = (double)a.sample_u[b] * total;
+  uint32_t first = mine > 0.0 && upto > target ? (uint32_t)tid : kNone;
+  uint32_t last = mine > 0.0 ? (uint32_t)tid + 1u : 0u;
+  group_first_last(first, last, s_u[0]);
+  if ((uint32_t)tid == (first != kNone ? first : last - 1u)) {  // (rounding: the last with any weight)
+    double run = upto - mine, start = run;
+    int found = g0;
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) {
+      const double v = per == 1 ? mine : segment_sum(g);
+      if (v > 0.0) {
+        found = g;
+        start = run;
+      }
+      run += v;
+      if (run > target) break;
+    }
+    s_seg = found;
+    s_before = start;
   }
   __syncthreads();
-  const int seg = s_seg;
-  const double inv_p = t.x > 0.0 ? 1.0 / t.x : 0.0, inv_q = t.y > 0.0 ? 1.0 / t.y : 0.0;
-  const T* rt = picked_target<T>(a, b, p);
-  const T* rd = p.mode == kResidual ? picked_draft<T>(a, b, p) : nullptr;
-  // 16 consecutive logits per thread
-  const int at = seg * kSeg + tid * kPer;
-  double r[kPer], sum = 0.0;
+  // the place in it
+  const int at = s_seg * kSeg + tid * 4;
+  const double sum = weigh(s_seg);
+  upto = group_scan_f64(sum, s_w[3], total) - sum + s_before;
+  first = kNone;
+  last = 0;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    r[k] = 0.0;
-    if (at + k < a.vocab) {
-      const float l = load_as_f32(rt + at + k);
-      if (p.mode == kResidual)
-        r[k] = residual(l, load_as_f32(rd + at + k), p, inv_t, inv_p, inv_q);
-      else if (p.mode == kPlain || (uint32_t)(at + k) != p.drafted)
-        r[k] = weight64(l, p.max_p, inv_t);
-    }
-    sum += r[k];
-  }
-  double seg_total;
-  double upto = group_scan_f64(sum, s4[3], seg_total) - sum + s_before;
-  uint32_t first = kNone, last = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
+  for (int k = 0; k < 4; ++k) {
     upto += r[k];
-    if (first == kNone && r[k] > 0.0 && upto > s_target) first = (uint32_t)(at + k);
+    if (first == kNone && r[k] > 0.0 && upto > target) first = (uint32_t)(at + k);
     if (r[k] > 0.0) last = (uint32_t)(at + k) + 1u;  // 0: none
   }
-  first = group_min(first, s_u[0]);
-  last = kNone - group_min(kNone - last, s_u[1]);
+  group_first_last(first, last, s_u[1]);
   if (tid == 0) *out = first != kNone ? first : last - 1u;
 }
 
 struct Sizes {
   int32_t segs;
-  size_t best_at, picks_at, sums_at, rest_at, bytes;
+  size_t max_at, rest_at, bytes;
 };
 Sizes sizes(int32_t num_seqs, int32_t max_drafts, int32_t vocab) {
   Sizes z;
   z.segs = (vocab + kSeg - 1) / kSeg;
-  const size_t t = (size_t)num_seqs * (max_drafts + 1), d = (size_t)num_seqs * max_drafts;
+  const size_t rows = (size_t)num_seqs * (2 * max_drafts + 1);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  size_t at = up((t + d) * z.segs * sizeof(float2));
-  z.best_at = at;
-  at += up(t * z.segs * sizeof(uint32_t));
-  z.picks_at = at;
-  at += up((size_t)num_seqs * sizeof(Pick));
-  z.sums_at = at;
-  at += up((size_t)num_seqs * z.segs * sizeof(double2));
-  z.rest_at = at;
-  at += up((size_t)num_seqs * z.segs * sizeof(double));
-  z.bytes = at;
+  z.rest_at = up(rows * z.segs * sizeof(double));
+  z.max_at = z.rest_at + up((size_t)num_seqs * z.segs * sizeof(double));
+  z.bytes = z.max_at + up(rows * z.segs * sizeof(float));
   return z;
 }
 
@@ -542,11 +651,9 @@ hipError_t verify_typed(const VerifyArgs& a, hipStream_t stream) {
   const Sizes z = sizes(a.num_seqs, a.max_drafts, a.vocab);
   char* base = static_cast<char*>(a.workspace);
   Buffers w;
-  w.stats = reinterpret_cast<float2*>(base);
-  w.best = reinterpret_cast<uint32_t*>(base + z.best_at);
-  w.picks = reinterpret_cast<Pick*>(base + z.picks_at);
-  w.sums = reinterpret_cast<double2*>(base + z.sums_at);
+  w.sum = reinterpret_cast<double*>(base);
   w.rest = reinterpret_cast<double*>(base + z.rest_at);
+  w.max = reinterpret_cast<float*>(base + z.max_at);
   w.segs = z.segs;
   auto whole = [](const void* p, int64_t s, int64_t r) {
     return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 &&
@@ -555,16 +662,13 @@ hipError_t verify_typed(const VerifyArgs& a, hipStream_t stream) {
   const bool vec_ok = whole(a.target, a.target_seq_stride, a.target_row_stride) &&
                       whole(a.draft, a.draft_seq_stride, a.draft_row_stride);
   const int rows = a.num_seqs * (a.max_drafts + 1) + (a.draft == nullptr ? 0 : a.num_seqs * a.max_drafts);
-  const dim3 per_seg((uint32_t)z.segs, (uint32_t)a.num_seqs);
   hipLaunchKernelGGL(verify_stats_kernel<T>, dim3((uint32_t)z.segs * (uint32_t)rows),
                      dim3(kThreads), 0, stream, a, w, vec_ok);
-  hipLaunchKernelGGL(verify_pick_kernel<T>, dim3((uint32_t)a.num_seqs), dim3(kThreads), 0, stream, a,
-                     w);
-  hipLaunchKernelGGL(verify_sums_kernel<T>, per_seg, dim3(kThreads), 0, stream, a, w, vec_ok);
   if (a.draft != nullptr)
-    hipLaunchKernelGGL(verify_rest_kernel<T>, per_seg, dim3(kThreads), 0, stream, a, w, vec_ok);
-  hipLaunchKernelGGL(verify_draw_kernel<T>, dim3((uint32_t)a.num_seqs), dim3(kThreads), 0, stream, a,
-                     w);
+    hipLaunchKernelGGL(verify_rest_kernel<T>, dim3((uint32_t)z.segs, (uint32_t)a.num_seqs),
+                       dim3(kThreads), 0, stream, a, w, vec_ok);
+  hipLaunchKernelGGL(verify_draw_kernel<T>, dim3((uint32_t)a.num_seqs), dim3(kDrawThreads), 0,
+                     stream, a, w, vec_ok);
   return hipGetLastError();
 }
 
