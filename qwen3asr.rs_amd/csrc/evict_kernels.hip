@@ -246,15 +246,6 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
   for (int t = a.budget + tid; t < L; t += kThreads) score[t] = 0.f;
 }
 
-// Workgroup barrier for data exchanged through LDS: the wave's global loads and
-// stores stay in flight across it.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // One workgroup per (sequence, kv head, K or V, group of DG dims): DG dims of a
 // cache block are one run of DG * BS elements in the key tile (whole chunks) and
 // in the value tile (whole rows) alike. The workgroup walks the table's columns in
@@ -399,7 +390,7 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
         }
         if (c == c_last && off == 0) s_p1 = (int)col.y + __builtin_popcount(col.x);
       }
-      lds_barrier();  // the batch is read and lies in LDS
+      lds_group_barrier();  // the batch is read and lies in LDS
       const int p1 = s_p1;
       const bool all_there = s_absent[flip] == 0;
       load_data(u, c0 + 2 * kCols);
@@ -444,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
       }
       p0 = p1;
       flip ^= 1;
-      lds_barrier();  // (LDS is read)
+      lds_group_barrier();  // (LDS is read)
     };
     uint4 even[NV], odd[NV];
     const int first = whole ? c_begin : 0;

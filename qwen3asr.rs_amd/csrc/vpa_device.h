@@ -324,6 +324,15 @@ __device__ __forceinline__ void lds_wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Workgroup barrier for data exchanged through LDS: waits for this wave's LDS
+// operations only, its global loads and stores stay in flight across it.
+__device__ __forceinline__ void lds_group_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // 16-byte load of streamed data (read once): the non-temporal form, which
 // keeps it from displacing cached lines (measured on MI355X: a flat
 // streaming read reaches 6.96 TB/s with it, 6.23 TB/s with plain loads).
