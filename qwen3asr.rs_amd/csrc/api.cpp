@@ -1022,12 +1022,26 @@ int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
   if (max_context_len > (1 << 28))
     return fail(VPA_ERR_UNSUPPORTED, "%s: max_context_len=%d exceeds %d", op, max_context_len,
                 1 << 28);
+  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
+                    cache_head_stride};
+  const WeightsArgs w{query, key_cache, k_scale, block_tables, block_table_stride, cu_seqlens_q,
+                      context_lens, softmax_scale, causal, num_seqs, max_query_len,
+                      max_context_len, total_query_rows, num_heads, scores, score_seq_stride,
+                      score_head_stride, workspace};
   {
-    const int64_t chunks = ((int64_t)max_context_len + kWeightsChunk - 1) / kWeightsChunk;
-    const int64_t row_groups = ((int64_t)max_query_len * (num_heads / num_kv_heads) + 15) / 16;
+    const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
+    const int64_t rows = (int64_t)max_query_len * (num_heads / num_kv_heads);
     // (256-lane workgroups: the grid's lane count must fit in 32 bits)
-    if (row_groups > 0xffffff || chunks * row_groups > 0xffffff / num_kv_heads)
-      return fail(VPA_ERR_UNSUPPORTED, "%s: too many rows and tokens for one launch", op);
+    bool fits = pairs <= 0xffffff && rows <= 0xfffff;
+    if (fits) {
+      const WeightsPlan p = weights_plan(dtype, w, g);
+      fits = p.first_grid <= 0xffffff && p.second_grid <= 0xffffff;
+    }
+    if (!fits)
+      return fail(VPA_ERR_UNSUPPORTED,
+                  "%s: num_seqs=%d, num_kv_heads=%d, max_query_len=%d and max_context_len=%d are "
+                  "too many rows and tokens for one launch",
+                  op, num_seqs, num_kv_heads, max_query_len, max_context_len);
   }
   if (scores == nullptr || query == nullptr || block_tables == nullptr || context_lens == nullptr)
     return fail(VPA_ERR_INVALID_ARGUMENT,
@@ -1048,12 +1062,6 @@ int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", op);
-  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
-                    cache_head_stride};
-  const WeightsArgs w{query, key_cache, k_scale, block_tables, block_table_stride, cu_seqlens_q,
-                      context_lens, softmax_scale, causal, num_seqs, max_query_len,
-                      max_context_len, total_query_rows, num_heads, scores, score_seq_stride,
-                      score_head_stride, workspace};
   return hip_status(op, launch_attention_weights(dtype, cache_dtype, w, g,
                                                  static_cast<hipStream_t>(stream)));
 }

@@ -316,8 +316,8 @@ hipError_t launch_rotary_cache(int dtype, int cache_dtype, const RotaryRows& a,
                                hipStream_t stream);
 
 // Attention weights of cached tokens (weights_kernels.hip). The workspace
-// holds every row's logits and, per chunk of kWeightsChunk tokens, its
-// maximum and sum.
+// holds, per row and chunk of at least kWeightsChunk tokens, the maximum and sum
+// of the row's logits, and the logits of few rows in front of them.
 constexpr int kWeightsChunk = 256;
 struct WeightsArgs {
   const void* query;
@@ -336,6 +336,15 @@ struct WeightsArgs {
   int64_t score_seq_stride, score_head_stride;
   void* workspace;
 };
+struct WeightsPlan {
+  bool few;    // at most 16 rows per (sequence, kv head): their logits are kept
+  bool whole;  // in LDS, of whole contexts, in one launch
+  int32_t lds_logits;
+  int32_t chunk_tokens, max_chunks, ctx_pad;
+  size_t stats_at;
+  int64_t first_grid, second_grid;  // workgroups
+};
+WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g);
 size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx);
 hipError_t launch_attention_weights(int dtype, int cache_dtype, const WeightsArgs& a,
                                     const CacheGeom& g, hipStream_t stream);

@@ -6,14 +6,18 @@
 // up to its own place at the context's end). A cache is cut by these sums
 // (evict_kernels.hip).
 //
-// A weight needs its row's maximum and sum over the whole context, so the
-// keys' logits are formed once and kept: a pass over the keys writes the
-// logits (f32, log2 units) and per chunk of 256 tokens the row's maximum and
-// sum, then a pass over the logits merges the chunks' pairs and adds the
-// weights up, each score by one thread in a fixed order. A logit costs 8 bytes
-// of traffic per query head against the token's D-element key row, read once:
-// 6 % at two query heads per kv head and D = 128 in 16 bits. Reading the keys a
-// second time instead would cost 100 %.
+// A weight needs its row's maximum and sum over the whole context, so every logit is
+// needed twice. Three forms, by the rows a (sequence, kv head) has at most (a row
+// being one query head of one new token) and the number of these pairs:
+//   * up to 16 rows, contexts whose logits fit 64 KiB of LDS, 512 pairs or more: one
+//     launch, a workgroup per pair, the logits kept in LDS (weight_logits_kernel, whole);
+//   * up to 16 rows otherwise: a pass over the keys writes the logits (f32, log2 units)
+//     and per chunk the row's maximum and sum, a pass over the logits joins the chunks'
+//     pairs and adds the weights up. A logit costs 8 bytes of traffic per row against
+//     the token's key row, read once: 6 % at two rows and D = 128 in 16 bits;
+//   * more rows: both passes read the keys (mostly from the last-level cache the second
+//     time) and form the logits, 16 rows at a time from registers (weight_rows_kernel).
+// Each score is added to by one thread in a fixed order.
 //
 // The key tile [D/x][block][x] of 16 tokens is, vector for vector, the B operand
 // of the 16-row matrix instructions: lane l holds token l % 16 and the x dims of
@@ -21,8 +25,13 @@
 // cores with no shuffle and no LDS; the query rows (a row being one query head of
 // one new token, 16 of one kv head per workgroup) are the A operand, loaded in
 // the same order of dims. f32 keys take v_mfma_f32_16x16x4_f32 in the same way.
-// Bound by the bytes of the keys.
+// Bound by the bytes of the keys, with many rows also by the vector instructions of
+// their exponentials and reductions. Measured in 16 bits at 16 query and 8 kv heads of
+// 128: 256 sequences of 16 to 4096 tokens (424 MB of keys), one row each, 76 us = 5.6
+// TB/s; 8 sequences of 1000 to 6000 tokens (57 MB), 32 rows each, 38 us (19 per pass;
+// 78 with stored logits); one sequence of 1500 tokens, 5.4 + 4.3 us.
 
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -34,7 +43,6 @@
 namespace vpa {
 namespace {
 
-constexpr int kChunk = kWeightsChunk;  // tokens of a workgroup, 64 per wave
 constexpr int kThreads = 256;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -93,297 +101,733 @@ __device__ __forceinline__ int seq_len(const WeightsArgs& a, int s, int bs) {
                   (uint64_t)a.block_table_stride * (uint64_t)bs);
 }
 
-// C: cache element; T: query element (C, or any with fp8 keys).
+// A workgroup's kv head, sequence and part of the sequence: consecutive workgroups
+// take the pairs, so the parts that only long sequences have come last.
+struct Place {
+  int j, s, part;
+};
+__device__ __forceinline__ Place place(const WeightsArgs& a, int num_kv_heads) {
+  const uint32_t pairs = (uint32_t)a.num_seqs * (uint32_t)num_kv_heads;
+  const uint32_t pair = blockIdx.x % pairs;
+  return {(int)(pair % (uint32_t)num_kv_heads), (int)(pair / (uint32_t)num_kv_heads),
+          (int)(blockIdx.x / pairs)};
+}
+
+// The sequence at place r of the lengths in descending order (equal 32nds of max_ctx
+// in the order of their indexes), for at most kOrdered sequences: a wave holds the
+// lengths and counts by ballots. The mixed batch above took 85 us in the order of the
+// indexes, 76 in this one.
+constexpr int kOrdered = 512;
+__device__ __forceinline__ int longest(const WeightsArgs& a, int r) {
+  const int lane = threadIdx.x & 63;
+  const int shift = max(27 - (int)__clz(a.max_ctx), 0);
+  int bin[kOrdered / 64];
+#pragma unroll
+  for (int i = 0; i < kOrdered / 64; ++i) {
+    const int s = i * 64 + lane;
+    bin[i] = s < a.num_seqs ? (int)(min(a.context_lens[s], (uint32_t)a.max_ctx) >> shift) : -1;
+  }
+  auto at_least = [&](int t) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kOrdered / 64; ++i) n += __popcll(__ballot(bin[i] >= t));
+    return n;
+  };
+  int t = 0;
+#pragma unroll
+  for (int b = 32; b > 0; b /= 2)
+    if (at_least(t + b) > r) t += b;
+  r -= at_least(t + 1);
+  int s = 0;
+#pragma unroll
+  for (int i = 0; i < kOrdered / 64; ++i) {
+    const uint64_t m = __ballot(bin[i] == t);
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    const uint64_t hit = __ballot(bin[i] == t && before == r);
+    if (hit != 0) s = i * 64 + __builtin_ctzll(hit);
+    r -= __popcll(m);
+  }
+  return s;
+}
+
+// Tiles of 16 tokens whose keys a wave holds, by the 16-byte chunks of a key row: at
+// most 64 registers.
+constexpr int wave_tiles(int chunks) { return chunks <= 16 ? 4 : chunks <= 32 ? 2 : 1; }
+
+// Shapes of the operands, by query type T, cache element C (T itself, or any with
+// fp8 keys) and head dim.
 template <typename T, typename C, int D>
-__global__ __launch_bounds__(kThreads) void weight_logits_kernel(WeightsArgs a, int32_t num_kv_heads,
-                                                                 int32_t bs_log2, int64_t num_blocks,
-                                                                 int64_t block_stride,
-                                                                 int64_t head_stride,
-                                                                 float* __restrict__ logits,
-                                                                 float2* __restrict__ stats,
-                                                                 int32_t ctx_pad, int32_t max_chunks) {
-  constexpr bool kF8 = std::is_same_v<C, fp8_t>;
-  constexpr bool kF32 = std::is_same_v<T, float>;
-  constexpr int X = pack_x<C>();
-  constexpr int CH = D / X;               // chunks of a key row
-  constexpr int KV = (CH + 3) / 4;        // vectors of a lane per 16 tokens
-  constexpr bool kRagged = CH % 4 != 0;   // (head dim 96 in fp8: the last vector is half there)
-  constexpr int QV = X * (int)ElemTraits<T>::kBytes / 16;  // query vectors per chunk
-  // tiles of 16 tokens whose keys are in flight together: at most 64 registers
-  constexpr int TW = KV * 4 <= 64 / 4 ? 4 : KV * 2 <= 64 / 4 ? 2 : 1;
+struct Frag {
+  static constexpr bool kF8 = std::is_same_v<C, fp8_t>;
+  static constexpr bool kF32 = std::is_same_v<T, float>;
+  static constexpr int X = pack_x<C>();
+  static constexpr int CH = D / X;              // chunks of a key row
+  static constexpr int KV = (CH + 3) / 4;       // vectors of a lane per 16 tokens
+  static constexpr bool kRagged = CH % 4 != 0;  // (head dim 96 in fp8: the last is half there)
+  static constexpr int QV = X * (int)ElemTraits<T>::kBytes / 16;  // query vectors per chunk
+  static constexpr int TW = wave_tiles(CH);
   static_assert(D % X == 0, "whole chunks");
 
-  __shared__ float s_m[4][16], s_s[4][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int bs = 1 << bs_log2;
-  const int s = blockIdx.y;
-  const int j = (int)(blockIdx.x % (uint32_t)num_kv_heads);
-  const int rest = (int)(blockIdx.x / (uint32_t)num_kv_heads);
-  const int chunk = rest % max_chunks, rg = rest / max_chunks;
-  const int group = a.num_heads / num_kv_heads;
-  const int L = seq_len(a, s, bs);
-  const SeqRows rows = seq_rows(a, s);
-  const int m_count = rows.n * group;  // rows of this kv head
-  if (chunk * kChunk >= L || rg * 16 >= m_count) return;
+  uint4 v[KV];
+};
 
-  // query row of this lane in the A operand, zeros past the last
-  const int c0 = lane >> 4;
-  uint4 qv[KV][QV];
-  {
-    const int m = rg * 16 + (lane & 15);
-    const int r = m / group;
-    const T* q = static_cast<const T*>(a.query) +
-                 ((rows.first + min(r, rows.n - 1)) * a.num_heads + j * group + (m - r * group)) * D;
+// The 16 query rows from m0 on as the A operand, zeros past the last.
+template <typename T, typename C, int D>
+__device__ __forceinline__ void load_rows(const WeightsArgs& a, const SeqRows& rows, int j, int group,
+                                          int m0, int m_count,
+                                          uint4 (&qv)[Frag<T, C, D>::KV][Frag<T, C, D>::QV]) {
+  using F = Frag<T, C, D>;
+  const int lane = threadIdx.x & 63;
+  const int m = m0 + (lane & 15), r = m / group;
+  const T* q = static_cast<const T*>(a.query) +
+               ((rows.first + min(r, rows.n - 1)) * a.num_heads + j * group + (m - r * group)) * D;
 #pragma unroll
-    for (int v = 0; v < KV; ++v)
+  for (int v = 0; v < F::KV; ++v)
 #pragma unroll
-      for (int h = 0; h < QV; ++h) {
-        const int c = c0 + 4 * v;
-        qv[v][h] = make_uint4(0u, 0u, 0u, 0u);
-        if (m < m_count && (!kRagged || c < CH))
-          qv[v][h] = *reinterpret_cast<const uint4*>(q + c * X + h * (16 / ElemTraits<T>::kBytes));
-      }
-  }
-  float scale = a.scale * 1.4426950408889634f;
-  if constexpr (kF8) scale *= *a.k_scale;
+    for (int h = 0; h < F::QV; ++h) {
+      const int c = (lane >> 4) + 4 * v;
+      qv[v][h] = make_uint4(0u, 0u, 0u, 0u);
+      if (m < m_count && (!F::kRagged || c < F::CH))
+        qv[v][h] =
+            *reinterpret_cast<const uint4*>(q + c * F::X + h * (16 / ElemTraits<T>::kBytes));
+    }
+}
 
-  const uint32_t* table = a.block_tables + (int64_t)s * a.block_table_stride;
-  const C* keys = static_cast<const C*>(a.key_cache) + j * head_stride;
-  const int t_wave = chunk * kChunk + wave * 64;
-  // last token each of the lane's four rows sees, plus one
-  int see[4];
+// The keys of 16 tokens: this lane's token lies at `off` of block `phys`.
+template <typename T, typename C, int D, bool kOnce>
+__device__ __forceinline__ void load_keys(const C* keys, int64_t block_stride, int64_t phys, int off,
+                                          int bs_log2, Frag<T, C, D>& f) {
+  using F = Frag<T, C, D>;
+  const int c0 = (threadIdx.x & 63) >> 4;
+  const uint4* tile = reinterpret_cast<const uint4*>(keys + phys * block_stride) + off;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = rg * 16 + (lane >> 4) * 4 + i;
-    const int r = m / group;
-    see[i] = m >= m_count ? 0 : a.causal ? min(L, r + 1 + L - rows.n) : L;
-  }
-  float lg[4][4];  // [tile][row]
-#pragma unroll
-  for (int t4 = 0; t4 < 4; t4 += TW) {
-    uint4 kv[TW][KV];
-    bool ok[TW];
-#pragma unroll
-    for (int u = 0; u < TW; ++u) {
-      const int tok = t_wave + (t4 + u) * 16 + (lane & 15);
-      const int tc = min(tok, L - 1);  // past the context: its last token, masked below
-      const uint32_t phys = table[tc >> bs_log2];
-      ok[u] = (int64_t)phys < num_blocks;
-      const uint4* tile = reinterpret_cast<const uint4*>(
-          keys + (ok[u] ? (int64_t)phys : 0) * block_stride) + (tc & (bs - 1));
-#pragma unroll
-      for (int v = 0; v < KV; ++v) {
-        const int c = c0 + 4 * v;
-        kv[u][v] = make_uint4(0u, 0u, 0u, 0u);
-        if (!kRagged || c < CH) kv[u][v] = load_stream(tile + (c << bs_log2));
-      }
+  for (int v = 0; v < F::KV; ++v) {
+    const int c = c0 + 4 * v;
+    f.v[v] = make_uint4(0u, 0u, 0u, 0u);
+    if (!F::kRagged || c < F::CH) {
+      const uint4* src = tile + (c << bs_log2);
+      if constexpr (kOnce) f.v[v] = load_stream(src);
+      else f.v[v] = *src;
     }
-#pragma unroll
-    for (int u = 0; u < TW; ++u) {
-      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int v = 0; v < KV; ++v) {
-        if constexpr (kF8 && kF32) {
-          const uint32_t w[4] = {kv[u][v].x, kv[u][v].y, kv[u][v].z, kv[u][v].w};
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint4 f;
-            fp8x4_f32(w[h], f);
-            acc = mma16_f32(qv[v][h], f, acc);
-          }
-        } else if constexpr (kF8) {
-          uint4 lo, hi;
-          fp8x16_to_pk<T>(kv[u][v], lo, hi);
-          acc = mma16<T>(qv[v][0], lo, acc);
-          acc = mma16<T>(qv[v][1], hi, acc);
-        } else if constexpr (kF32) {
-          acc = mma16_f32(qv[v][0], kv[u][v], acc);
-        } else {
-          acc = mma16<T>(qv[v][0], kv[u][v], acc);
-        }
-      }
-      const int tok = t_wave + (t4 + u) * 16 + (lane & 15);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        lg[t4 + u][i] = ok[u] && tok < see[i] ? acc[i] * scale : -INFINITY;
-    }
-  }
-  // the logits, and the row's maximum and sum over the wave's tokens
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int mi = (lane >> 4) * 4 + i, m = rg * 16 + mi;
-    const float mx = row16_max(fmaxf(fmaxf(lg[0][i], lg[1][i]), fmaxf(lg[2][i], lg[3][i])));
-    float sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      sum += lg[u][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lg[u][i] - mx);
-    sum = row16_sum(sum);
-    if ((lane & 15) == 0) {
-      s_m[wave][mi] = mx;
-      s_s[wave][mi] = sum;
-    }
-    if (m < m_count) {
-      const int r = m / group;
-      float* dst = logits + ((rows.first + r) * a.num_heads + j * group + (m - r * group)) * ctx_pad +
-                   t_wave + (lane & 15);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) dst[16 * u] = lg[u][i];
-    }
-  }
-  __syncthreads();
-  const int m = rg * 16 + threadIdx.x;
-  if (threadIdx.x < 16 && m < m_count) {
-    float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_m[w][threadIdx.x]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float sw = s_s[w][threadIdx.x];
-      if (sw != 0.f) sum += sw * __builtin_amdgcn_exp2f(s_m[w][threadIdx.x] - mx);
-    }
-    const int r = m / group;
-    stats[((rows.first + r) * a.num_heads + j * group + (m - r * group)) * max_chunks + chunk] =
-        make_float2(mx, sum);
   }
 }
 
-// Rows merged at once in the second pass.
-constexpr int kRowTile = 64;
+// Products of 16 rows and 16 tokens: lane l gets rows (l / 16) * 4 + i of token l % 16.
+template <typename T, typename C, int D>
+__device__ __forceinline__ f32x4_t products(
+    const uint4 (&qv)[Frag<T, C, D>::KV][Frag<T, C, D>::QV], const Frag<T, C, D>& f) {
+  using F = Frag<T, C, D>;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < F::KV; ++v) {
+    if constexpr (F::kF8 && F::kF32) {
+      const uint32_t w[4] = {f.v[v].x, f.v[v].y, f.v[v].z, f.v[v].w};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        uint4 k;
+        fp8x4_f32(w[h], k);
+        acc = mma16_f32(qv[v][h], k, acc);
+      }
+    } else if constexpr (F::kF8) {
+      uint4 lo, hi;
+      fp8x16_to_pk<T>(f.v[v], lo, hi);
+      acc = mma16<T>(qv[v][0], lo, acc);
+      acc = mma16<T>(qv[v][1], hi, acc);
+    } else if constexpr (F::kF32) {
+      acc = mma16_f32(qv[v][0], f.v[v], acc);
+    } else {
+      acc = mma16<T>(qv[v][0], f.v[v], acc);
+    }
+  }
+  return acc;
+}
 
-// One workgroup per (1024 tokens, kv head, sequence), four tokens per thread.
+// Running maximum and sum of one row over the tokens a lane has seen. They begin at
+// the lowest value, so that a masked logit (-inf) adds exp2(-inf) = 0.
+struct RowStat {
+  float m = -FLT_MAX, s = 0.f;
+  __device__ __forceinline__ void add(float l) {
+    const float n = fmaxf(m, l);
+    s = fmaf(s, __builtin_amdgcn_exp2f(m - n), __builtin_amdgcn_exp2f(l - n));
+    m = n;
+  }
+  __device__ __forceinline__ void join(float om, float os) {
+    const float n = fmaxf(m, om);
+    s = s * __builtin_amdgcn_exp2f(m - n) + os * __builtin_amdgcn_exp2f(om - n);
+    m = n;
+  }
+  // over the 16 lanes of a row
+  __device__ __forceinline__ void join16() {
+    const float n = row16_max(m);
+    s = row16_sum(s * __builtin_amdgcn_exp2f(m - n));
+    m = n;
+  }
+};
+
+// Few rows (one tile of 16 per kv head), first pass or both. One workgroup per (kv
+// head, sequence, chunk): its waves share the chunk's tiles of 16 tokens evenly, each
+// a run of them, with the next TW tiles' keys in flight. kWhole: the chunk is the
+// whole context; its logits stay in LDS and the weights are added here.
+template <typename T, typename C, int D, bool kWhole>
+__global__ __launch_bounds__(kThreads) void weight_logits_kernel(
+    WeightsArgs a, int32_t num_kv_heads, int32_t bs_log2, int64_t num_blocks, int64_t block_stride,
+    int64_t head_stride, float* __restrict__ logits, float2* __restrict__ stats, int32_t ctx_pad,
+    int32_t max_chunks, int32_t chunk_tokens) {
+  using F = Frag<T, C, D>;
+  constexpr int TW = F::TW;
+  __shared__ float s_m[4][16], s_s[4][16];
+  extern __shared__ uint32_t s_dyn[];  // the chunk's block ids, then its logits (kWhole)
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place at = place(a, num_kv_heads);
+  const int j = at.j, chunk = at.part;
+  // the longest first, so that none is left to run alone at the end
+  const int s = kWhole && a.num_seqs <= kOrdered ? longest(a, at.s) : at.s;
+  const int group = a.num_heads / num_kv_heads;
+  const int L = seq_len(a, s, 1 << bs_log2);
+  const SeqRows rows = seq_rows(a, s);
+  const int m_count = min(rows.n * group, 16);  // rows of this kv head
+  const int64_t begin = (int64_t)chunk * chunk_tokens;
+  if (begin >= L || m_count == 0) return;
+
+  const int tiles = ((int)min((int64_t)chunk_tokens, L - begin) + 15) / 16;
+  const int per = (tiles + 3) / 4;
+  const int nt = min(per, tiles - wave * per);  // tiles of this wave, none if negative
+  const int t_wave = (int)begin + wave * per * 16;
+  const int b_first = (int)begin >> bs_log2;  // (chunks are whole blocks)
+  {
+    const int n = (((int)begin + tiles * 16 - 1) >> bs_log2) - b_first + 1;
+    const int last = (L - 1) >> bs_log2;
+    const uint32_t* table = a.block_tables + (int64_t)s * a.block_table_stride;
+    for (int i = threadIdx.x; i < n; i += kThreads) s_dyn[i] = table[min(b_first + i, last)];
+  }
+  uint4 qv[F::KV][F::QV];
+  load_rows<T, C, D>(a, rows, j, group, 0, m_count, qv);
+  float scale = a.scale * 1.4426950408889634f;
+  if constexpr (F::kF8) scale *= *a.k_scale;
+  const C* keys = static_cast<const C*>(a.key_cache) + j * head_stride;
+
+  // per row of the lane: last token it sees, plus one, and where its logits go
+  float* s_logits = reinterpret_cast<float*>(s_dyn + (chunk_tokens >> bs_log2));
+  int see[4];
+  float* dst[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = (lane >> 4) * 4 + i, r = m / group;
+    see[i] = m >= m_count ? 0 : a.causal ? min(L, r + 1 + L - rows.n) : L;
+    dst[i] = (kWhole ? s_logits + m * chunk_tokens
+                     : logits + ((rows.first + r) * a.num_heads + j * group + (m - r * group)) *
+                                    ctx_pad) +
+             t_wave + (lane & 15);
+  }
+  lds_group_barrier();
+  Frag<T, C, D> f[TW];
+  bool ok[TW];
+  auto load = [&](int u, int i) {
+    const int tok = min(t_wave + i * 16 + (lane & 15), L - 1);  // past the end: masked below
+    const uint32_t phys = s_dyn[(tok >> bs_log2) - b_first];
+    ok[u] = (int64_t)phys < num_blocks;
+    load_keys<T, C, D, true>(keys, block_stride, ok[u] ? (int64_t)phys : 0,
+                             tok & ((1 << bs_log2) - 1), bs_log2, f[u]);
+  };
+  RowStat st[4];
+  auto use = [&](int u, int i, const f32x4_t& acc, bool there) {
+    const int tok = t_wave + i * 16 + (lane & 15);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k >= m_count) break;  // (uniform: rows 0 .. 3 are in the first lanes)
+      const float l = there && tok < see[k] ? acc[k] * scale : -INFINITY;
+      st[k].add(l);
+      if ((lane >> 4) * 4 + k < m_count) dst[k][i * 16] = l;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < TW; ++u)
+    if (u < nt) load(u, u);
+  int i0 = 0;
+#pragma unroll 1
+  for (; i0 + 2 * TW <= nt; i0 += TW) {
+#pragma unroll
+    for (int u = 0; u < TW; ++u) {
+      const f32x4_t acc = products<T, C, D>(qv, f[u]);
+      const bool there = ok[u];
+      load(u, i0 + u + TW);
+      use(u, i0 + u, acc, there);
+    }
+  }
+#pragma unroll 1
+  for (; i0 < nt; i0 += TW) {  // at most two rounds
+#pragma unroll
+    for (int u = 0; u < TW; ++u) {
+      if (i0 + u < nt) {
+        const f32x4_t acc = products<T, C, D>(qv, f[u]);
+        const bool there = ok[u];
+        if (i0 + u + TW < nt) load(u, i0 + u + TW);
+        use(u, i0 + u, acc, there);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    st[k].join16();
+    if ((lane & 15) == 0) {
+      s_m[wave][(lane >> 4) * 4 + k] = st[k].m;
+      s_s[wave][(lane >> 4) * 4 + k] = st[k].s;
+    }
+  }
+  lds_group_barrier();
+  const int m = threadIdx.x;
+  if constexpr (kWhole) {
+    if (m < m_count) {
+      RowStat all;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) all.join(s_m[w][m], s_s[w][m]);
+      s_m[0][m] = all.m;
+      s_s[0][m] = all.s == 0.f ? 0.f : 1.f / all.s;  // (a row that sees no token adds nothing)
+    }
+    lds_group_barrier();
+    float* out = a.scores + s * a.score_seq_stride + j * a.score_head_stride;
+    for (int t = threadIdx.x; t < L; t += kThreads) {
+      float sum = 0.f;
+      for (int i = 0; i < m_count; ++i) {
+        const float l = s_logits[i * chunk_tokens + t];
+        sum += l == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l - s_m[0][i]) * s_s[0][i];
+      }
+      out[t] += sum;
+    }
+  } else if (m < m_count) {
+    RowStat all;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) all.join(s_m[w][m], s_s[w][m]);
+    const int r = m / group;
+    stats[((rows.first + r) * a.num_heads + j * group + (m - r * group)) * max_chunks + chunk] =
+        make_float2(all.m, all.s);
+  }
+}
+
+// Maximum and reciprocal sum of a row, from its chunks' pairs, by kLanes lanes (four
+// pairs each in flight); a row that sees no token gets a reciprocal of 0.
+template <int kLanes>
+__device__ __forceinline__ float2 merge_row(const float2* st, int chunks, int part) {
+  RowStat all;
+  for (int c = part; c < chunks; c += 4 * kLanes) {
+    float2 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = st[min(c + i * kLanes, chunks - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i * kLanes < chunks) all.join(v[i].x, v[i].y);
+  }
+#pragma unroll
+  for (int x = 1; x < kLanes; x *= 2)
+    all.join(__shfl_xor(all.m, x, 64), __shfl_xor(all.s, x, 64));
+  return make_float2(all.m, all.s == 0.f ? 0.f : 1.f / all.s);
+}
+
+// Second pass of few rows: one workgroup per (kv head, sequence, 1024 tokens), every
+// fourth row of 256 tokens to a thread.
 __global__ __launch_bounds__(kThreads) void weight_sum_kernel(WeightsArgs a, int32_t num_kv_heads,
                                                               int32_t bs,
                                                               const float* __restrict__ logits,
                                                               const float2* __restrict__ stats,
-                                                              int32_t ctx_pad, int32_t max_chunks) {
-  __shared__ float s_max[kRowTile], s_inv[kRowTile];
-  const int s = blockIdx.z, j = blockIdx.y;
-  const int t = blockIdx.x * 1024 + threadIdx.x * 4;
+                                                              int32_t ctx_pad, int32_t max_chunks,
+                                                              int32_t chunk_tokens) {
+  __shared__ float2 s_row[16];
+  const Place at = place(a, num_kv_heads);
+  const int j = at.j, s = at.s;
+  const int64_t begin = (int64_t)at.part * 1024;
   const int group = a.num_heads / num_kv_heads;
   const int L = seq_len(a, s, bs);
-  if (blockIdx.x * 1024 >= (uint32_t)L) return;
   const SeqRows rows = seq_rows(a, s);
-  const int m_count = rows.n * group;
-  const int chunks = (L + kChunk - 1) / kChunk;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int m0 = 0; m0 < m_count; m0 += kRowTile) {
-    const int n = min(kRowTile, m_count - m0);
-    __syncthreads();
-    {  // four lanes per row merge the chunks' pairs
-      const int mi = threadIdx.x >> 2, part = threadIdx.x & 3;
-      float mx = -INFINITY, sum = 0.f;
-      if (mi < n) {
-        const int m = m0 + mi, r = m / group;
-        const float2* st =
-            stats + ((rows.first + r) * a.num_heads + j * group + (m - r * group)) * max_chunks;
-        for (int c = part; c < chunks; c += 4) mx = fmaxf(mx, st[c].x);
-        mx = wave_max_range<1, 2>(mx);
-        for (int c = part; c < chunks; c += 4)
-          if (st[c].y != 0.f) sum += st[c].y * __builtin_amdgcn_exp2f(st[c].x - mx);
-        sum = wave_sum_range<1, 2>(sum);
-      }
-      if (mi < n && part == 0) {
-        // a row that sees no token adds nothing
-        s_max[mi] = mx == -INFINITY ? 0.f : mx;
-        s_inv[mi] = sum == 0.f ? 0.f : 1.f / sum;
-      }
-    }
-    __syncthreads();
-    if (t < L) {
-      for (int mi = 0; mi < n; ++mi) {
-        const int m = m0 + mi, r = m / group;
-        const float4 l = *reinterpret_cast<const float4*>(
-            logits + ((rows.first + r) * a.num_heads + j * group + (m - r * group)) * ctx_pad + t);
-        const float mx = s_max[mi], inv = s_inv[mi];
-        acc[0] += l.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l.x - mx) * inv;
-        acc[1] += l.y == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l.y - mx) * inv;
-        acc[2] += l.z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l.z - mx) * inv;
-        acc[3] += l.w == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l.w - mx) * inv;
-      }
-    }
-  }
+  const int m_count = min(rows.n * group, 16);
+  if (begin >= L || m_count == 0) return;
+  const int t = (int)begin + threadIdx.x;
+  auto row_of = [&](int m) {
+    const int r = m / group;
+    return (rows.first + r) * a.num_heads + j * group + (m - r * group);
+  };
   float* out = a.scores + s * a.score_seq_stride + j * a.score_head_stride + t;
+  float l[4], acc[4];
+  auto load = [&](int m) {
+    const float* src = logits + row_of(m) * ctx_pad + t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] = t + i * 256 < L ? src[i * 256] : -INFINITY;
+  };
+  load(0);  // in flight while the rows' sums are joined
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = t + i * 256 < L ? out[i * 256] : 0.f;
+  {
+    const int m = threadIdx.x >> 4, part = threadIdx.x & 15;
+    const int chunks = (L + chunk_tokens - 1) / chunk_tokens;
+    const float2 row = merge_row<16>(stats + row_of(min(m, m_count - 1)) * max_chunks, chunks, part);
+    if (part == 0) s_row[m] = row;
+  }
+  lds_group_barrier();
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int m = 0; m < m_count; ++m) {
+    const float2 row = s_row[m];
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = l[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l[i] - row.x) * row.y;
+    if (m + 1 < m_count) load(m + 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += w[i];
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (t + i < L) out[i] += acc[i];
+    if (t + i * 256 < L) out[i * 256] = acc[i] + sum[i];
 }
 
-struct Layout {
-  int64_t rows;  // (query row, head) pairs
-  int32_t ctx_pad, max_chunks;
-  size_t stats_at, bytes;
-};
-Layout layout(int64_t total_rows, int32_t num_heads, int32_t max_ctx) {
-  Layout l;
-  l.rows = total_rows * num_heads;
-  l.max_chunks = std::max(1, (max_ctx + kChunk - 1) / kChunk);
-  l.ctx_pad = l.max_chunks * kChunk;
-  l.stats_at = (size_t)l.rows * l.ctx_pad * sizeof(float);
-  l.bytes = l.stats_at + (size_t)l.rows * l.max_chunks * sizeof(float2);
-  return l;
+// Sizes of the passes of many rows, by the 16-byte vectors of a query row: the keys of a
+// wave's tiles take 64 registers (in the query's type), the queries of a block of rows
+// 16 KiB of LDS.
+constexpr int row_tiles(int vectors) { return vectors <= 16 ? 4 : vectors <= 32 ? 2 : 1; }
+constexpr int row_block(int vectors) { return 16 * row_tiles(vectors); }
+
+// Waves per SIMD of these passes: four (128 registers), or three where 32-bit queries
+// meet fp8 keys, which would spill. The first pass over 8 sequences of 1000 to 6000
+// tokens with 64 rows each took 18.6 us, with three 21.6.
+template <typename T, typename C>
+constexpr int kRowWaves = std::is_same_v<T, float> && !std::is_same_v<T, C> ? 3 : 4;
+
+// Both passes of many rows; the logits are formed anew in the second (kSum). A workgroup
+// holds the keys of a piece of 4 * TW tiles in registers, converted to the query's type,
+// while a block of rows passes by in LDS, 16 at a time. First pass: one workgroup per (kv
+// head, sequence, chunk of `subs` pieces, block of rows), writing the rows' pairs;
+// second: per (kv head, sequence, piece), all rows.
+template <typename T, typename C, int D, bool kSum>
+__global__ __launch_bounds__(kThreads, (kRowWaves<T, C>)) void weight_rows_kernel(
+    WeightsArgs a, int32_t num_kv_heads, int32_t bs_log2, int64_t num_blocks, int64_t block_stride,
+    int64_t head_stride, float2* __restrict__ stats, int32_t max_chunks, int32_t subs) {
+  using F = Frag<T, C, D>;
+  constexpr int RV = D * (int)ElemTraits<T>::kBytes / 16;  // vectors of a query row
+  constexpr int TW = row_tiles(RV), RB = row_block(RV);
+  constexpr int kPiece = 64 * TW;
+  __shared__ uint4 s_q[RB][RV + 1];  // (padded: 16 rows in different banks)
+  __shared__ float2 s_row[kSum ? 1 : 4][RB];
+  __shared__ int s_see[RB];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place at = place(a, num_kv_heads);
+  const int j = at.j, s = at.s;
+  const int group = a.num_heads / num_kv_heads;
+  const int L = seq_len(a, s, 1 << bs_log2);
+  const SeqRows rows = seq_rows(a, s);
+  const int m_count = rows.n * group;
+  const int chunk = kSum ? 0 : at.part % max_chunks;
+  const int mb = kSum ? 0 : at.part / max_chunks * RB;
+  const int chunks = (L + kPiece * subs - 1) / (kPiece * subs);
+  const int64_t begin = kSum ? (int64_t)at.part * kPiece : (int64_t)chunk * subs * kPiece;
+  if (begin >= L || mb >= m_count) return;
+  float scale = a.scale * 1.4426950408889634f;
+  if constexpr (F::kF8) scale *= *a.k_scale;
+  const C* keys = static_cast<const C*>(a.key_cache) + j * head_stride;
+  const uint32_t* table = a.block_tables + (int64_t)s * a.block_table_stride;
+  auto row_of = [&](int m) {
+    const int r = m / group;
+    return (rows.first + r) * a.num_heads + j * group + (m - r * group);
+  };
+  uint4 kv[TW][F::KV][F::QV];
+  bool ok[TW];
+  auto load = [&](int t_wave) {
+    uint32_t phys[TW];
+#pragma unroll
+    for (int u = 0; u < TW; ++u)
+      phys[u] = table[min(t_wave + u * 16 + (lane & 15), L - 1) >> bs_log2];
+#pragma unroll
+    for (int u = 0; u < TW; ++u) {
+      const int tok = min(t_wave + u * 16 + (lane & 15), L - 1);
+      ok[u] = (int64_t)phys[u] < num_blocks;
+      Frag<T, C, D> f;
+      load_keys<T, C, D, false>(keys, block_stride, ok[u] ? (int64_t)phys[u] : 0,
+                                tok & ((1 << bs_log2) - 1), bs_log2, f);
+#pragma unroll
+      for (int v = 0; v < F::KV; ++v) {
+        if constexpr (F::kF8 && F::kF32) {
+          fp8x4_f32(f.v[v].x, kv[u][v][0]);
+          fp8x4_f32(f.v[v].y, kv[u][v][1]);
+          fp8x4_f32(f.v[v].z, kv[u][v][2]);
+          fp8x4_f32(f.v[v].w, kv[u][v][3]);
+        } else if constexpr (F::kF8) {
+          fp8x16_to_pk<T>(f.v[v], kv[u][v][0], kv[u][v][1]);
+        } else {
+          kv[u][v][0] = f.v[v];
+        }
+      }
+    }
+  };
+  // the queries of a block of rows (zeros past the last) and the last token each sees,
+  // plus one
+  auto stage = [&](int m_at) {
+    for (int i = threadIdx.x; i < RB * RV; i += kThreads) {
+      const int mi = i / RV, m = m_at + mi;
+      uint4 q = make_uint4(0u, 0u, 0u, 0u);
+      if (m < m_count)
+        q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.query) + row_of(m) * D)[i - mi * RV];
+      s_q[mi][i - mi * RV] = q;
+    }
+    const int m = m_at + threadIdx.x;
+    if (threadIdx.x < RB)
+      s_see[threadIdx.x] = m >= m_count ? 0 : a.causal ? min(L, m / group + 1 + L - rows.n) : L;
+  };
+  // the products of a block's rows: visit(first of the lane's four rows in the block, acc)
+  auto block_rows = [&](int n, auto visit) {
+#pragma unroll 1
+    for (int m0 = 0; m0 < n; m0 += 16) {
+      asm volatile("" ::: "memory");  // (no later read of LDS moves up: registers)
+      f32x4_t acc[TW];
+#pragma unroll
+      for (int u = 0; u < TW; ++u) acc[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < F::KV; ++v) {
+        const int c = (lane >> 4) + 4 * v;
+#pragma unroll
+        for (int h = 0; h < F::QV; ++h) {
+          uint4 q = make_uint4(0u, 0u, 0u, 0u);
+          if (!F::kRagged || c < F::CH) q = s_q[m0 + (lane & 15)][c * F::QV + h];
+#pragma unroll
+          for (int u = 0; u < TW; ++u) {
+            if constexpr (F::kF32) acc[u] = mma16_f32(q, kv[u][v][h], acc[u]);
+            else acc[u] = mma16<T>(q, kv[u][v][h], acc[u]);
+          }
+        }
+      }
+      visit(m0 + (lane >> 4) * 4, acc);
+    }
+  };
+  // whether every row sees every token of the wave's tiles (uniform)
+  auto all_seen = [&](int t_wave) {
+    bool there = true;
+#pragma unroll
+    for (int u = 0; u < TW; ++u) there &= ok[u];
+    return t_wave + 16 * TW <= (a.causal ? L - rows.n + 1 : L) && __all(there);
+  };
+  auto logit = [&](float acc, int u, int t_wave, int see) {
+    return ok[u] && t_wave + u * 16 + (lane & 15) < see ? acc * scale : -INFINITY;
+  };
+  if constexpr (!kSum) {
+    const int n = min(RB, m_count - mb);
+    stage(mb);
+    for (int sub = 0; sub < subs; ++sub) {
+      const int64_t piece = begin + sub * kPiece;
+      if (piece >= L) break;
+      const int t_wave = (int)piece + wave * 16 * TW;
+      load(t_wave);
+      if (sub == 0) lds_group_barrier();
+      auto stat = [&](int mi, const float(&l)[TW]) {
+        RowStat st;
+#pragma unroll
+        for (int u = 0; u < TW; ++u) st.m = fmaxf(st.m, l[u]);
+        st.m = row16_max(st.m);
+#pragma unroll
+        for (int u = 0; u < TW; ++u) st.s += __builtin_amdgcn_exp2f(l[u] - st.m);
+        st.s = row16_sum(st.s);
+        float2& mine = s_row[wave][mi];
+        if ((lane & 15) == 0) {
+          if (sub > 0) st.join(mine.x, mine.y);
+          mine = make_float2(st.m, st.s);
+        }
+      };
+      if (all_seen(t_wave)) {
+        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float l[TW];
+#pragma unroll
+            for (int u = 0; u < TW; ++u) l[u] = acc[u][k] * scale;
+            stat(mi + k, l);
+          }
+        });
+      } else {
+        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float l[TW];
+#pragma unroll
+            for (int u = 0; u < TW; ++u) l[u] = logit(acc[u][k], u, t_wave, s_see[mi + k]);
+            stat(mi + k, l);
+          }
+        });
+      }
+    }
+    lds_group_barrier();
+    const int m = mb + threadIdx.x;
+    if (threadIdx.x < n) {
+      RowStat all;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) all.join(s_row[w][threadIdx.x].x, s_row[w][threadIdx.x].y);
+      stats[row_of(m) * max_chunks + chunk] = make_float2(all.m, all.s);
+    }
+  } else {
+    const int t_wave = (int)begin + wave * 16 * TW;
+    constexpr int kLanes = kThreads / RB;  // lanes that merge a row's pairs
+    float sum[TW];
+#pragma unroll
+    for (int u = 0; u < TW; ++u) sum[u] = 0.f;
+    load(t_wave);
+#pragma unroll 1
+    for (int m_at = 0; m_at < m_count; m_at += RB) {
+      const int n = min(RB, m_count - m_at);
+      if (m_at > 0) lds_group_barrier();  // (the rows before are used)
+      stage(m_at);
+      const int m = threadIdx.x / kLanes, part = threadIdx.x % kLanes;
+      const float2 row =
+          merge_row<kLanes>(stats + row_of(min(m_at + m, m_count - 1)) * max_chunks, chunks, part);
+      // (rows past the last have queries of zero: their weights are 1 * 0)
+      if (part == 0) s_row[0][m] = m < n ? row : make_float2(0.f, 0.f);
+      lds_group_barrier();
+      if (all_seen(t_wave)) {
+        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 row = s_row[0][mi + k];
+#pragma unroll
+            for (int u = 0; u < TW; ++u)
+              sum[u] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[u][k], scale, -row.x)), row.y, sum[u]);
+          }
+        });
+      } else {
+        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 row = s_row[0][mi + k];
+#pragma unroll
+            for (int u = 0; u < TW; ++u) {
+              const float l = logit(acc[u][k], u, t_wave, s_see[mi + k]);
+              sum[u] += l == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l - row.x) * row.y;
+            }
+          }
+        });
+      }
+    }
+    float* out = a.scores + s * a.score_seq_stride + j * a.score_head_stride;
+#pragma unroll
+    for (int u = 0; u < TW; ++u) {
+      sum[u] += __shfl_xor(sum[u], 16, 64);
+      sum[u] += __shfl_xor(sum[u], 32, 64);
+      const int tok = t_wave + u * 16 + lane;
+      if (lane < 16 && tok < L) out[tok] += sum[u];
+    }
+  }
 }
 
 template <typename T, typename C, int D>
-void logits_launch(const WeightsArgs& a, const CacheGeom& g, const Layout& l, hipStream_t stream) {
-  const int group = a.num_heads / g.num_kv_heads;
-  const int64_t rgs = ((int64_t)a.max_query_len * group + 15) / 16;
-  const dim3 grid((uint32_t)(g.num_kv_heads * l.max_chunks * rgs), (uint32_t)a.num_seqs);
-  float* logits = static_cast<float*>(a.workspace);
-  float2* stats = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + l.stats_at);
-  hipLaunchKernelGGL((weight_logits_kernel<T, C, D>), grid, dim3(kThreads), 0, stream, a,
-                     g.num_kv_heads, __builtin_ctz((unsigned)g.block_size), g.num_blocks,
-                     g.block_stride, g.head_stride, logits, stats, l.ctx_pad, l.max_chunks);
+hipError_t weights_launch(const WeightsArgs& a, const WeightsPlan& p, const CacheGeom& g,
+                          hipStream_t stream) {
+  const int bs_log2 = __builtin_ctz((unsigned)g.block_size);
+  float2* stats = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + p.stats_at);
+  if (p.few) {
+    float* logits = static_cast<float*>(a.workspace);
+    const uint32_t lds = (uint32_t)(p.chunk_tokens >> bs_log2) * 4;
+    if (p.whole) {
+      hipLaunchKernelGGL((weight_logits_kernel<T, C, D, true>), dim3((uint32_t)p.first_grid),
+                         dim3(kThreads), lds + (uint32_t)p.lds_logits, stream, a, g.num_kv_heads,
+                         bs_log2, g.num_blocks, g.block_stride, g.head_stride, logits, stats,
+                         p.ctx_pad, p.max_chunks, p.chunk_tokens);
+      return hipGetLastError();
+    }
+    hipLaunchKernelGGL((weight_logits_kernel<T, C, D, false>), dim3((uint32_t)p.first_grid),
+                       dim3(kThreads), lds, stream, a, g.num_kv_heads, bs_log2, g.num_blocks,
+                       g.block_stride, g.head_stride, logits, stats, p.ctx_pad, p.max_chunks,
+                       p.chunk_tokens);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(weight_sum_kernel, dim3((uint32_t)p.second_grid), dim3(kThreads), 0, stream,
+                       a, g.num_kv_heads, g.block_size, logits, stats, p.ctx_pad, p.max_chunks,
+                       p.chunk_tokens);
+    return hipGetLastError();
+  }
+  const int subs = p.chunk_tokens / (64 * row_tiles(D * (int)ElemTraits<T>::kBytes / 16));
+  hipLaunchKernelGGL((weight_rows_kernel<T, C, D, false>), dim3((uint32_t)p.first_grid),
+                     dim3(kThreads), 0, stream, a, g.num_kv_heads, bs_log2, g.num_blocks,
+                     g.block_stride, g.head_stride, stats, p.max_chunks, subs);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((weight_rows_kernel<T, C, D, true>), dim3((uint32_t)p.second_grid),
+                     dim3(kThreads), 0, stream, a, g.num_kv_heads, bs_log2, g.num_blocks,
+                     g.block_stride, g.head_stride, stats, p.max_chunks, subs);
+  return hipGetLastError();
 }
 
 template <typename T, typename C>
-hipError_t logits_typed(const WeightsArgs& a, const CacheGeom& g, const Layout& l,
-                        hipStream_t stream) {
+hipError_t weights_typed(const WeightsArgs& a, const WeightsPlan& p, const CacheGeom& g,
+                         hipStream_t stream) {
   switch (g.head_dim) {
-    case 64: logits_launch<T, C, 64>(a, g, l, stream); break;
-    case 96: logits_launch<T, C, 96>(a, g, l, stream); break;
-    case 128: logits_launch<T, C, 128>(a, g, l, stream); break;
-    case 192: logits_launch<T, C, 192>(a, g, l, stream); break;
-    case 256: logits_launch<T, C, 256>(a, g, l, stream); break;
-    default: return hipErrorInvalidValue;
+    case 64: return weights_launch<T, C, 64>(a, p, g, stream);
+    case 96: return weights_launch<T, C, 96>(a, p, g, stream);
+    case 128: return weights_launch<T, C, 128>(a, p, g, stream);
+    case 192: return weights_launch<T, C, 192>(a, p, g, stream);
+    case 256: return weights_launch<T, C, 256>(a, p, g, stream);
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx) {
-  return layout(total_rows, num_heads, max_ctx).bytes;
+  const int64_t chunks = (max_ctx + kWeightsChunk - 1) / kWeightsChunk;
+  return (size_t)(total_rows * num_heads * chunks) * (kWeightsChunk * sizeof(float) + sizeof(float2));
+}
+
+WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g) {
+  WeightsPlan p;
+  const int64_t pairs = (int64_t)g.num_kv_heads * a.num_seqs;
+  const int64_t m_max = (int64_t)a.max_query_len * (a.num_heads / g.num_kv_heads);
+  auto parts = [&](int tokens) { return ((int64_t)a.max_ctx + tokens - 1) / tokens; };
+  // (at 16 rows the stored logits took 26 us for 8 sequences of 4000 tokens and 76 for
+  // 64 of 2000, the second reading of the keys 28 and 86)
+  p.few = m_max <= 16;
+  p.whole = false;
+  p.lds_logits = 0;
+  p.ctx_pad = (int32_t)(parts(kWeightsChunk) * kWeightsChunk);
+  p.chunk_tokens = kWeightsChunk;
+  if (p.few) {
+    // Whole contexts per workgroup once every compute unit has two: 256 sequences of up to
+    // 500 tokens took 49 us (57 in two launches), 64 of 1000 tokens 26 (28), 512 of mixed
+    // lengths 207 (246); with fewer, long sequences are left alone at the end (64 of up
+    // to 4096 tokens 40 (39), 8 of 1000 11 (9)).
+    const int64_t lds = m_max * p.ctx_pad * (int64_t)sizeof(float);
+    p.whole = pairs >= 512 && lds <= 65536;
+    if (p.whole) {
+      p.chunk_tokens = p.ctx_pad;
+      p.lds_logits = (int32_t)lds;
+    }
+    // chunks of 256 to 1024 tokens (64 to 256 per wave) while each compute unit has four
+    while (!p.whole && p.chunk_tokens < 1024 && pairs * parts(2 * p.chunk_tokens) >= 1024)
+      p.chunk_tokens *= 2;
+    p.first_grid = pairs * parts(p.chunk_tokens);
+    p.second_grid = pairs * parts(1024);
+  } else {
+    const int vectors = g.head_dim * (dtype == VPA_DTYPE_F32 ? 4 : 2) / 16;
+    const int64_t blocks = (m_max + row_block(vectors) - 1) / row_block(vectors);
+    while (p.chunk_tokens < 1024 && pairs * blocks * parts(2 * p.chunk_tokens) >= 1024)
+      p.chunk_tokens *= 2;
+    p.first_grid = pairs * blocks * parts(p.chunk_tokens);
+    p.second_grid = pairs * parts(64 * row_tiles(vectors));
+  }
+  p.max_chunks = (int32_t)parts(p.chunk_tokens);
+  p.stats_at = p.few ? (size_t)(a.total_rows * a.num_heads) * p.ctx_pad * sizeof(float) : 0;
+  return p;
 }
 
 hipError_t launch_attention_weights(int dtype, int cache_dtype, const WeightsArgs& a,
                                     const CacheGeom& g, hipStream_t stream) {
-  const Layout l = layout(a.total_rows, a.num_heads, a.max_ctx);
   const bool fp8 = cache_dtype == VPA_DTYPE_FP8_E4M3;
-  hipError_t e = hipErrorInvalidValue;
+  const WeightsPlan p = weights_plan(dtype, a, g);
   switch (dtype) {
     case VPA_DTYPE_F32:
-      e = fp8 ? logits_typed<float, fp8_t>(a, g, l, stream)
-              : logits_typed<float, float>(a, g, l, stream);
-      break;
+      return fp8 ? weights_typed<float, fp8_t>(a, p, g, stream)
+                 : weights_typed<float, float>(a, p, g, stream);
     case VPA_DTYPE_F16:
-      e = fp8 ? logits_typed<f16_t, fp8_t>(a, g, l, stream)
-              : logits_typed<f16_t, f16_t>(a, g, l, stream);
-      break;
+      return fp8 ? weights_typed<f16_t, fp8_t>(a, p, g, stream)
+                 : weights_typed<f16_t, f16_t>(a, p, g, stream);
     case VPA_DTYPE_BF16:
-      e = fp8 ? logits_typed<bf16_t, fp8_t>(a, g, l, stream)
-              : logits_typed<bf16_t, bf16_t>(a, g, l, stream);
-      break;
+      return fp8 ? weights_typed<bf16_t, fp8_t>(a, p, g, stream)
+                 : weights_typed<bf16_t, bf16_t>(a, p, g, stream);
   }
-  if (e != hipSuccess) return e;
-  const float* logits = static_cast<const float*>(a.workspace);
-  const float2* stats =
-      reinterpret_cast<const float2*>(static_cast<const char*>(a.workspace) + l.stats_at);
-  hipLaunchKernelGGL(weight_sum_kernel,
-                     dim3((uint32_t)((l.ctx_pad + 1023) / 1024), (uint32_t)g.num_kv_heads,
-                          (uint32_t)a.num_seqs),
-                     dim3(kThreads), 0, stream, a, g.num_kv_heads, g.block_size, logits, stats,
-                     l.ctx_pad, l.max_chunks);
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 }  // namespace vpa

@@ -106,6 +106,40 @@ def test_several_rows(device, dtype, fp8, causal):
     check(p, run(device, p, causal), causal)
 
 
+@pytest.mark.parametrize("dtype,fp8,d,bs", [(torch.bfloat16, False, 128, 16),
+                                            (torch.float32, False, 64, 8),
+                                            (torch.float16, True, 96, 32),
+                                            (torch.float32, True, 256, 16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_sequences(device, dtype, fp8, d, bs, causal):
+    """512 and more (sequence, kv head) pairs: contexts in one launch, the longest first;
+    ragged rows and lengths, some of them none."""
+    rng = np.random.default_rng(d)
+    lens = rng.integers(0, 150, size=131)
+    lens[[3, 77]] = [700, 1]
+    rows = np.minimum(rng.integers(0, 4, size=131), np.maximum(lens, 1))
+    p = problem(device, dtype, fp8, d, bs, 8, 4, lens, rows=rows, seed=21)
+    check(p, run(device, p, causal), causal)
+
+
+def test_more_sequences_than_are_ordered(device):
+    rng = np.random.default_rng(5)
+    p = problem(device, torch.bfloat16, False, 64, 16, 1, 1, rng.integers(0, 90, size=601), seed=22)
+    check(p, run(device, p))
+
+
+@pytest.mark.parametrize("dtype,fp8,d", [(torch.bfloat16, False, 64), (torch.float32, False, 64),
+                                         (torch.bfloat16, True, 192)])
+def test_many_rows_of_many_sequences(device, dtype, fp8, d):
+    """Chunks of several pieces, blocks of rows that are not full."""
+    rng = np.random.default_rng(6)
+    lens = rng.integers(1, 1100, size=48)
+    lens[0] = 2100
+    rows = np.minimum(rng.integers(0, 12, size=48), lens)
+    p = problem(device, dtype, fp8, d, 16, 18, 6, lens, rows=rows, seed=23)
+    check(p, run(device, p))
+
+
 def test_sum_of_weights(device):
     """Every row's weights sum to 1: 40 additions of 600 values, f32."""
     p = problem(device, torch.bfloat16, False, 128, 16, 16, 8, [600, 1, 4096], seed=1)
