@@ -92,16 +92,19 @@ def paged_attention_weights(q: torch.Tensor, key_cache: torch.Tensor,
     if cu_seqlens_q is not None:
         cu_seqlens_q = cu_seqlens_q.contiguous()
     with _on_device_of(q):
+        lib = _lib.load()
         if workspace is None:
-            workspace = paged_attention_weights_workspace(rows, h, int(max_context_len), q.device)
-        check(_lib.load().vpa_paged_attention_weights(
+            nbytes = lib.vpa_paged_attention_weights_workspace_size(rows, h, int(max_context_len))
+            workspace = context_lens.new_empty(((nbytes + 3) // 4,))
+        else:
+            nbytes = workspace.nbytes
+        check(lib.vpa_paged_attention_weights(
             scores.data_ptr(), seq_stride, head_stride, q.data_ptr(), _ptr(k_scale),
             key_cache.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
             _ptr(cu_seqlens_q), context_lens.data_ptr(), b, int(max_query_len),
             int(max_context_len), rows, float(softmax_scale), int(causal), h, kvh, d, bs, nb,
             key_cache.stride(0), key_cache.stride(1), dtype_code(q.dtype),
-            dtype_code(key_cache.dtype), _ptr(workspace),
-            0 if workspace is None else workspace.nbytes, _stream(q)))
+            dtype_code(key_cache.dtype), workspace.data_ptr(), nbytes, _stream(q)))
     return scores
 
 
@@ -137,24 +140,27 @@ def evict_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: t
         max_context_len = int(context_lens.long().max().item()) if b else 0
     seq_stride, head_stride = _score_strides(scores, b, kvh, int(max_context_len))
     if new_context_lens is None:
-        new_context_lens = torch.empty(b, dtype=torch.uint32, device=scores.device)
+        new_context_lens = context_lens.new_empty((b,))
     elif new_context_lens.dtype != torch.uint32 or new_context_lens.shape != (b,) or \
             not new_context_lens.is_contiguous():
         raise _err(f"new_context_lens must be a contiguous u32 [{b}] tensor")
     if kept is None:
-        kept = torch.empty((b, kvh, max(int(budget), 0)), dtype=torch.uint32, device=scores.device)
+        kept = context_lens.new_empty((b, kvh, max(int(budget), 0)))
     elif kept.dtype != torch.uint32 or kept.shape != (b, kvh, budget) or not kept.is_contiguous():
         raise _err(f"kept must be a contiguous u32 [{b}, {kvh}, {budget}] tensor")
     block_tables = block_tables.contiguous()
     context_lens = context_lens.contiguous()
     with _on_device_of(scores):
+        lib = _lib.load()
         if workspace is None:
-            workspace = evict_kv_cache_workspace(b, kvh, int(max_context_len), bs, scores.device)
-        check(_lib.load().vpa_evict_kv_cache(
+            nbytes = lib.vpa_evict_kv_cache_workspace_size(b, kvh, int(max_context_len), bs)
+            workspace = context_lens.new_empty(((nbytes + 3) // 4,))
+        else:
+            nbytes = workspace.nbytes
+        check(lib.vpa_evict_kv_cache(
             key_cache.data_ptr(), value_cache.data_ptr(), scores.data_ptr(), seq_stride,
             head_stride, block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(),
             new_context_lens.data_ptr(), kept.data_ptr(), b, int(max_context_len), int(budget),
             int(keep_first), int(keep_last), kvh, d, bs, nb, bstride, hstride,
-            dtype_code(key_cache.dtype), _ptr(workspace),
-            0 if workspace is None else workspace.nbytes, _stream(scores)))
+            dtype_code(key_cache.dtype), workspace.data_ptr(), nbytes, _stream(scores)))
     return new_context_lens, kept

@@ -90,7 +90,7 @@ def _norm(name: str, w: Optional[torch.Tensor], like: torch.Tensor) -> Optional[
 
 def _out(name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.dtype != like.dtype or _rows(name, out) is not out:
         raise _err(f"{name} must be shaped and typed like its input, heads contiguous")
     return out

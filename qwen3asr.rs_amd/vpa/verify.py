@@ -67,20 +67,22 @@ def verify_draft_tokens(target_logits: torch.Tensor, draft_ids: torch.Tensor,
             draft_logits = draft_logits.contiguous()
         ds, dr = draft_logits.stride(0), draft_logits.stride(1)
     if out is None:
-        ids = torch.empty((b, k1), dtype=torch.uint32, device=target_logits.device)
-        count = torch.empty(b, dtype=torch.uint32, device=target_logits.device)
+        ids, count = draft_ids.new_empty((b, k1)), draft_ids.new_empty((b,))
     else:
         ids, count = out
         if ids.dtype != torch.uint32 or ids.shape != (b, k1) or not ids.is_contiguous() or \
                 count.dtype != torch.uint32 or count.shape != (b,) or not count.is_contiguous():
             raise _err(f"out must be contiguous u32 [{b}, {k1}] and [{b}] tensors")
     with _on_device_of(target_logits):
+        lib = _lib.load()
         if workspace is None:
-            workspace = verify_draft_tokens_workspace(b, k, v, target_logits.device)
-        check(_lib.load().vpa_verify_draft_tokens(
+            nbytes = lib.vpa_verify_draft_tokens_workspace_size(b, k, v)
+            workspace = draft_ids.new_empty(((nbytes + 3) // 4,))
+        else:
+            nbytes = workspace.nbytes
+        check(lib.vpa_verify_draft_tokens(
             ids.data_ptr(), count.data_ptr(), target_logits.data_ptr(), target_logits.stride(0),
             target_logits.stride(1), _ptr(draft_logits), ds, dr, draft_ids.data_ptr(),
             _ptr(num_drafts), _ptr(temperature), accept_u.data_ptr(), sample_u.data_ptr(), b, k, v,
-            dtype_code(target_logits.dtype), _ptr(workspace),
-            0 if workspace is None else workspace.nbytes, _stream(target_logits)))
+            dtype_code(target_logits.dtype), workspace.data_ptr(), nbytes, _stream(target_logits)))
     return ids, count
