@@ -536,6 +536,7 @@ class DeviceBlockAllocator:
         if num_tokens.dtype != torch.uint32 or num_tokens.shape != (self.batch,):
             raise _err(f"num_tokens must be u32 [{self.batch}], got {num_tokens.dtype} "
                        f"{tuple(num_tokens.shape)}")
+        _require_device(num_tokens, self.positions)
         self.positions.copy_(num_tokens)
         bs = self.block_size
         # (u32 arithmetic through the bits: torch has none of its own)
