@@ -572,10 +572,10 @@ __global__ __launch_bounds__(kThreads, (kRowWaves<T, C>)) void weight_rows_kerne
     if (threadIdx.x < RB)
       s_see[threadIdx.x] = m >= m_count ? 0 : a.causal ? min(L, m / group + 1 + L - rows.n) : L;
   };
-  // the products of a block's rows: visit(first of the lane's four rows in the block, acc)
-  auto block_rows = [&](int n, auto visit) {
+  // the products of rows from .. to of the block: visit(first of the lane's four rows, acc)
+  auto block_rows = [&](int from, int to, auto visit) {
 #pragma unroll 1
-    for (int m0 = 0; m0 < n; m0 += 16) {
+    for (int m0 = from; m0 < to; m0 += 16) {
       asm volatile("" ::: "memory");  // (no later read of LDS moves up: registers)
       f32x4_t acc[TW];
 #pragma unroll
@@ -631,7 +631,7 @@ __global__ __launch_bounds__(kThreads, (kRowWaves<T, C>)) void weight_rows_kerne
         }
       };
       if (all_seen(t_wave)) {
-        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+        block_rows(0, n, [&](int mi, const f32x4_t(&acc)[TW]) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float l[TW];
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(kThreads, (kRowWaves<T, C>)) void weight_rows_kerne
           }
         });
       } else {
-        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+        block_rows(0, n, [&](int mi, const f32x4_t(&acc)[TW]) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float l[TW];
@@ -675,11 +675,13 @@ __global__ __launch_bounds__(kThreads, (kRowWaves<T, C>)) void weight_rows_kerne
       const int m = threadIdx.x / kLanes, part = threadIdx.x % kLanes;
       const float2 row =
           merge_row<kLanes>(stats + row_of(min(m_at + m, m_count - 1)) * max_chunks, chunks, part);
-      // (rows past the last have queries of zero: their weights are 1 * 0)
-      if (part == 0) s_row[0][m] = m < n ? row : make_float2(0.f, 0.f);
+      if (part == 0) s_row[0][m] = row;
       lds_group_barrier();
-      if (all_seen(t_wave)) {
-        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+      // (tiles with rows past the last take the masked form: an infinite key has no
+      // product with a query of zeros)
+      const int plain = all_seen(t_wave) ? n & ~15 : 0;
+      if (plain > 0) {
+        block_rows(0, plain, [&](int mi, const f32x4_t(&acc)[TW]) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float2 row = s_row[0][mi + k];
@@ -688,8 +690,9 @@ __global__ __launch_bounds__(kThreads, (kRowWaves<T, C>)) void weight_rows_kerne
               sum[u] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[u][k], scale, -row.x)), row.y, sum[u]);
           }
         });
-      } else {
-        block_rows(n, [&](int mi, const f32x4_t(&acc)[TW]) {
+      }
+      if (plain < n) {
+        block_rows(plain, n, [&](int mi, const f32x4_t(&acc)[TW]) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float2 row = s_row[0][mi + k];

@@ -192,6 +192,42 @@ def test_nan_query_marks_its_own_scores_only(device):
     assert torch.equal(got[keep], clean[keep])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 9, 33])
+def test_infinite_keys(device, dtype, rows):
+    """A key of -inf against positive queries has weight 0, whatever rows share its tile."""
+    p = problem(device, dtype, False, 64, 16, 4, 2, [300, 40], rows=[rows, rows], seed=9)
+    p["q"][..., 3] = p["q"][..., 3].abs() + 1
+    blk = int(p["tables"][0, 2])
+    x = p["kc"].shape[-1]
+    p["kc"][blk, :, 3 // x, 7, 3 % x] = float("-inf")
+    p["keys"][blk, :, 3 // x, 7, 3 % x] = -np.inf
+    got = run(device, p)
+    assert torch.equal(got[0, :, 39], p["scores"][0, :, 39])
+    p["keys"][blk, :, 3 // x, 7, 3 % x] = -1e6  # (as far as exp is concerned)
+    size = np64(p["q"])
+    want = ref.attention_weights(size, p["keys"], p["tables"], p["lens"], 0.125, np64(p["scores"]),
+                                 p["cu"], True)
+    p["keys"][blk, :, 3 // x, 7, 3 % x] = 0  # the bound is that of the finite keys
+    rel = 2 * 67 * U * 0.125 * np.abs(size).sum(-1).max() * np.abs(p["keys"]).max()
+    rel += (24 + 2 * 0.125 * np.abs(size).sum(-1).max() * np.abs(p["keys"]).max()) * U
+    tol = (want - np64(p["scores"])) * rel + want * (rows * 2 + 2) * U
+    assert np.all(np.abs(np64(got) - want) <= tol)
+
+
+def test_longest_context_held_in_one_workgroup(device):
+    """512 pairs of one row each, the logits of 16384 tokens in LDS; one token more takes
+    two launches."""
+    lens = np.full(64, 5)
+    lens[40] = 16384
+    p = problem(device, torch.bfloat16, False, 64, 32, 8, 8, lens, seed=10)
+    check(p, run(device, p))
+    wide = np.concatenate([p["tables"], np.zeros((64, 1), np.uint32)], 1)
+    a = dict(p, tables=wide, scores=torch.nn.functional.pad(p["scores"], (0, 32)))
+    got = run(device, a, max_context_len=16385)
+    check(a, got)
+
+
 def test_large_logits(device):
     """Logits of several hundred: one weight takes it all."""
     p = problem(device, torch.float32, False, 64, 16, 4, 2, [500, 3], seed=5, scale_q=40.0)
