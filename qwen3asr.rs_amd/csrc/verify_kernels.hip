@@ -18,18 +18,18 @@
 // the cumulative sum is off by 2^-24 of the total, more than many of its 150 000 steps,
 // so weights and sums are f64 throughout, exponentials included (within 4e-14). The
 // f64 instructions of the exponentials, not the logits' bytes, bound the calls with
-// draft logits: 93 cycles of a SIMD per 64 logits, 85 us for the 87.5 million of 64
-// sequences with four drafts (151 936 tokens, bf16; 175 MB, 27 us at the streaming
-// rate). f32 first and f64 for the drawn row alone needs that row read once more by a
-// launch of its own and took 148 us against 121 in all.
+// draft logits: 17 of them, 93 cycles of a SIMD, per 64 logits, 62 of the 75 us that the
+// 87.5 million of 64 sequences with four drafts take (151 936 tokens, bf16; 175 MB, 27
+// us at the streaming rate). f32 first and f64 for the drawn row alone needs that row
+// read once more by a launch of its own and took 148 us in all against 121 then.
 //
 // Launches, over segments of 4096 logits: stats (every row's segment maxima and sums,
 // or first maxima: each logit is read once), rest (max(p - q, 0) needs both rows'
 // totals first; only where drafts have logits), draw (the segment, then the place in
 // it). Rest and draw merge the stats and test the drafts themselves (pick_row: cheaper
-// than a launch between them). Measured: 64 sequences as above 85 + 26 + 10 us; one
+// than a launch between them). Measured: 64 sequences as above 75 + 24 + 11 us; one
 // sequence of four drafts without logits 4.3 + 9.6; 128 of up to three, greedy (156
-// MB), 27 + 4.
+// MB), 20 + 4.
 
 #include <float.h>
 #include <math.h>
@@ -124,22 +124,22 @@ __device__ __forceinline__ const T* draft_row(const VerifyArgs& a, int b, int i)
   return static_cast<const T*>(a.draft) + b * a.draft_seq_stride + i * a.draft_row_stride;
 }
 
-// The thread's 16 logits of a segment, -inf past the row: vector q = tid + 256 i
-// of the segment, so element e of it is logit seg * 4096 + q * X + e.
-template <typename T>
-__device__ __forceinline__ void load_segment(const T* row, int seg, int vocab, bool vec_ok,
-                                             float (&f)[kPer]) {
-  constexpr int X = pack_x<T>();
+// One of N threads' logits of a segment, -inf past the row: vector q = t + N i of the
+// segment, so element e of it is logit seg * 4096 + q * X + e.
+template <typename T, int N>
+__device__ __forceinline__ void load_segment(const T* row, int t, int seg, int vocab, bool vec_ok,
+                                             float (&f)[kSeg / N]) {
+  constexpr int X = pack_x<T>(), kPer = kSeg / N;
   uint4 u[kPer / X];
 #pragma unroll
   for (int i = 0; i < kPer / X; ++i) {
-    const int at = seg * kSeg + ((int)threadIdx.x + kThreads * i) * X;
+    const int at = seg * kSeg + (t + N * i) * X;
     u[i] = make_uint4(0u, 0u, 0u, 0u);
     if (vec_ok && at + X <= vocab) u[i] = load_stream(reinterpret_cast<const uint4*>(row + at));
   }
 #pragma unroll
   for (int i = 0; i < kPer / X; ++i) {
-    const int at = seg * kSeg + ((int)threadIdx.x + kThreads * i) * X;
+    const int at = seg * kSeg + (t + N * i) * X;
     if (vec_ok && at + X <= vocab) {
       const T* e = reinterpret_cast<const T*>(&u[i]);
 #pragma unroll
@@ -151,10 +151,10 @@ __device__ __forceinline__ void load_segment(const T* row, int seg, int vocab, b
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ int segment_index(int seg, int k) {  // logit of f[k]
+template <typename T, int N>
+__device__ __forceinline__ int segment_index(int t, int seg, int k) {  // logit of f[k]
   constexpr int X = pack_x<T>();
-  return seg * kSeg + ((int)threadIdx.x + kThreads * (k / X)) * X + k % X;
+  return seg * kSeg + (t + N * (k / X)) * X + k % X;
 }
 
 template <int kCtrl>
@@ -199,42 +199,54 @@ __device__ __forceinline__ void take_best(Best& a, float v, uint32_t i) {
   if (v > a.v || (v == a.v && i < a.i)) a = {v, i};
 }
 
-template <typename T>
+// Statistics of each segment of each row, by kWaves waves: four where there are few
+// segments; else one, whose reductions and addresses serve 64 logits of a thread
+// instead of 16.
+template <typename T, int kWaves>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a, Buffers w,
                                                                 bool vec_ok) {
+  constexpr int N = 64 * kWaves, kPer = kSeg / N;
   __shared__ float s_m[4];
   __shared__ uint32_t s_i[4];
   __shared__ double s_s[4];
   const int rows_t = a.num_seqs * (a.max_drafts + 1);
-  const int r = (int)(blockIdx.x / (uint32_t)w.segs);
-  const int seg = (int)(blockIdx.x - (uint32_t)r * (uint32_t)w.segs);
+  const int rows = rows_t + (a.draft == nullptr ? 0 : a.num_seqs * a.max_drafts);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const uint32_t unit = kWaves == 4 ? blockIdx.x : blockIdx.x * 4 + (uint32_t)wave;
+  const int r = (int)(unit / (uint32_t)w.segs);
+  if (r >= rows) return;  // (whole units; of four waves, whole workgroups)
+  const int seg = (int)(unit - (uint32_t)r * (uint32_t)w.segs);
+  const int t = kWaves == 4 ? (int)threadIdx.x : lane;
   const bool is_target = r < rows_t;
   const int per = is_target ? a.max_drafts + 1 : a.max_drafts;
   const int rr = is_target ? r : r - rows_t;
   const int b = rr / per, i = rr - b * per;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float temp = seq_temperature(a, b);
   const bool greedy = !(temp > 0.f);
   if (i >= seq_drafts(a, b) + (is_target ? 1 : 0) || (greedy && !is_target)) return;
   float f[kPer];
-  load_segment<T>(is_target ? target_row<T>(a, b, i) : draft_row<T>(a, b, i), seg, a.vocab, vec_ok,
-                  f);
+  load_segment<T, N>(is_target ? target_row<T>(a, b, i) : draft_row<T>(a, b, i), t, seg, a.vocab,
+                     vec_ok, f);
   const int64_t at = (int64_t)r * w.segs + seg;
   if (greedy) {
     Best best{-INFINITY, kNone};
 #pragma unroll
     for (int k = 0; k < kPer; ++k)  // (indices ascend with k; a NaN is never greater)
-      if (f[k] > best.v) best = {f[k], (uint32_t)segment_index<T>(seg, k)};
+      if (f[k] > best.v) best = {f[k], (uint32_t)segment_index<T, N>(t, seg, k)};
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1)
       take_best(best, __shfl_xor(best.v, m, 64), __shfl_xor(best.i, m, 64));
-    if (lane == 0) {
-      s_m[wave] = best.v;
-      s_i[wave] = best.i;
+    if constexpr (kWaves == 4) {
+      if (lane == 0) {
+        s_m[wave] = best.v;
+        s_i[wave] = best.i;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0)
+        for (int v = 1; v < 4; ++v) take_best(best, s_m[v], s_i[v]);
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int v = 1; v < 4; ++v) take_best(best, s_m[v], s_i[v]);
+    if (t == 0) {
       w.max[at] = best.v;
       w.sum[at] = __builtin_bit_cast(double, (uint64_t)best.i);
     }
@@ -245,9 +257,11 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a, Bu
   for (int k = 1; k < kPer; ++k) mx = fmaxf(mx, f[k]);  // (a NaN loses)
   mx = fmaxf(mx, -INFINITY);
   mx = wave_max_dpp(mx);
-  if (lane == 0) s_m[wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  if constexpr (kWaves == 4) {
+    if (lane == 0) s_m[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  }
   const Scale sc(mx, temp);
   double s0 = 0.0, s1 = 0.0;
   if (sc.odd) {
@@ -260,8 +274,10 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a, Bu
       s1 += sc.plain(f[k + 1]);
     }
   }
-  const double sum = group_sum_f64(s0 + s1, s_s);
-  if (threadIdx.x == 0) {
+  double sum;
+  if constexpr (kWaves == 4) sum = group_sum_f64(s0 + s1, s_s);
+  else sum = wave_sum_f64(s0 + s1);
+  if (t == 0) {
     w.max[at] = mx;
     w.sum[at] = sum;
   }
@@ -430,27 +446,33 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a, Buf
                                                                bool vec_ok) {
   __shared__ PickShared sh;
   __shared__ double s4[4];
-  const int seg = blockIdx.x, b = blockIdx.y;
+  const int b = blockIdx.y;
   const Pick p = pick_row<T, kThreads, 16>(a, w, b, sh);
   if (p.greedy || !p.rejected) return;
   const float temp = seq_temperature(a, b);
-  float f[kPer], d[kPer];
-  load_segment<T>(target_row<T>(a, b, p.took), seg, a.vocab, vec_ok, f);
-  load_segment<T>(draft_row<T>(a, b, p.took), seg, a.vocab, vec_ok, d);
   const Scale sp(p.max_p, temp), sq(p.max_q, temp);
   const double inv_p = inverse(p.sum_p), inv_q = inverse(p.sum_q);
-  double r = 0.0;
-  if (sp.odd || sq.odd) {
+  const T* rt = target_row<T>(a, b, p.took);
+  const T* rd = draft_row<T>(a, b, p.took);
 #pragma unroll 1
-    for (int k = 0; k < kPer; ++k)
-      r += residual(sp.weight(f[k]), sq.weight(d[k]), inv_p, inv_q);
-  } else {
+  for (int seg = blockIdx.x; seg < w.segs; seg += gridDim.x) {
+    float f[kPer], d[kPer];
+    load_segment<T, kThreads>(rt, threadIdx.x, seg, a.vocab, vec_ok, f);
+    load_segment<T, kThreads>(rd, threadIdx.x, seg, a.vocab, vec_ok, d);
+    double r = 0.0;
+    if (sp.odd || sq.odd) {
+#pragma unroll 1
+      for (int k = 0; k < kPer; ++k)
+        r += residual(sp.weight(f[k]), sq.weight(d[k]), inv_p, inv_q);
+    } else {
 #pragma unroll
-    for (int k = 0; k < kPer; ++k)
-      r += residual(sp.plain(f[k]), sq.plain(d[k]), inv_p, inv_q);
+      for (int k = 0; k < kPer; ++k)
+        r += residual(sp.plain(f[k]), sq.plain(d[k]), inv_p, inv_q);
+    }
+    r = group_sum_f64(r, s4);
+    if (threadIdx.x == 0) w.rest[(int64_t)b * w.segs + seg] = r;
+    __syncthreads();  // (s4 is read)
   }
-  r = group_sum_f64(r, s4);
-  if (threadIdx.x == 0) w.rest[(int64_t)b * w.segs + seg] = r;
 }
 
 constexpr int kDrawThreads = 1024;
@@ -666,10 +688,21 @@ hipError_t verify_typed(const VerifyArgs& a, hipStream_t stream) {
   const bool vec_ok = whole(a.target, a.target_seq_stride, a.target_row_stride) &&
                       whole(a.draft, a.draft_seq_stride, a.draft_row_stride);
   const int rows = a.num_seqs * (a.max_drafts + 1) + (a.draft == nullptr ? 0 : a.num_seqs * a.max_drafts);
-  hipLaunchKernelGGL(verify_stats_kernel<T>, dim3((uint32_t)z.segs * (uint32_t)rows),
-                     dim3(kThreads), 0, stream, a, w, vec_ok);
+  const uint32_t units = (uint32_t)z.segs * (uint32_t)rows;
+  // (9728 segments of one sequence's row each take 43 us in all, 45 by four waves; 190
+  // take 16, 13 by four)
+  if (units >= 4096)
+    hipLaunchKernelGGL((verify_stats_kernel<T, 1>), dim3((units + 3) / 4), dim3(kThreads), 0, stream,
+                       a, w, vec_ok);
+  else
+    hipLaunchKernelGGL((verify_stats_kernel<T, 4>), dim3(units), dim3(kThreads), 0, stream, a, w,
+                       vec_ok);
+  // (two segments to a workgroup share its merge of the stats where every compute unit
+  // has eight: 24 us for 64 sequences of 151 936 tokens, 27 one by one, 27 by three)
+  const int per_group = z.segs * a.num_seqs >= 2048 ? 2 : 1;
   if (a.draft != nullptr)
-    hipLaunchKernelGGL(verify_rest_kernel<T>, dim3((uint32_t)z.segs, (uint32_t)a.num_seqs),
+    hipLaunchKernelGGL(verify_rest_kernel<T>,
+                       dim3((uint32_t)((z.segs + per_group - 1) / per_group), (uint32_t)a.num_seqs),
                        dim3(kThreads), 0, stream, a, w, vec_ok);
   hipLaunchKernelGGL(verify_draw_kernel<T>, dim3((uint32_t)a.num_seqs), dim3(kDrawThreads), 0,
                      stream, a, w, vec_ok);

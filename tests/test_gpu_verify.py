@@ -77,6 +77,18 @@ def test_large_vocabulary(device, draft):
     check(device, p)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("b,k,v", [(600, 3, 50), (300, 3, 4097), (700, 1, 8200)])
+def test_many_sequences(device, dtype, b, k, v):
+    """4096 segments and more: a wave each, with odd logits among them."""
+    p = problem(dtype, b, k, v, draft=True, seed=b, ragged=True, greedy=(2, 5, b - 1))
+    p["target"][9, 0, ::2] = float("nan")
+    p["target"][10, 0] = torch.finfo(dtype).min
+    p["target"][11, 0, 7] = float("inf")
+    p["target"][12, 0] = float("-inf")
+    check(device, p)
+
+
 def test_flat_rows_of_a_large_vocabulary(device):
     """Every token about as likely as the next: the draw's sum has 100 000 borders."""
     p = problem(torch.float32, 24, 1, 100003, draft=True, spread=0.01, noise=0.01, seed=4)
