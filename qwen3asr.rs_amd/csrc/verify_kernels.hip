@@ -18,7 +18,7 @@
 // the cumulative sum is off by 2^-24 of the total, more than many of its 150 000 steps,
 // so weights and sums are f64 throughout, exponentials included (within 4e-14). The
 // f64 instructions of the exponentials, not the logits' bytes, bound the calls with
-// draft logits: 17 of them, 93 cycles of a SIMD, per 64 logits, 62 of the 75 us that the
+// draft logits: 17 of them, 93 cycles of a SIMD, per 64 logits, 62 of the 73 us that the
 // 87.5 million of 64 sequences with four drafts take (151 936 tokens, bf16; 175 MB, 27
 // us at the streaming rate). f32 first and f64 for the drawn row alone needs that row
 // read once more by a launch of its own and took 148 us in all against 121 then.
@@ -27,7 +27,7 @@
 // or first maxima: each logit is read once), rest (max(p - q, 0) needs both rows'
 // totals first; only where drafts have logits), draw (the segment, then the place in
 // it). Rest and draw merge the stats and test the drafts themselves (pick_row: cheaper
-// than a launch between them). Measured: 64 sequences as above 75 + 24 + 11 us; one
+// than a launch between them). Measured: 64 sequences as above 73 + 24 + 11 us; one
 // sequence of four drafts without logits 4.3 + 9.6; 128 of up to three, greedy (156
 // MB), 20 + 4.
 
