@@ -80,9 +80,9 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
   constexpr int kWaves = kThreads / 64;
   constexpr int kChunk = kThreads * kItems;
   constexpr int kPer = kBins / kThreads;  // bins per thread
-  __shared__ int s_hist[kBins];
+  __shared__ int s_hist[3][kBins];  // (a digit's each: cleared at once)
   __shared__ int s_w[2][kWaves];
-  __shared__ int s_digit, s_rank;
+  __shared__ int s_digit, s_rank, s_count;
   const int j = (int)(blockIdx.x % (uint32_t)num_kv_heads);
   const int s = (int)(blockIdx.x / (uint32_t)num_kv_heads);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -120,6 +120,9 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
     asm volatile("" : "+v"(inside), "+v"(middle));
   };
   load_chunk(0);
+#pragma unroll
+  for (int i = tid; i < 3 * kBins; i += kThreads) s_hist[i / kBins][i % kBins] = 0;
+  __syncthreads();
 
   // threshold: `prefix` is the pattern of the want-th highest score of the
   // middle, `rank` how many scores equal to it are kept
@@ -132,8 +135,6 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
       const int bits = pass < 2 ? 11 : 10;
       const uint32_t seen = pass == 0 ? 0u : 0xffffffffu << shift;
       shift -= bits;
-      for (int i = tid; i < kBins; i += kThreads) s_hist[i] = 0;
-      __syncthreads();
       for (int c = 0; c < chunks; ++c) {
         if (chunks > 1) load_chunk(c);
         const int R = items_of(c);
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
           if (i >= R) continue;  // (uniform)
           const uint32_t key = score_key(f[i]);
           if (((middle >> i) & 1u) && (key & seen) == prefix)
-            atomicAdd(&s_hist[(key >> shift) & ((1u << bits) - 1)], 1);
+            atomicAdd(&s_hist[pass][(key >> shift) & ((1u << bits) - 1)], 1);
         }
       }
       __syncthreads();
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
       int n[kPer], mine = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        n[i] = s_hist[b - i];
+        n[i] = s_hist[pass][b - i];
         mine += n[i];
       }
       int total;
@@ -164,6 +165,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
           if (before < rank && rank <= before + n[i]) {
             s_digit = b - i;
             s_rank = rank - before;
+            s_count = n[i];
           }
           before += n[i];
         }
@@ -171,6 +173,13 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
       __syncthreads();
       prefix |= (uint32_t)s_digit << shift;
       rank = s_rank;
+      // all scores of the digit stay (often one, after two digits): they are above the
+      // pattern before its first
+      if (pass == 1 && rank == s_count && prefix != 0) {
+        --prefix;
+        rank = 0;
+        break;
+      }
     }
   }
   // in token order: kept indices, moved scores, and each table column's kept
