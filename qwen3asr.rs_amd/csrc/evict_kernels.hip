@@ -271,7 +271,8 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a, int
 // tokens; 197 us so.) Reading whole columns costs nothing: a value row's 32-byte
 // sector holds 16 tokens. The next two batches' runs are in flight while one is
 // written: they lie behind everything that is written (a place is at or before
-// the token that moves to it). Columns before the first evicted token stay.
+// the token that moves to it). Columns before the first evicted token stay, and
+// columns without kept tokens are left out of the batches.
 // E: cache element, moved as it is; BS tokens per block; NV vectors per thread and
 // batch.
 template <typename E, int BS, int DG, int kThreads, int NV>
@@ -294,12 +295,14 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
   constexpr int kInfo = 512;  // columns whose masks, places and blocks wait in LDS
   static_assert(DG % X == 0 && kThreads * NV % VPB == 0 && kCols >= 1 && kInfo % (2 * kCols) == 0,
                 "whole chunks, columns and pairs of batches");
+  static_assert(kThreads == kInfo, "a column per thread");
   __shared__ __align__(16) E s_run[kCols * RUN];
   __shared__ __align__(16) uint32_t s_src[kTok + 2 * U];  // of each place: its token's byte in s_run
   __shared__ uint2 s_col[kInfo];                          // {mask, place of the first kept token}
   // offsets (elements) of the blocks of the columns and of the places, -1: absent
   __shared__ int64_t s_from[kInfo], s_to[kInfo + 1];
-  __shared__ int s_p1, s_absent[2];
+  __shared__ uint16_t s_list[kInfo];  // the columns with kept tokens
+  __shared__ int s_p1, s_absent[2], s_listed[kThreads / 64];
   const int groups = head_dim / DG;
   uint32_t w = blockIdx.x;
   const int dg = (int)(w % (uint32_t)groups);
@@ -359,21 +362,34 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
       }
     }
     __syncthreads();
+    // the columns that move, in order
+    const bool moves = tid < n && (!whole || tid >= c_begin) && s_col[tid].x != 0;
+    const uint64_t mask = __ballot(moves);
+    if ((tid & 63) == 0) s_listed[tid >> 6] = __builtin_popcountll(mask);
+    __syncthreads();
+    int before = 0, listed = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+      before += i < tid >> 6 ? s_listed[i] : 0;
+      listed += s_listed[i];
+    }
+    if (moves) s_list[before + __builtin_popcountll(mask & ((1ull << (tid & 63)) - 1))] = (uint16_t)tid;
+    __syncthreads();
     // (a column whose block is not one of the pool's is neither read nor moved)
     auto load_data = [&](uint4(&u)[NV], int c0) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = uniform(c0 + (k * kThreads + tid) / VPB);
         u[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (c < n && uniform((int)s_col[c].x) != 0) {
-          const int64_t at = uniform64(s_from[c]);
+        if (c < listed) {
+          const int64_t at = uniform64(s_from[s_list[c]]);
           if (at >= 0)
             u[k] = load_stream(reinterpret_cast<const uint4*>(cache + at) + (k * kThreads + tid) % VPB);
         }
       }
     };
     auto batch = [&](uint4(&u)[NV], int c0) {
-      const int c_last = min(c0 + kCols, n) - 1;
+      const int c_last = min(c0 + kCols, listed) - 1;
       const int aligned = p0 / U * U;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -390,9 +406,10 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
       for (int i = tid; i < kTok; i += kThreads) {
         const int off = i % BS, c = c0 + i / BS;
         if (c > c_last) break;
-        const uint2 col = s_col[c];
+        const int at = s_list[c];
+        const uint2 col = s_col[at];
         if ((col.x >> off) & 1u) {
-          const bool there = s_from[c] >= 0;
+          const bool there = s_from[at] >= 0;
           s_src[(int)col.y + __builtin_popcount(col.x & ((1u << off) - 1u)) - aligned] =
               there ? (uint32_t)(i / BS * RUN + (value ? off : off * X)) * EB : kNone;
           if (!there) s_absent[flip] = 1;
@@ -447,12 +464,11 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
       lds_group_barrier();  // (LDS is read)
     };
     uint4 even[NV], odd[NV];
-    const int first = whole ? c_begin : 0;
-    load_data(even, first);
-    load_data(odd, first + kCols);
-    for (int c0 = first; c0 < n; c0 += 2 * kCols) {
+    load_data(even, 0);
+    load_data(odd, kCols);
+    for (int c0 = 0; c0 < listed; c0 += 2 * kCols) {
       batch(even, c0);
-      if (c0 + kCols < n) batch(odd, c0 + kCols);
+      if (c0 + kCols < listed) batch(odd, c0 + kCols);
     }
   }
 }

@@ -114,6 +114,20 @@ def test_long_sequence(device):
     check(p, run(device, p, 19000, 4, 64), 19000, 4, 64)
 
 
+@pytest.mark.parametrize("elem,bs,d", [(1, 8, 64), (2, 16, 128), (2, 8, 96), (4, 32, 64)])
+@pytest.mark.parametrize("budget,first,last", [(5, 0, 0), (40, 1, 3), (300, 260, 20)])
+def test_most_columns_empty(device, elem, bs, d, budget, first, last):
+    """Few tokens stay of contexts of several table windows and of one: whole stretches
+    of columns, and whole windows, keep nothing."""
+    lens = [600 * bs + 5, 1100 * bs + 1, 511 * bs + 3, 512 * bs, 40 * bs]
+    p = problem(device, elem, 2, d, bs, lens, seed=budget + d)
+    p["scores"][1, 0, 20 * bs:] = 0.0    # nothing behind but the last
+    p["scores"][0, 1, :560 * bs] = -1.0  # nothing before
+    check(p, run(device, p, budget, first, last), budget, first, last)
+    got = run(device, p, budget, first, last, max_context_len=512 * bs)
+    check(p, got, budget, first, last, lens=np.minimum(lens, 512 * bs))
+
+
 def test_already_sorted_prefix_stays(device):
     """The highest scores in front: nothing moves; in the back: everything does."""
     p = problem(device, 2, 2, 128, 16, [1500, 1500], seed=5)
