@@ -43,19 +43,16 @@ def rotary_frequencies(rotary_dim: int, theta: float, device, *,
     return inv_freq, torch.tensor(axes, dtype=torch.uint8, device=device)
 
 
-def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
-    """[T, heads, D] with contiguous heads, as it is or copied."""
+def _rows(name: str, t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """([T, heads, D] with contiguous heads, as it is or copied; its token stride)."""
     if t.dim() != 3:
         raise _err(f"{name} must be [T, heads, D], got {tuple(t.shape)}")
-    _, h, d = t.shape
-    if t.stride(2) != 1 or (t.stride(1) != d and h > 1) or (t.stride(0) < h * d and t.shape[0] > 1):
-        return t.contiguous()
-    return t
-
-
-def _token_stride(t: torch.Tensor) -> int:
+    n, h, d = t.shape
+    st, sh, sd = t.stride()
+    if sd != 1 or (sh != d and h > 1) or (st < h * d and n > 1):
+        return t.contiguous(), h * d
     # (a single row's stride is never stepped over: torch leaves anything there)
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return t, st if n > 1 else h * d
 
 
 def _tables(positions, inv_freq, axes, tokens):
@@ -88,12 +85,14 @@ def _norm(name: str, w: Optional[torch.Tensor], like: torch.Tensor) -> Optional[
     return w
 
 
-def _out(name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+def _out(name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> Tuple[torch.Tensor, int]:
     if out is None:
-        return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if out.shape != like.shape or out.dtype != like.dtype or _rows(name, out) is not out:
+        return (torch.empty_like(like, memory_format=torch.contiguous_format),
+                like.shape[1] * like.shape[2])
+    rows, stride = _rows(name, out)
+    if out.shape != like.shape or out.dtype != like.dtype or rows is not out:
         raise _err(f"{name} must be shaped and typed like its input, heads contiguous")
-    return out
+    return out, stride
 
 
 def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -109,20 +108,19 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
     ``rotary_frequencies`` gives them. Split pairs (i, i + R/2), or with
     ``adjacent`` (2i, 2i + 1). ``out_q`` / ``out_k`` may be q and k themselves."""
     _require_device(q, k, positions, inv_freq, axes, q_norm, k_norm, out_q, out_k)
-    q, k = _rows("q", q), _rows("k", k)
+    (q, qs), (k, ks) = _rows("q", q), _rows("k", k)
     t, h, d = q.shape
     if k.shape[0] != t or k.shape[2] != d or k.dtype != q.dtype:
         raise _err(f"k must be {q.dtype} [{t}, kv_heads, {d}], got {k.dtype} {tuple(k.shape)}")
     positions, stride, is64, num_axes, rot = _tables(positions, inv_freq, axes, t)
     _norm("q_norm", q_norm, q)
     _norm("k_norm", k_norm, k)
-    out_q, out_k = _out("out_q", out_q, q), _out("out_k", out_k, k)
+    (out_q, oqs), (out_k, oks) = _out("out_q", out_q, q), _out("out_k", out_k, k)
     with _on_device_of(q):
         check(_lib.load().vpa_rotary_qk(
-            out_q.data_ptr(), out_k.data_ptr(), q.data_ptr(), k.data_ptr(), _token_stride(out_q),
-            _token_stride(out_k), _token_stride(q), _token_stride(k), positions.data_ptr(), stride,
-            is64, inv_freq.data_ptr(), _ptr(axes), num_axes, rot, int(adjacent), _ptr(q_norm),
-            _ptr(k_norm), float(norm_eps), t, h, k.shape[1], d, dtype_code(q.dtype), _stream(q)))
+            out_q.data_ptr(), out_k.data_ptr(), q.data_ptr(), k.data_ptr(), oqs, oks, qs, ks,
+            positions.data_ptr(), stride, is64, inv_freq.data_ptr(), _ptr(axes), num_axes, rot,
+            int(adjacent), _ptr(q_norm), _ptr(k_norm), float(norm_eps), t, h, k.shape[1], d, dtype_code(q.dtype), _stream(q)))
     return out_q, out_k
 
 
@@ -141,7 +139,7 @@ def rotary_reshape_and_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require_device(q, k, v, positions, inv_freq, axes, k_scale, v_scale, key_cache, value_cache,
                     slot_mapping, q_norm, k_norm, out)
     nb, kvh, d, bs, bstride, hstride = cache_geometry(key_cache, value_cache)
-    q, k, v = _rows("q", q), _rows("k", k), _rows("v", v)
+    (q, qs), (k, ks), (v, vs) = _rows("q", q), _rows("k", k), _rows("v", v)
     t, h, qd = q.shape
     if qd != d or k.shape != (t, kvh, d) or v.shape != k.shape:
         raise _err(f"q, k and v must be [{t}, heads, {d}] and twice [{t}, {kvh}, {d}], got "
@@ -154,14 +152,14 @@ def rotary_reshape_and_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     positions, stride, is64, num_axes, rot = _tables(positions, inv_freq, axes, t)
     _norm("q_norm", q_norm, q)
     _norm("k_norm", k_norm, k)
-    out = _out("out", out, q)
+    out, outs = _out("out", out, q)
     slot_mapping = slot_mapping.contiguous()
     with _on_device_of(q):
         check(_lib.load().vpa_rotary_reshape_and_cache(
-            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _token_stride(out),
-            _token_stride(q), _token_stride(k), _token_stride(v), positions.data_ptr(), stride,
-            is64, inv_freq.data_ptr(), _ptr(axes), num_axes, rot, int(adjacent), _ptr(q_norm),
-            _ptr(k_norm), float(norm_eps), _ptr(k_scale), _ptr(v_scale), key_cache.data_ptr(),
+            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), outs, qs, ks,
+            vs,
+            positions.data_ptr(), stride, is64, inv_freq.data_ptr(), _ptr(axes), num_axes, rot,
+            int(adjacent), _ptr(q_norm), _ptr(k_norm), float(norm_eps), _ptr(k_scale), _ptr(v_scale), key_cache.data_ptr(),
             value_cache.data_ptr(), slot_mapping.data_ptr(), t, h, kvh, d, bs, nb, bstride, hstride,
             dtype_code(q.dtype), dtype_code(key_cache.dtype), _stream(q)))
     return out
