@@ -120,7 +120,8 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
         check(_lib.load().vpa_rotary_qk(
             out_q.data_ptr(), out_k.data_ptr(), q.data_ptr(), k.data_ptr(), oqs, oks, qs, ks,
             positions.data_ptr(), stride, is64, inv_freq.data_ptr(), _ptr(axes), num_axes, rot,
-            int(adjacent), _ptr(q_norm), _ptr(k_norm), float(norm_eps), t, h, k.shape[1], d, dtype_code(q.dtype), _stream(q)))
+            int(adjacent), _ptr(q_norm), _ptr(k_norm), float(norm_eps), t, h, k.shape[1], d,
+            dtype_code(q.dtype), _stream(q)))
     return out_q, out_k
 
 
@@ -156,10 +157,9 @@ def rotary_reshape_and_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     slot_mapping = slot_mapping.contiguous()
     with _on_device_of(q):
         check(_lib.load().vpa_rotary_reshape_and_cache(
-            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), outs, qs, ks,
-            vs,
+            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), outs, qs, ks, vs,
             positions.data_ptr(), stride, is64, inv_freq.data_ptr(), _ptr(axes), num_axes, rot,
-            int(adjacent), _ptr(q_norm), _ptr(k_norm), float(norm_eps), _ptr(k_scale), _ptr(v_scale), key_cache.data_ptr(),
-            value_cache.data_ptr(), slot_mapping.data_ptr(), t, h, kvh, d, bs, nb, bstride, hstride,
+            int(adjacent), _ptr(q_norm), _ptr(k_norm), float(norm_eps), _ptr(k_scale),
+            _ptr(v_scale), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), t, h, kvh, d, bs, nb, bstride, hstride,
             dtype_code(q.dtype), dtype_code(key_cache.dtype), _stream(q)))
     return out
