@@ -115,8 +115,8 @@ __device__ __forceinline__ Place place(const WeightsArgs& a, int num_kv_heads) {
 
 // The sequence at place r of the lengths in descending order (equal 32nds of max_ctx
 // in the order of their indexes), for at most kOrdered sequences: a wave holds the
-// lengths and counts by ballots. The mixed batch above took 85 us in the order of the
-// indexes, 76 in this one.
+// lengths and counts by ballots. The 256 sequences of the head of this file took 85 us in
+// the order of the indexes, 76 in this one.
 constexpr int kOrdered = 512;
 __device__ __forceinline__ int longest(const WeightsArgs& a, int r) {
   const int lane = threadIdx.x & 63;
@@ -425,8 +425,8 @@ __device__ __forceinline__ float2 merge_row(const float2* st, int chunks, int pa
   return make_float2(all.m, all.s == 0.f ? 0.f : 1.f / all.s);
 }
 
-// Second pass of few rows: one workgroup per (kv head, sequence, 1024 tokens), every
-// fourth row of 256 tokens to a thread.
+// Second pass of few rows: one workgroup per (kv head, sequence, 1024 tokens), four tokens
+// 256 apart per thread (single words: score rows have any alignment).
 __global__ __launch_bounds__(kThreads) void weight_sum_kernel(WeightsArgs a, int32_t num_kv_heads,
                                                               int32_t bs,
                                                               const float* __restrict__ logits,

@@ -223,3 +223,84 @@ def test_trim(device):
         alloc.trim(torch.zeros(4, dtype=torch.int32, device=device))
     with pytest.raises(vpa.VpaError, match="num_tokens"):
         alloc.trim(u32([1, 2, 3], device))
+
+
+def test_loop_on_a_side_stream(device):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        test_loop(device)
+    torch.cuda.current_stream().wait_stream(side)
+
+
+class Step:
+    """A decode step of a bounded cache: append, attention, weights, the cut to 40 tokens,
+    verification of two drafts; every buffer fixed, so that it can be captured."""
+
+    def __init__(self, device):
+        gen = torch.Generator().manual_seed(8)
+        rand = lambda *s: torch.randn(s, generator=gen).to(device)  # noqa: E731
+        self.alloc = vpa.DeviceBlockAllocator(20, BS, 3, 4, device)
+        assert self.alloc.allocate(u32([50, 23, 39], device)).all()
+        self.alloc.positions.copy_(u32([50, 23, 39], device))
+        self.kc, self.vc = rand(20, KVH, D // 4, BS, 4), rand(20, KVH, D, BS)
+        self.scores = rand(3, KVH, 64).abs()
+        self.q, self.k, self.v = rand(3, H, D), rand(3, KVH, D), rand(3, KVH, D)
+        self.pos = torch.tensor([[50, 23, 39]], device=device)
+        self.inv_freq, self.axes = vpa.rotary_frequencies(D, 1e4, device)
+        self.target, self.draft = 2 * rand(3, 3, 900), 2 * rand(3, 2, 900)
+        self.ids = u32(self.draft.argmax(-1).cpu().numpy(), device)
+        self.u = torch.rand((3, 3), generator=gen).to(device)
+        self.out = self.verified = None
+
+    def __call__(self):
+        a = self.alloc
+        slots, ctx = a.step()
+        q = vpa.rotary_reshape_and_cache(self.q, self.k, self.v, self.pos, self.inv_freq, self.axes,
+                                         None, None, self.kc, self.vc, slots)
+        self.out = vpa.paged_attention(q, None, None, self.kc, self.vc, a.block_tables, ctx, None, 64,
+                                       SCALE, 1.0, None)
+        vpa.paged_attention_weights(q, self.kc, None, a.block_tables, ctx, SCALE, self.scores,
+                                    max_context_len=64)
+        lens, self.kept = vpa.evict_kv_cache(self.kc, self.vc, self.scores, a.block_tables, ctx, 40,
+                                             keep_first=2, keep_last=4, max_context_len=64)
+        a.trim(lens)
+        self.verified = vpa.verify_draft_tokens(self.target, self.ids, self.u[:, :2], self.u[:, 2],
+                                                draft_logits=self.draft)
+        self.pos.add_(1)
+
+    def state(self):
+        a = self.alloc
+        return [self.out, self.kc, self.vc, self.scores, self.kept, self.pos, *self.verified,
+                a.positions, a.row_blocks, a.block_tables, a.free_ring, a.free_ring_state]
+
+    def inputs(self, i):
+        for x, scale in ((self.q, 1.0), (self.k, 1.1), (self.target, 0.9)):
+            x.copy_(torch.roll(x, i + 1, -1) * scale)
+        self.u.copy_(torch.roll(self.u, 1, 0))
+
+
+def test_step_captured_and_replayed(device):
+    """Two captured steps of two states, replayed in turn, against the same steps run
+    eagerly between the replays."""
+    eager, graphs, steps = Step(device), [], [Step(device), Step(device)]
+    Step(device)()  # (first use outside a capture)
+    torch.cuda.synchronize()
+    for s in steps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s()
+        graphs.append(g)
+    for i in range(5):
+        eager()
+        for g, s in zip(graphs, steps):
+            g.replay()
+        torch.cuda.synchronize()
+        for s in steps:
+            for x, y in zip(s.state(), eager.state()):
+                x, y = (t.view(torch.int32) if t.dtype == torch.uint32 else t for t in (x, y))
+                assert torch.equal(x, y), i
+        for s in (eager, *steps):
+            s.inputs(i)
+    assert eager.alloc.positions.cpu().numpy().tolist() == [40, 28, 40]
+    assert eager.alloc.row_blocks.cpu().numpy().tolist() == [3, 2, 3]
