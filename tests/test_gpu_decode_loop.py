@@ -304,3 +304,75 @@ def test_step_captured_and_replayed(device):
             s.inputs(i)
     assert eager.alloc.positions.cpu().numpy().tolist() == [40, 28, 40]
     assert eager.alloc.row_blocks.cpu().numpy().tolist() == [3, 2, 3]
+
+
+def refusals(device):
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device=device)  # noqa: E731
+    w = lambda *s: z(*s, dtype=torch.int32).view(torch.uint32)  # noqa: E731
+    q, k, pos, f = z(5, 4, 64), z(5, 2, 64), z(1, 5, dtype=torch.int64), z(32, dtype=torch.float64)
+    kc, vc, slots = z(9, 2, 16, 16, 4), z(9, 2, 64, 16), z(5, dtype=torch.int64)
+    bt, cl, sc = w(3, 4), w(3), z(3, 2, 64)
+    t, ids, au, su = z(3, 3, 50), w(3, 2), z(3, 2), z(3)
+    rq, rc = vpa.rotary_qk, vpa.rotary_reshape_and_cache
+    pw, ev, vd = vpa.paged_attention_weights, vpa.evict_kv_cache, vpa.verify_draft_tokens
+    cache = (None, None, kc, vc)
+    return [
+        ("must be \\[T, heads, D\\]", lambda: rq(q[0], k, pos, f)),
+        ("k must be", lambda: rq(q, k[:4], pos, f)),
+        ("k must be", lambda: rq(q, k.half(), pos, f)),
+        ("positions", lambda: rq(q, k, pos[:, :4], f)),
+        ("positions", lambda: rq(q, k, pos.int(), f)),
+        ("inv_freq", lambda: rq(q, k, pos, f.float())),
+        ("axes", lambda: rq(q, k, pos, f, z(31, dtype=torch.uint8))),
+        ("q_norm", lambda: rq(q, k, pos, f, q_norm=z(64).half())),
+        ("k_norm", lambda: rq(q, k, pos, f, k_norm=z(32))),
+        ("out_q", lambda: rq(q, k, pos, f, out_q=z(5, 4, 32))),
+        ("rotary_dim", lambda: rq(q, k, pos, z(33, dtype=torch.float64))),
+        ("num_axes", lambda: rq(q, k, z(5, 5, dtype=torch.int64), f)),
+        ("q, k and v", lambda: rc(q, k, z(5, 2, 32), pos, f, None, *cache, slots)),
+        ("one dtype", lambda: rc(q, k, k.half(), pos, f, None, *cache, slots)),
+        ("slot_mapping", lambda: rc(q, k, k, pos, f, None, *cache, slots[:4])),
+        ("differs", lambda: rc(q.half(), k.half(), k.half(), pos, f, None, *cache, slots)),
+        ("out must", lambda: rc(q, k, k, pos, f, None, *cache, slots, out=k)),
+        ("a row per sequence", lambda: pw(q, kc, None, bt, cl, 1.0, sc, max_context_len=64)),
+        ("q must be", lambda: pw(q[:3, :, :32], kc, None, bt, cl, 1.0, sc, max_context_len=64)),
+        ("cu_seqlens_q", lambda: pw(q, kc, None, bt, cl, 1.0, sc, cu_seqlens_q=w(3), max_query_len=2,
+                                    max_context_len=64)),
+        ("scores", lambda: pw(q[:3], kc, None, bt, cl, 1.0, sc[:, :, :60], max_context_len=64)),
+        ("scores", lambda: pw(q[:3], kc, None, bt, cl, 1.0, sc.half(), max_context_len=64)),
+        ("contiguous along", lambda: pw(q[:3], kc, None, bt, cl, 1.0, z(3, 2, 128)[..., ::2],
+                                        max_context_len=64)),
+        ("overlap", lambda: pw(q[:3], kc, None, bt, cl, 1.0, z(1, 2, 64).expand(3, 2, 64),
+                               max_context_len=64)),
+        ("too small", lambda: pw(q[:3], kc, None, bt, cl, 1.0, z(3, 2, 65), max_context_len=65)),
+        ("bytes needed", lambda: pw(q[:3], kc, None, bt, cl, 1.0, sc, max_context_len=64,
+                                    workspace=z(1))),
+        ("block_tables", lambda: ev(kc, vc, sc, bt.view(torch.int32), cl, 8, max_context_len=64)),
+        ("context_lens", lambda: ev(kc, vc, sc, bt, cl[:2], 8, max_context_len=64)),
+        ("budget", lambda: ev(kc, vc, sc, bt, cl, 0, max_context_len=64)),
+        ("budget", lambda: ev(kc, vc, sc, bt, cl, 8, keep_first=5, keep_last=4, max_context_len=64)),
+        ("new_context_lens", lambda: ev(kc, vc, sc, bt, cl, 8, max_context_len=64,
+                                        new_context_lens=cl)),
+        ("kept", lambda: ev(kc, vc, sc, bt, cl, 8, max_context_len=64, kept=w(3, 2, 7))),
+        ("shape mismatch", lambda: ev(kc, vc[:8], sc, bt, cl, 8, max_context_len=64)),
+        ("target_logits", lambda: vd(t[0], ids, au, su)),
+        ("draft_ids", lambda: vd(t, ids[:, :1], au, su)),
+        ("accept_u", lambda: vd(t, ids, au.double(), su)),
+        ("sample_u", lambda: vd(t, ids, au, su[:2])),
+        ("draft_logits", lambda: vd(t, ids, au, su, draft_logits=t)),
+        ("temperature", lambda: vd(t, ids, au, su, temperature=z(2))),
+        ("num_drafts", lambda: vd(t, ids, au, su, num_drafts=z(3, dtype=torch.int32))),
+        ("out must", lambda: vd(t, ids, au, su, out=(w(3, 2), w(3)))),
+        ("exceeds 64", lambda: vd(z(1, 66, 8), w(1, 65), z(1, 65), z(1))),
+        ("dtype", lambda: vd(t.double(), ids, au, su)),
+        ("GPU only", lambda: vd(t, ids.cpu(), au, su)),
+    ]
+
+
+@pytest.mark.parametrize("i", range(44))
+def test_wrong_tensors_are_refused(device, i):
+    cases = refusals(device)
+    assert len(cases) == 44
+    needle, call = cases[i]
+    with pytest.raises(vpa.VpaError, match=needle):
+        call()
