@@ -339,6 +339,7 @@ struct WeightsArgs {
 struct WeightsPlan {
   bool few;    // at most 16 rows per (sequence, kv head): their logits are kept
   bool whole;  // in LDS, of whole contexts, in one launch
+  bool wide;   // by eight waves, not four
   int32_t lds_logits;
   int32_t chunk_tokens, max_chunks, ctx_pad;
   size_t stats_at;

@@ -9,7 +9,7 @@
 // A weight needs its row's maximum and sum over the whole context, so every logit is
 // needed twice. Three forms, by the rows a (sequence, kv head) has at most (a row
 // being one query head of one new token) and the number of these pairs:
-//   * up to 16 rows, contexts whose logits fit 64 KiB of LDS, 512 pairs or more: one
+//   * up to 16 rows, contexts whose logits fit 64 KiB of LDS and are short or many: one
 //     launch, a workgroup per pair, the logits kept in LDS (weight_logits_kernel, whole);
 //   * up to 16 rows otherwise: a pass over the keys writes the logits (f32, log2 units)
 //     and per chunk the row's maximum and sum, a pass over the logits joins the chunks'
@@ -269,14 +269,14 @@ struct RowStat {
 // head, sequence, chunk): its waves share the chunk's tiles of 16 tokens evenly, each
 // a run of them, with the next TW tiles' keys in flight. kWhole: the chunk is the
 // whole context; its logits stay in LDS and the weights are added here.
-template <typename T, typename C, int D, bool kWhole>
-__global__ __launch_bounds__(kThreads) void weight_logits_kernel(
+template <typename T, typename C, int D, bool kWhole, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void weight_logits_kernel(
     WeightsArgs a, int32_t num_kv_heads, int32_t bs_log2, int64_t num_blocks, int64_t block_stride,
     int64_t head_stride, float* __restrict__ logits, float2* __restrict__ stats, int32_t ctx_pad,
     int32_t max_chunks, int32_t chunk_tokens) {
   using F = Frag<T, C, D>;
   constexpr int TW = F::TW;
-  __shared__ float s_m[4][16], s_s[4][16];
+  __shared__ float s_m[kWaves][16], s_s[kWaves][16];
   extern __shared__ uint32_t s_dyn[];  // the chunk's block ids, then its logits (kWhole)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void weight_logits_kernel(
   if (begin >= L || m_count == 0) return;
 
   const int tiles = ((int)min((int64_t)chunk_tokens, L - begin) + 15) / 16;
-  const int per = (tiles + 3) / 4;
+  const int per = (tiles + kWaves - 1) / kWaves;
   const int nt = min(per, tiles - wave * per);  // tiles of this wave, none if negative
   const int t_wave = (int)begin + wave * per * 16;
   const int b_first = (int)begin >> bs_log2;  // (chunks are whole blocks)
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void weight_logits_kernel(
     const int n = (((int)begin + tiles * 16 - 1) >> bs_log2) - b_first + 1;
     const int last = (L - 1) >> bs_log2;
     const uint32_t* table = a.block_tables + (int64_t)s * a.block_table_stride;
-    for (int i = threadIdx.x; i < n; i += kThreads) s_dyn[i] = table[min(b_first + i, last)];
+    for (int i = threadIdx.x; i < n; i += 64 * kWaves) s_dyn[i] = table[min(b_first + i, last)];
   }
   uint4 qv[F::KV][F::QV];
   load_rows<T, C, D>(a, rows, j, group, 0, m_count, qv);
@@ -382,13 +382,13 @@ __global__ __launch_bounds__(kThreads) void weight_logits_kernel(
     if (m < m_count) {
       RowStat all;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) all.join(s_m[w][m], s_s[w][m]);
+      for (int w = 0; w < kWaves; ++w) all.join(s_m[w][m], s_s[w][m]);
       s_m[0][m] = all.m;
       s_s[0][m] = all.s == 0.f ? 0.f : 1.f / all.s;  // (a row that sees no token adds nothing)
     }
     lds_group_barrier();
     float* out = a.scores + s * a.score_seq_stride + j * a.score_head_stride;
-    for (int t = threadIdx.x; t < L; t += kThreads) {
+    for (int t = threadIdx.x; t < L; t += 64 * kWaves) {
       float sum = 0.f;
       for (int i = 0; i < m_count; ++i) {
         const float l = s_logits[i * chunk_tokens + t];
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void weight_logits_kernel(
   } else if (m < m_count) {
     RowStat all;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) all.join(s_m[w][m], s_s[w][m]);
+    for (int w = 0; w < kWaves; ++w) all.join(s_m[w][m], s_s[w][m]);
     const int r = m / group;
     stats[((rows.first + r) * a.num_heads + j * group + (m - r * group)) * max_chunks + chunk] =
         make_float2(all.m, all.s);
@@ -724,14 +724,21 @@ hipError_t weights_launch(const WeightsArgs& a, const WeightsPlan& p, const Cach
   if (p.few) {
     float* logits = static_cast<float*>(a.workspace);
     const uint32_t lds = (uint32_t)(p.chunk_tokens >> bs_log2) * 4;
+    if (p.whole && p.wide) {
+      hipLaunchKernelGGL((weight_logits_kernel<T, C, D, true, 8>), dim3((uint32_t)p.first_grid),
+                         dim3(512), lds + (uint32_t)p.lds_logits, stream, a, g.num_kv_heads,
+                         bs_log2, g.num_blocks, g.block_stride, g.head_stride, logits, stats,
+                         p.ctx_pad, p.max_chunks, p.chunk_tokens);
+      return hipGetLastError();
+    }
     if (p.whole) {
-      hipLaunchKernelGGL((weight_logits_kernel<T, C, D, true>), dim3((uint32_t)p.first_grid),
+      hipLaunchKernelGGL((weight_logits_kernel<T, C, D, true, 4>), dim3((uint32_t)p.first_grid),
                          dim3(kThreads), lds + (uint32_t)p.lds_logits, stream, a, g.num_kv_heads,
                          bs_log2, g.num_blocks, g.block_stride, g.head_stride, logits, stats,
                          p.ctx_pad, p.max_chunks, p.chunk_tokens);
       return hipGetLastError();
     }
-    hipLaunchKernelGGL((weight_logits_kernel<T, C, D, false>), dim3((uint32_t)p.first_grid),
+    hipLaunchKernelGGL((weight_logits_kernel<T, C, D, false, 4>), dim3((uint32_t)p.first_grid),
                        dim3(kThreads), lds, stream, a, g.num_kv_heads, bs_log2, g.num_blocks,
                        g.block_stride, g.head_stride, logits, stats, p.ctx_pad, p.max_chunks,
                        p.chunk_tokens);
@@ -782,17 +789,21 @@ WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g) {
   // (at 16 rows the stored logits took 26 us for 8 sequences of 4000 tokens and 76 for
   // 64 of 2000, the second reading of the keys 28 and 86)
   p.few = m_max <= 16;
-  p.whole = false;
+  p.whole = p.wide = false;
   p.lds_logits = 0;
   p.ctx_pad = (int32_t)(parts(kWeightsChunk) * kWeightsChunk);
   p.chunk_tokens = kWeightsChunk;
   if (p.few) {
-    // Whole contexts per workgroup once every compute unit has two: 256 sequences of up to
-    // 500 tokens took 49 us (57 in two launches), 64 of 1000 tokens 26 (28), 512 of mixed
-    // lengths 207 (246); with fewer, long sequences are left alone at the end (64 of up
-    // to 4096 tokens 40 (39), 8 of 1000 11 (9)).
+    // Whole contexts per workgroup where none is left alone for long: eight waves take 2.8
+    // us per 1000 tokens, two launches of many workgroups 8.7 us at the least. Short
+    // contexts (one sequence of 300 tokens, 8 kv heads: 7.0 us; 8.6 in two launches; 1000
+    // tokens 9.2 and 8.7), contexts short for the number of pairs (32 sequences of 1000
+    // 13.9 and 17.1, 48 of 2000 38 and 40; 32 of up to 4096 30 and 28), and 512 pairs or
+    // more (64 of up to 4096 36 and 40, 512 of them 207 and 246). By four waves from 2048
+    // pairs on (256 sequences of up to 4096: 104 us, 110 by eight; 128 of them 62 and 53).
     const int64_t lds = m_max * p.ctx_pad * (int64_t)sizeof(float);
-    p.whole = pairs >= 512 && lds <= 65536;
+    p.whole = lds <= 65536 && (pairs >= 512 || a.max_ctx <= std::max<int64_t>(768, 4 * pairs));
+    p.wide = pairs < 2048;
     if (p.whole) {
       p.chunk_tokens = p.ctx_pad;
       p.lds_logits = (int32_t)lds;

@@ -89,6 +89,28 @@ def test_decode_rows(device, dtype, fp8, d, bs):
     check(p, run(device, p))
 
 
+@pytest.mark.parametrize("dtype,fp8", COMBOS)
+@pytest.mark.parametrize("d,bs", [(64, 8), (96, 32), (128, 16), (192, 8), (256, 32)])
+def test_longer_contexts(device, dtype, fp8, d, bs):
+    """Contexts that are split over workgroups, in two launches."""
+    p = problem(device, dtype, fp8, d, bs, 6, 3, [1, 769, 0, 1500], seed=d + bs + 1)
+    check(p, run(device, p))
+
+
+@pytest.mark.parametrize("dtype,fp8,d", [(torch.bfloat16, False, 128), (torch.float32, False, 64),
+                                         (torch.float16, True, 96), (torch.float32, True, 192)])
+def test_thousands_of_pairs(device, dtype, fp8, d):
+    """2048 (sequence, kv head) pairs and more, more sequences than are ordered."""
+    rng = np.random.default_rng(d)
+    lens = rng.integers(0, 70, size=515)
+    lens[300] = 333
+    p = problem(device, dtype, fp8, d, 16, 8, 4, lens, seed=24)
+    check(p, run(device, p))
+    short = np.minimum(lens, 500)[:512]
+    p = problem(device, dtype, fp8, d, 16, 4, 4, short, seed=25)
+    check(p, run(device, p))
+
+
 @pytest.mark.parametrize("h,kvh", [(16, 8), (8, 8), (14, 2), (32, 1), (40, 2), (3, 1)])
 @pytest.mark.parametrize("dtype,fp8", COMBOS[:4])
 def test_groups(device, dtype, fp8, h, kvh):
