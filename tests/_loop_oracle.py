@@ -24,16 +24,12 @@ def rotary(x, positions, inv_freq, axes, *, weight=None, eps=1e-6, adjacent=Fals
     return y, mag
 
 
-def rows_of(cache, table, length, is_key):
+def rows_of(cache, table, length):
     """K or V rows [KVH, length, D] of one sequence from a float64 cache."""
-    if is_key:
-        nb, kvh, dx, bs, x = cache.shape
-        flat = cache.transpose(0, 3, 1, 2, 4).reshape(nb, bs, kvh, dx * x)
-    else:
-        nb, kvh, d, bs = cache.shape
-        flat = cache.transpose(0, 3, 1, 2)
+    bs = cache.shape[3]
     t = np.arange(length)
-    return flat[table[t // bs].astype(np.int64), t % bs].transpose(1, 0, 2)
+    rows = cache[table[t // bs].astype(np.int64), :, :, t % bs]  # [length, KVH, D / x, x] or [.., D]
+    return rows.reshape(length, cache.shape[1], -1).transpose(1, 0, 2)
 
 
 def attention_weights(q, key_cache, tables, lens, scale, scores, cu=None, causal=True):
@@ -51,7 +47,7 @@ def attention_weights(q, key_cache, tables, lens, scale, scores, cu=None, causal
             continue
         table = tables[s].astype(np.int64)
         there = table[np.arange(size) // bs] < nb
-        k = rows_of(key_cache, np.where(table < nb, table, 0), size, True)
+        k = rows_of(key_cache, np.where(table < nb, table, 0), size)
         for r in range(n):
             see = there & (np.arange(size) <= (r + size - n if causal else size))
             if not see.any():

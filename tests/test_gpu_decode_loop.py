@@ -74,7 +74,7 @@ class Loop:
         kc, vc, tables = np64(self.kc), np64(self.vc), self.tables()
         for s in range(3):
             n = len(self.tokens[s][0])
-            k, v = ref.rows_of(kc, tables[s], n, True), ref.rows_of(vc, tables[s], n, False)
+            k, v = ref.rows_of(kc, tables[s], n), ref.rows_of(vc, tables[s], n)
             for j in range(KVH):
                 want = [np.stack(x) for x in zip(*self.tokens[s][j])]
                 assert np.all(np.abs(k[j] - want[0]) <= want[1])
@@ -86,7 +86,7 @@ class Loop:
         q, want, i = np64(q), [], 0
         for s, r in enumerate(rows):
             n = len(self.tokens[s][0])
-            k, v = ref.rows_of(kc, tables[s], n, True), ref.rows_of(vc, tables[s], n, False)
+            k, v = ref.rows_of(kc, tables[s], n), ref.rows_of(vc, tables[s], n)
             for t in range(r):
                 see = n - r + t + 1 if causal else n
                 for h in range(H):
