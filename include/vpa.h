@@ -693,8 +693,8 @@ size_t vpa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t max_draf
  * A draw is the first v with cumsum(r)[v] > sample_u[b] * sum(r), summed in
  * f64. T <= 0 or NaN: draft i is accepted if it is the first maximum of row i,
  * and the row's first maximum replaces it or follows. Logits of -inf and NaN
- * have probability 0; a row of nothing else gives id 0. Ids >= vocab are
- * never accepted.
+ * have probability 0; a row of nothing else gives id 0 (where T <= 0 that is its
+ * first maximum, and a draft of 0 is accepted). Ids >= vocab are never accepted.
  *   out_ids[b, 0 .. c - 1], c = out_count[b] = accepted + 1: the emitted
  *   tokens; 0xffffffff behind them (u32 [num_seqs, max_drafts + 1])
  * max_drafts 0 samples one token per sequence; at most 64. accept_u f32

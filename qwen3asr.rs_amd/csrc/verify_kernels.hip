@@ -394,16 +394,17 @@ __device__ __forceinline__ Pick pick_row(const VerifyArgs& a, const Buffers& w, 
     if (q < rows && part == 0) {
       sh.max[q] = mx;
       sh.sum[q] = sum;
-      if (is_target) sh.best[q] = best;
+      // (a greedy row without a number: 0, as the argmax gives)
+      if (is_target) sh.best[q] = best == kNone ? 0u : best;
     }
   }
   __syncthreads();
   if (wave == 0) {  // lane i tests draft i
     bool good = false;
-    if (lane < n) {
+    if (lane < n && x < (uint32_t)a.vocab) {
       if (greedy) {
         good = sh.best[lane] == x;
-      } else if (x < (uint32_t)a.vocab) {
+      } else {
         const double px = Scale(sh.max[lane], temp).weight(lx) / sh.sum[lane];
         double qx = 1.0;
         if (have_q) {
@@ -556,8 +557,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a,
     if (i != p.took) out[i] = i < p.took ? a.draft_ids[(int64_t)b * K + i] : kNone;
   if (tid == 0) a.out_count[b] = (uint32_t)p.took + 1u;
   out += p.took;
-  if (p.greedy) {  // a row with no number: 0, as the argmax gives
-    if (tid == 0) *out = p.best == kNone ? 0u : p.best;
+  if (p.greedy) {
+    if (tid == 0) *out = p.best;
     return;
   }
   const float temp = seq_temperature(a, b);
