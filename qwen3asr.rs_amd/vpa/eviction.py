@@ -60,7 +60,12 @@ def paged_attention_weights(q: torch.Tensor, key_cache: torch.Tensor,
     with it (u32 [B + 1]) a sequence has several rows, its last tokens, and
     with ``causal`` each sees the tokens up to its own. ``max_query_len`` and
     ``max_context_len`` size the launch; a caller that knows them on the host
-    passes them to skip a device read."""
+    passes them to skip a device read.
+
+    A sequence of length 0 adds nothing. A row that did not run in a step
+    (``DeviceBlockAllocator.step``: negative slot) has context_lens 1, which would add
+    a whole weight to its first token; give it 0:
+    ``(context_lens.view(torch.int32) * (slot_mapping >= 0)).view(torch.uint32)``."""
     _require_device(q, key_cache, k_scale, block_tables, context_lens, scores, cu_seqlens_q,
                     workspace)
     if key_cache.dim() != 5:
@@ -131,7 +136,8 @@ def evict_kv_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: t
     Returns (new_context_lens u32 [B], kept u32 [B, KVH, budget]: the old
     position of each token that stayed, 0xffffffff past the last). The blocks past
     ceil(new_context_lens / block_size) may then be given back
-    (``DeviceBlockAllocator.trim``)."""
+    (``DeviceBlockAllocator.trim``, with the step's slot_mapping where rows may not
+    have run: their new length is not what they hold)."""
     _require_device(key_cache, value_cache, scores, block_tables, context_lens, new_context_lens,
                     kept, workspace)
     nb, kvh, d, bs, bstride, hstride = cache_geometry(key_cache, value_cache)

@@ -528,19 +528,32 @@ class DeviceBlockAllocator:
             self.batch, _stream(self.block_tables)))
         return self.slot_mapping, self.context_lens
 
-    def trim(self, num_tokens: torch.Tensor) -> None:
+    def trim(self, num_tokens: torch.Tensor,
+             slot_mapping: Optional[torch.Tensor] = None) -> None:
         """Rows hold num_tokens[r] tokens from here on (u32 [batch], at most what
         they held): the next step appends there, and the blocks past them go
         back (trim_request_to_num_tokens, paged_cache_runtime.rs:320-340). For rows
-        whose drafted tokens were rejected or whose cache was cut."""
+        whose drafted tokens were rejected or whose cache was cut. With the
+        ``slot_mapping`` of the step before (i64 [batch]), a row that did not run in
+        it (negative slot: finished, or stalled for lack of a block; its context_lens
+        is 1 whatever it holds) keeps all it holds."""
         if num_tokens.dtype != torch.uint32 or num_tokens.shape != (self.batch,):
             raise _err(f"num_tokens must be u32 [{self.batch}], got {num_tokens.dtype} "
                        f"{tuple(num_tokens.shape)}")
-        _require_device(num_tokens, self.positions)
-        self.positions.copy_(num_tokens)
+        if slot_mapping is not None and (slot_mapping.dtype != torch.int64 or
+                                         slot_mapping.shape != (self.batch,)):
+            raise _err(f"slot_mapping must be i64 [{self.batch}], got {slot_mapping.dtype} "
+                       f"{tuple(slot_mapping.shape)}")
+        _require_device(num_tokens, self.positions, slot_mapping)
         bs = self.block_size
         # (u32 arithmetic through the bits: torch has none of its own)
-        keep = (num_tokens.view(torch.int32).long() + (bs - 1)) // bs
+        tokens = num_tokens.view(torch.int32)
+        keep = (tokens.long() + (bs - 1)) // bs
+        if slot_mapping is not None:
+            ran = slot_mapping >= 0
+            tokens = torch.where(ran, tokens, self.positions.view(torch.int32))
+            keep = torch.where(ran, keep, self.cols)  # (no row has more blocks)
+        self.positions.view(torch.int32).copy_(tokens)
         self.release(keep.to(torch.int32).view(torch.uint32))
 
     def release(self, keep_blocks: torch.Tensor) -> None:
