@@ -323,9 +323,10 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
     const uint32_t b = table[c];
     return (int64_t)b < num_blocks ? (int64_t)b * block_stride : (int64_t)-1;
   };
-  // Where all columns fit, they are read together with the length (one round
-  // trip before the first data, not three; what lies past the context is not
-  // used); else window by window.
+  const int L = context_of(a, s, BS);
+  if (L <= a.budget) return;  // (and the selection wrote no columns)
+  // Where all columns fit, they are read at once (what lies past the context is
+  // not used); else window by window.
   const bool whole = a.max_columns <= kInfo;
   if (whole)
     for (int i = threadIdx.x; i < a.max_columns; i += kThreads) {
@@ -333,8 +334,6 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(
       s_from[i] = offset_of(i);
     }
   const int c_begin = (int)a.first_column[pair];
-  const int L = context_of(a, s, BS);
-  if (L <= a.budget) return;
   E* cache = static_cast<E*>(value ? a.value_cache : a.key_cache) + j * head_stride +
              (int64_t)dg * DG * BS;
   const int tid = threadIdx.x;
@@ -534,6 +533,8 @@ hipError_t launch_evict(int cache_dtype, const EvictArgs& args, void* workspace,
                        g.num_kv_heads, bs_log2);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
+  // no sequence is cut; of contexts without tokens there is no workspace either
+  if (a.max_ctx <= a.budget) return e;
   if (cache_dtype == VPA_DTYPE_F32) return move_typed<uint32_t>(a, g, stream);
   if (cache_dtype == VPA_DTYPE_FP8_E4M3) return move_typed<uint8_t>(a, g, stream);
   return move_typed<uint16_t>(a, g, stream);
