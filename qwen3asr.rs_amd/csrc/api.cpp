@@ -1104,8 +1104,10 @@ int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
   if (max_context_len > (1 << 30) || budget > (1 << 30))
     return fail(VPA_ERR_UNSUPPORTED, "%s: max_context_len=%d or budget=%d exceeds 2^30", op,
                 max_context_len, budget);
-  if (scores == nullptr || block_tables == nullptr || context_lens == nullptr ||
-      new_context_lens == nullptr || kept == nullptr)
+  // (contexts without tokens have no scores and no table columns: those tensors may be
+  // empty)
+  if ((max_context_len > 0 && (scores == nullptr || block_tables == nullptr)) ||
+      context_lens == nullptr || new_context_lens == nullptr || kept == nullptr)
     return fail(VPA_ERR_INVALID_ARGUMENT,
                 "%s: scores, block_tables, context_lens, new_context_lens and kept must be non-null",
                 op);

@@ -46,3 +46,15 @@ def test_contexts_within_the_budget(device):
     check(device, [0, 1, 33], 33)
     check(device, [0, 1, 33], 60, keep_first=4, keep_last=9, max_context_len=60)
     check(device, [0, 1, 33], 33, max_context_len=64)
+
+
+@pytest.mark.parametrize("width,cols", [(0, 4), (64, 0), (0, 0)])
+def test_empty_scores_and_tables(device, width, cols):
+    """Before the first token scores and tables may have no columns at all (their data
+    pointers are null); the weights of such contexts are nothing."""
+    check(device, [0, 0], 7, width=width, cols=cols)
+    kc, _, sc = state(device, 2, width)
+    q = torch.ones((2, 4, 64), dtype=torch.bfloat16, device=device)
+    got = vpa.paged_attention_weights(q, kc, None, u32(np.zeros((2, cols)), device), u32([0, 0], device),
+                                      1.0, sc)
+    assert got is sc and torch.equal(sc, state(device, 2, width)[2])
