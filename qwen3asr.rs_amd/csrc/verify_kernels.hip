@@ -31,12 +31,12 @@
 // sequence of four drafts without logits 4.3 + 9.6; 128 of up to three, greedy (156
 // MB), 20 + 4.
 
-#include <float.h>
 #include <math.h>
 
 #include <algorithm>
 #include <type_traits>
 
+#include "verify_weight.h"
 #include "vpa_device.h"
 #include "vpa_internal.h"
 
@@ -57,55 +57,6 @@ struct Buffers {
   double* sum;
   double* rest;  // [num_seqs][segments] of max(p - q, 0)
   int32_t segs;
-};
-
-// 2^t for 0 >= t > -2^31 in f64, 0 below -1074: t = n + f, and for 2^f,
-// |f| <= 1/2, the polynomial 1 + f g(f) with g through the 9 Chebyshev nodes of
-// (2^f - 1) / f: within 4e-14 of the value. A draw among 150 000 tokens then has
-// about one chance in 10^8 to see a border on its wrong side.
-__device__ __forceinline__ double exp2_nonpos(double t) {
-  const double n = __builtin_rint(t);
-  const double f = t - n;
-  double p = 1.02031210633917290e-07;
-  p = __builtin_fma(p, f, 1.32552248786688168e-06);
-  p = __builtin_fma(p, f, 1.52526868462677196e-05);
-  p = __builtin_fma(p, f, 1.54034558524538382e-04);
-  p = __builtin_fma(p, f, 1.33335581790431116e-03);
-  p = __builtin_fma(p, f, 9.61812915940255843e-03);
-  p = __builtin_fma(p, f, 5.55041086647604237e-02);
-  p = __builtin_fma(p, f, 2.40226506958129887e-01);
-  p = __builtin_fma(p, f, 6.93147180559945286e-01);
-  p = __builtin_fma(p, f, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
-}
-// The weights e^((l - m) / T) of logits l against a maximum m: 1 at the maximum
-// (also an infinite one), 0 for -inf and NaN.
-struct Scale {
-  double c;  // log2 e / T
-  double m64;
-  float m;
-  float floor;  // logits below it, and NaN, count as it: an exponent below every f64
-  bool odd;     // (uniform) the maximum is infinite or the lowest number: only its equals weigh
-  __device__ __forceinline__ Scale(float max, float temp)
-      // (T above 1e30 as 1e30: a masked logit's weight stays 0)
-      : c(fmax(1.44269504088896340736 / (double)temp, 1e-30)),
-        m64((double)max),
-        m(max),
-        floor(fmaxf(fminf(max - 2000.f * temp, below(max)), -FLT_MAX)),
-        odd(!(max > -FLT_MAX && max < INFINITY)) {}
-  // the next number below a finite one
-  static __device__ __forceinline__ float below(float v) {
-    const uint32_t u = __float_as_uint(v);
-    return __uint_as_float(v > 0.f ? u - 1u : v < 0.f ? u + 1u : 0x80000001u);
-  }
-  __device__ __forceinline__ double plain(float l) const {
-    // (the difference first: logits of the lowest value have products whose
-    // rounding alone would be a huge exponent)
-    return exp2_nonpos(((double)fmaxf(l, floor) - m64) * c);
-  }
-  __device__ __forceinline__ double weight(float l) const {
-    return odd ? (l == m && l > -INFINITY ? 1.0 : 0.0) : plain(l);
-  }
 };
 
 __device__ __forceinline__ float seq_temperature(const VerifyArgs& a, int b) {
