@@ -580,11 +580,24 @@ int vpa_rotary_reshape_and_cache(
     void* stream);
 
 /*
- * Bytes of caller workspace vpa_paged_attention_weights needs. Depends only
- * on the arguments; 0 where one of them is.
+ * Bytes of caller workspace that vpa_paged_attention_weights needs at most,
+ * however the rows lie in the sequences (1032 per row, head and 256 tokens of
+ * context). Depends only on the arguments; 0 where one of them is.
  */
 size_t vpa_paged_attention_weights_workspace_size(int64_t total_query_rows, int32_t num_heads,
                                                   int32_t max_context_len);
+
+/*
+ * Bytes of caller workspace that one call of vpa_paged_attention_weights needs:
+ * as above, but 8 in place of 1032 where a kv head can have more than 16 rows
+ * in a sequence (max_query_len * num_heads / num_kv_heads > 16, the rows of a
+ * prompt), whose logits are not stored. Depends only on the arguments; 0 where
+ * one of them is.
+ */
+size_t vpa_paged_attention_weights_call_workspace_size(int64_t total_query_rows,
+                                                       int32_t max_query_len,
+                                                       int32_t max_context_len,
+                                                       int32_t num_heads, int32_t num_kv_heads);
 
 /*
  * paged_attention_weights - adds the attention weight that each cached token
@@ -608,7 +621,7 @@ size_t vpa_paged_attention_weights_workspace_size(int64_t total_query_rows, int3
  * Types, head dims and block sizes as the chunked prefill, any number of
  * query heads per kv head. n_s and L_s are clamped to max_query_len and
  * max_context_len, rows at or past total_query_rows are not read. workspace:
- * vpa_paged_attention_weights_workspace_size bytes, 256-byte aligned; calls
+ * vpa_paged_attention_weights_call_workspace_size bytes, 256-byte aligned; calls
  * that run concurrently need one each.
  */
 int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,

@@ -976,7 +976,18 @@ int vpa_rotary_reshape_and_cache(
 size_t vpa_paged_attention_weights_workspace_size(int64_t total_query_rows, int32_t num_heads,
                                                   int32_t max_context_len) {
   if (total_query_rows <= 0 || num_heads <= 0 || max_context_len <= 0) return 0;
-  return weights_workspace_bytes(total_query_rows, num_heads, max_context_len);
+  return weights_workspace_bytes(total_query_rows, num_heads, max_context_len, true);
+}
+
+size_t vpa_paged_attention_weights_call_workspace_size(int64_t total_query_rows,
+                                                       int32_t max_query_len,
+                                                       int32_t max_context_len,
+                                                       int32_t num_heads, int32_t num_kv_heads) {
+  if (total_query_rows <= 0 || max_query_len <= 0 || max_context_len <= 0 || num_heads <= 0 ||
+      num_kv_heads <= 0)
+    return 0;
+  return weights_workspace_bytes(total_query_rows, num_heads, max_context_len,
+                                 weights_few(max_query_len, num_heads, num_kv_heads));
 }
 
 int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
@@ -1056,7 +1067,9 @@ int vpa_paged_attention_weights(float* scores, int64_t score_seq_stride,
     return fail(VPA_ERR_INVALID_ARGUMENT,
                 "%s: score strides (seq=%lld head=%lld) overlap for max_context_len=%d", op,
                 (long long)score_seq_stride, (long long)score_head_stride, max_context_len);
-  const size_t need = weights_workspace_bytes(total_query_rows, num_heads, max_context_len);
+  const size_t need =
+      weights_workspace_bytes(total_query_rows, num_heads, max_context_len,
+                              weights_few(max_query_len, num_heads, num_kv_heads));
   if (workspace == nullptr || workspace_bytes < need)
     return fail(VPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", op, need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);

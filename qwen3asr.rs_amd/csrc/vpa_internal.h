@@ -346,7 +346,11 @@ struct WeightsPlan {
   int64_t first_grid, second_grid;  // workgroups
 };
 WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g);
-size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx);
+// At most 16 rows per (sequence, kv head): the form that may store its logits.
+inline bool weights_few(int32_t max_query_len, int32_t num_heads, int32_t num_kv_heads) {
+  return (int64_t)max_query_len * (num_heads / num_kv_heads) <= 16;
+}
+size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx, bool few);
 hipError_t launch_attention_weights(int dtype, int cache_dtype, const WeightsArgs& a,
                                     const CacheGeom& g, hipStream_t stream);
 

@@ -776,9 +776,12 @@ hipError_t weights_typed(const WeightsArgs& a, const WeightsPlan& p, const Cache
 
 }  // namespace
 
-size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx) {
-  const int64_t chunks = (max_ctx + kWeightsChunk - 1) / kWeightsChunk;
-  return (size_t)(total_rows * num_heads * chunks) * (kWeightsChunk * sizeof(float) + sizeof(float2));
+// A pair per row and chunk (of kWeightsChunk tokens or a multiple), and of few rows the
+// logits.
+size_t weights_workspace_bytes(int64_t total_rows, int32_t num_heads, int32_t max_ctx, bool few) {
+  const int64_t chunks = ((int64_t)max_ctx + kWeightsChunk - 1) / kWeightsChunk;
+  return (size_t)(total_rows * num_heads * chunks) *
+         ((few ? kWeightsChunk * sizeof(float) : 0) + sizeof(float2));
 }
 
 WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g) {
@@ -788,7 +791,7 @@ WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g) {
   auto parts = [&](int tokens) { return ((int64_t)a.max_ctx + tokens - 1) / tokens; };
   // (at 16 rows the stored logits took 26 us for 8 sequences of 4000 tokens and 76 for
   // 64 of 2000, the second reading of the keys 28 and 86)
-  p.few = m_max <= 16;
+  p.few = weights_few(a.max_query_len, a.num_heads, g.num_kv_heads);
   p.whole = p.wide = false;
   p.lds_logits = 0;
   p.ctx_pad = (int32_t)(parts(kWeightsChunk) * kWeightsChunk);

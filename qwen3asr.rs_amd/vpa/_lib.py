@@ -82,6 +82,7 @@ SIGNATURES = {
         _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _p, _p,
         _f32, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _p]),
     "vpa_paged_attention_weights_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "vpa_paged_attention_weights_call_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "vpa_paged_attention_weights": (ctypes.c_int, [
         _p, _i64, _i64, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i64, _f32, _i32, _i32,
         _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _p, _sz, _p]),

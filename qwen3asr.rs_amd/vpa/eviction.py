@@ -37,10 +37,21 @@ def _score_strides(scores: torch.Tensor, b: int, kvh: int, max_context_len: int)
 
 
 def paged_attention_weights_workspace(total_query_rows: int, num_heads: int,
-                                      max_context_len: int, device) -> Optional[torch.Tensor]:
-    """Caller-side workspace of ``paged_attention_weights`` (None when not needed)."""
-    n = _lib.load().vpa_paged_attention_weights_workspace_size(total_query_rows, num_heads,
-                                                               max_context_len)
+                                      max_context_len: int, device, *,
+                                      max_query_len: Optional[int] = None,
+                                      num_kv_heads: Optional[int] = None
+                                      ) -> Optional[torch.Tensor]:
+    """Caller-side workspace of ``paged_attention_weights`` (None when not needed). With
+    ``max_query_len`` and ``num_kv_heads`` that of calls of these sizes: where a kv head
+    can have more than 16 rows in a sequence (a prompt's) 8 bytes per row, head and 256
+    tokens in place of 1032."""
+    lib = _lib.load()
+    if max_query_len is None or num_kv_heads is None:
+        n = lib.vpa_paged_attention_weights_workspace_size(total_query_rows, num_heads,
+                                                           max_context_len)
+    else:
+        n = lib.vpa_paged_attention_weights_call_workspace_size(
+            total_query_rows, max_query_len, max_context_len, num_heads, num_kv_heads)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -99,7 +110,8 @@ def paged_attention_weights(q: torch.Tensor, key_cache: torch.Tensor,
     with _on_device_of(q):
         lib = _lib.load()
         if workspace is None:
-            nbytes = lib.vpa_paged_attention_weights_workspace_size(rows, h, int(max_context_len))
+            nbytes = lib.vpa_paged_attention_weights_call_workspace_size(
+                rows, int(max_query_len), int(max_context_len), h, kvh)
             workspace = context_lens.new_empty(((nbytes + 3) // 4,))
         else:
             nbytes = workspace.nbytes
