@@ -704,7 +704,8 @@ size_t vpa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t max_draf
  *   scaled to sum 1 (from p_i where that is 0 everywhere); if all n are
  *   accepted, a draw from p_n follows.
  * A draw is the first v with cumsum(r)[v] > sample_u[b] * sum(r), summed in
- * f64. T <= 0 or NaN: draft i is accepted if it is the first maximum of row i,
+ * f64. T <= 0 or NaN: draft i is accepted if it is the first maximum of row i
+ * (a NaN is skipped wherever it stands; vpa_argmax_rows keeps one at index 0),
  * and the row's first maximum replaces it or follows. Logits of -inf and NaN
  * have probability 0; a row of nothing else gives id 0 (where T <= 0 that is its
  * first maximum, and a draft of 0 is accepted). Ids >= vocab are never accepted.

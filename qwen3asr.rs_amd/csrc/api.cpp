@@ -1109,8 +1109,9 @@ int vpa_evict_kv_cache(void* key_cache, void* value_cache, float* scores,
                 "%s: budget=%d must be positive and hold keep_first=%d + keep_last=%d", op, budget,
                 keep_first, keep_last);
   if (num_seqs == 0) return VPA_OK;
-  // (up to 64 workgroups of 256 lanes each: the grid's lane count must fit in
-  // 32 bits)
+  // (the grid's lane count must fit in 32 bits: the selection has a workgroup of up to
+  // 1024 lanes per pair, the move at most 16 of 512, or four times as many where those
+  // are under 1024 in all)
   if ((int64_t)num_seqs * num_kv_heads >= ((int64_t)1 << 18))
     return fail(VPA_ERR_UNSUPPORTED, "%s: num_seqs=%d times num_kv_heads=%d reaches 2^18", op,
                 num_seqs, num_kv_heads);

@@ -17,10 +17,11 @@
 // The answers are whole numbers next to a border of a sum over the vocabulary: in f32
 // the cumulative sum is off by 2^-24 of the total, more than many of its 150 000 steps,
 // so weights and sums are f64 throughout, exponentials included (within 4e-14). The
-// f64 instructions of the exponentials, not the logits' bytes, bound the calls with
-// draft logits: 17 of them, 93 cycles of a SIMD, per 64 logits, 62 of the 73 us that the
-// 87.5 million of 64 sequences with four drafts take (151 936 tokens, bf16; 175 MB, 27
-// us at the streaming rate). f32 first and f64 for the drawn row alone needs that row
+// f64 instructions of the exponentials are most of the calls with draft logits: 17 of
+// them, 93 cycles of a SIMD at the rates measured alone, per 64 logits, which is 52 of
+// the 71 to 75 us that the 87.5 million of 64 sequences with four drafts take at 2.4 GHz
+// (151 936 tokens, bf16; 175 MB, 27 us at the streaming rate); what the other 20 us are
+// has not been taken apart. f32 first and f64 for the drawn row alone needs that row
 // read once more by a launch of its own and took 148 us in all against 121 then.
 //
 // Launches, over segments of 4096 logits: stats (every row's segment maxima and sums,
@@ -29,7 +30,8 @@
 // it). Rest and draw merge the stats and test the drafts themselves (pick_row: cheaper
 // than a launch between them). Measured: 64 sequences as above 73 + 24 + 11 us; one
 // sequence of four drafts without logits 4.3 + 9.6; 128 of up to three, greedy (156
-// MB), 20 + 4.
+// MB), 20 + 4; one token of each of 64 sequences sampled 14 + 8. Rows that do not all
+// begin at 16 bytes are read by element: 64 sequences of 151 935 tokens 173 + 34 + 12.
 
 #include <math.h>
 

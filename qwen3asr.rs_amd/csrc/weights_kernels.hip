@@ -28,8 +28,9 @@
 // Bound by the bytes of the keys, with many rows also by the vector instructions of
 // their exponentials and reductions. Measured in 16 bits at 16 query and 8 kv heads of
 // 128: 256 sequences of 16 to 4096 tokens (424 MB of keys), one row each, 76 us = 5.6
-// TB/s; 8 sequences of 1000 to 6000 tokens (57 MB), 32 rows each, 38 us (19 per pass;
-// 78 with stored logits); one sequence of 1500 tokens, 5.4 + 4.3 us.
+// TB/s (f32 142 us, fp8 keys 49); 8 sequences of 1000 to 6000 tokens (57 MB), 32 rows
+// each, 38 us (19 per pass; 78 with stored logits); one sequence of 1500 tokens, 5.6 +
+// 4.3 us; all rows of one prompt of 512 tokens 110 us, of 2048 432, of 8192 2360.
 
 #include <float.h>
 #include <math.h>
@@ -803,7 +804,9 @@ WeightsPlan weights_plan(int dtype, const WeightsArgs& a, const CacheGeom& g) {
     // tokens 9.2 and 8.7), contexts short for the number of pairs (32 sequences of 1000
     // 13.9 and 17.1, 48 of 2000 38 and 40; 32 of up to 4096 30 and 28), and 512 pairs or
     // more (64 of up to 4096 36 and 40, 512 of them 207 and 246). By four waves from 2048
-    // pairs on (256 sequences of up to 4096: 104 us, 110 by eight; 128 of them 62 and 53).
+    // pairs on (256 sequences of up to 4096: 104 us, 110 by eight; 128 of them 62 and 53;
+    // nothing between was measured). All at 128 dims in 16 bits; the other types and dims
+    // follow the same borders.
     const int64_t lds = m_max * p.ctx_pad * (int64_t)sizeof(float);
     p.whole = lds <= 65536 && (pairs >= 512 || a.max_ctx <= std::max<int64_t>(768, 4 * pairs));
     p.wide = pairs < 2048;
