@@ -726,6 +726,219 @@ int vpa_verify_draft_tokens(uint32_t* out_ids, uint32_t* out_count, const void* 
                             int32_t max_drafts, int32_t vocab, int32_t dtype, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/*
+ * Caches of E4M3 bytes with a scale for each block and kv head
+ * ("block-scaled"): the fp8 cache's layout, and for K and for V f32
+ * scales [num_blocks, num_kv_heads] (heads contiguous, scale_block_stride
+ * elements between blocks, the same for both). A byte of block b, kv head j
+ * stands for (float)byte * scales[b, j]. Where the one scale of an fp8 cache
+ * has to be chosen before its values are known, these follow the values. No
+ * counterpart in the reference. The two entry points below read and write
+ * them; the entry points that take one k_scale / v_scale, and
+ * vpa_evict_kv_cache (which moves tokens between blocks), do not know of
+ * them. vpa_copy_blocks copies a block's scales as one more buffer.
+ */
+
+/*
+ * reshape_and_cache_block_scaled - vpa_reshape_and_cache into a block-scaled
+ * cache. Arguments, strides, skipped slots and errors as there (dtype: the
+ * rows' type, f32, f16 or bf16; the cache is E4M3).
+ *
+ * A block's scale is the smallest power of two s (at least 2^-100) with
+ * |x| <= 448 s for the finite elements written to it, for K and V apart. A
+ * token at offset 0 opens its block: the scale is what the call's tokens
+ * need and nothing of before counts. Otherwise s' = max(s, what they need),
+ * and where that is more than s the bytes there become E4M3(byte * s / s')
+ * (exact but below E4M3's normal range). Elements are stored as
+ * E4M3(x * (1 / s')), rounded to nearest even; infinities as +-448, NaN stays
+ * NaN. So a pool's scales may start as anything finite (zeros, say) where
+ * blocks are filled from offset 0 on.
+ * Tokens of one block are neighbours in the call (a sequence's tokens in
+ * order are); where a slot repeats among them the last token counts. A block
+ * whose tokens are not neighbours gets undefined contents.
+ */
+int vpa_reshape_and_cache_block_scaled(const void* key, const void* value,
+                                       int64_t key_token_stride, int64_t value_token_stride,
+                                       float* key_scales, float* value_scales,
+                                       int64_t scale_block_stride, void* key_cache,
+                                       void* value_cache, const int64_t* slot_mapping,
+                                       int64_t num_tokens, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t block_size, int64_t num_blocks,
+                                       int64_t cache_block_stride, int64_t cache_head_stride,
+                                       int32_t dtype, void* stream);
+
+/*
+ * Bytes of caller workspace vpa_paged_attention_block_scaled needs. Depends
+ * only on the arguments; 0 where one call's keys are not split.
+ */
+size_t vpa_paged_attention_block_scaled_workspace_size(int32_t num_seqs, int32_t max_query_len,
+                                                       int32_t max_context_len,
+                                                       int64_t total_query_rows,
+                                                       int32_t num_heads, int32_t num_kv_heads,
+                                                       int32_t head_dim, int32_t dtype);
+
+/*
+ * paged_attention_block_scaled - attention over a block-scaled cache, for a
+ * decode step, drafted tokens or the rows of a prompt.
+ *
+ * query/out [total_query_rows, num_heads, head_dim] packed, f32, f16 or
+ * bf16; sequence s owns rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 (n_s of
+ * them; NULL: row s alone) and its first L_s = context_lens[s] cached tokens,
+ * the rows' own included. With p_t = exp(softmax_scale * key_scales[b(t), j]
+ * * q . K_t - m), m the maximum of the exponents,
+ *   out = sum_t p_t value_scales[b(t), j] V_t / (sum_t p_t + denom_eps)
+ * over the tokens the row sees: all t < L_s, or with causal != 0 t <= r + L_s -
+ * n_s for its r-th row. A row that sees none is zeros; block ids >= num_blocks
+ * are absent. vpa_paged_attention adds a denom_eps of 1e-6,
+ * vpa_chunked_prefill_paged_attention the caller's. Scales may be any finite
+ * numbers, not only powers of two.
+ * Any number of query heads per kv head, head_dim 64, 96, 128, 192 or 256,
+ * block_size 8, 16 or 32. n_s and L_s are clamped to max_query_len and
+ * max_context_len, which size the grid; rows at or past total_query_rows are
+ * neither read nor written. Sums have a fixed order: results do not vary from
+ * call to call. workspace: ..._workspace_size bytes, 256-byte aligned (NULL
+ * where that is 0); calls that run concurrently need one each.
+ */
+int vpa_paged_attention_block_scaled(
+    void* out, const void* query, const float* key_scales, const float* value_scales,
+    int64_t scale_block_stride, const void* key_cache, const void* value_cache,
+    const uint32_t* block_tables, int32_t block_table_stride, const uint32_t* cu_seqlens_q,
+    const uint32_t* context_lens, int32_t num_seqs, int32_t max_query_len,
+    int32_t max_context_len, int64_t total_query_rows, float softmax_scale, float denom_eps,
+    int32_t causal, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int64_t num_blocks, int64_t cache_block_stride,
+    int64_t cache_head_stride, int32_t dtype, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/*
+ * Blocks that several rows of the device block allocator hold (its state:
+ * vpa_allocate_rows), with one more array:
+ *   shared [num_blocks] u32   rows that hold a block besides the first
+ * all zeros before the first fork. vpa_allocate_rows and
+ * vpa_decode_step_metadata go on as they are (their blocks are fresh); rows
+ * give blocks back with vpa_release_shared_blocks in place of
+ * vpa_release_blocks. A shared block is full for all its holders, so nobody
+ * writes to it, unless a row is cut back (vpa_unshare_rows). Block 0 is not
+ * counted. No counterparts in the reference, whose blocks have one owner.
+ */
+
+/*
+ * copy_blocks - copies blocks within each of num_buffers pools (the K, V and
+ * scales of every layer): for p < min(*num_pairs, max_pairs) (num_pairs NULL:
+ * max_pairs) the block_bytes[k] bytes at block src_blocks[p] of buffer k go to
+ * block dst_blocks[p]. buffers, block_strides and block_bytes are host arrays
+ * (strides and sizes in bytes, the first num_blocks blocks of each buffer are
+ * device memory), the rest device memory. A block id >= num_blocks, or a pair
+ * of the same block, copies nothing. dst_blocks are distinct and none of them
+ * is a source. Buffers, strides and sizes that are multiples of 16 go in
+ * 16-byte vectors.
+ */
+int vpa_copy_blocks(void** buffers, const int64_t* block_strides, const int64_t* block_bytes,
+                    int32_t num_buffers, const uint32_t* src_blocks, const uint32_t* dst_blocks,
+                    const uint32_t* num_pairs, int32_t max_pairs, int64_t num_blocks,
+                    void* stream);
+
+/*
+ * fork_rows - row dst_rows[f], which holds no blocks, becomes a copy of row
+ * src_rows[f]: of its first min(positions, blocks * block_size) tokens, the
+ * whole blocks are shared and a partly filled one is to be copied to a fresh
+ * block of the ring. In index order: ok[f] = 0, and nothing changes for the row,
+ * where dst holds blocks or is an earlier fork's, where a row is >= num_rows or
+ * where the ring has no block left. Sources are read as they stand before the
+ * call; one may serve many forks. Pairs copy_src / copy_dst [num_forks] and
+ * their number *copy_count are for vpa_copy_blocks, which has to run before
+ * either row is written to or read. num_forks at most 1024 (VPA_ERR_UNSUPPORTED).
+ */
+int vpa_fork_rows(uint32_t* block_tables, int32_t block_table_stride, uint32_t* row_blocks,
+                  uint32_t* positions, uint32_t* shared, int64_t num_blocks,
+                  const uint32_t* src_rows, const uint32_t* dst_rows, int32_t num_forks,
+                  uint8_t* ok, uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
+                  uint32_t* free_ring, uint32_t* free_ring_state, int32_t free_ring_capacity,
+                  int32_t block_size, int32_t num_rows, void* stream);
+
+/*
+ * release_shared_blocks - vpa_release_blocks where blocks may have several
+ * holders: each block a row gives back loses a holder, and goes to the ring
+ * with its last one, as if the rows were taken in index order, last block
+ * first.
+ */
+int vpa_release_shared_blocks(uint32_t* block_tables, int32_t block_table_stride,
+                              uint32_t* row_blocks, uint32_t* shared, int64_t num_blocks,
+                              const uint32_t* keep_blocks, uint32_t* free_ring,
+                              uint32_t* free_ring_state, int32_t free_ring_capacity,
+                              int32_t num_rows, void* stream);
+
+/*
+ * unshare_rows - every row whose next token (positions[r]) falls inside a block
+ * that others hold too takes a fresh block from the ring in its place, in index
+ * order; the last holder keeps the block. Needed after a row was cut back to
+ * fewer tokens than it shares, before it is appended to. ok[r] = 0 for a row the
+ * ring cannot serve, which must not be appended to; 1 otherwise. Pairs
+ * copy_src / copy_dst [num_rows] and *copy_count as in vpa_fork_rows.
+ */
+int vpa_unshare_rows(uint32_t* block_tables, int32_t block_table_stride, uint32_t* row_blocks,
+                     const uint32_t* positions, uint32_t* shared, int64_t num_blocks,
+                     uint8_t* ok, uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
+                     uint32_t* free_ring, uint32_t* free_ring_state, int32_t free_ring_capacity,
+                     int32_t block_size, int32_t num_rows, void* stream);
+
+/* Bytes of caller workspace vpa_compact_blocks needs; 0 where num_blocks is. */
+size_t vpa_compact_blocks_workspace_size(int64_t num_blocks);
+
+/*
+ * compact_blocks - brings the n blocks that are not in the ring to ids 1 .. n,
+ * so that a pool can be cut or its end given away: the k-th of them past n
+ * moves to the k-th free id up to n. The rows' tables (and `shared`, where not
+ * NULL) follow, the ring becomes n + 1 .. num_blocks - 1 in order. The moves,
+ * *copy_count pairs copy_src / copy_dst ([num_blocks] each), are for
+ * vpa_copy_blocks, which has to run before any row is read or written; ids
+ * that a caller keeps elsewhere move by the same pairs. The ring's ids are
+ * distinct. num_blocks at most 2^31 - 1. workspace:
+ * vpa_compact_blocks_workspace_size bytes, 256-byte aligned; calls that run
+ * concurrently need one each.
+ */
+int vpa_compact_blocks(uint32_t* block_tables, int32_t block_table_stride,
+                       const uint32_t* row_blocks, uint32_t* shared, int64_t num_blocks,
+                       uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
+                       uint32_t* free_ring, uint32_t* free_ring_state,
+                       int32_t free_ring_capacity, int32_t num_rows, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
+ * adjust_logits - penalties for repeated tokens, biases and grammar masks, in
+ * place, before a token is chosen (vpa_argmax_rows, vpa_verify_draft_tokens).
+ * No counterpart in the reference, which decodes greedily.
+ *
+ * logits [num_seqs, rows_per_seq, vocab] of dtype, strides in elements, vocab
+ * contiguous, rows distinct. Let c be how often token v occurs in
+ * generated[b, 0 .. gen_len[b] - 1] and, for row i, among draft_ids[b, 0 ..
+ * i - 1] (NULL: no drafts). Then, in f32 and rounded once,
+ *   x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *                                     if c > 0 or v is in prompt[b, 0 ..
+ *                                     prompt_len[b] - 1]
+ *   x = x - frequency[b] * c;  x = x - presence[b]          if c > 0
+ *   x = x + bias[b, e]     e the last entry < bias_len[b] with bias_ids[b, e] = v
+ *   x = -inf               if the row has a mask and its bit v is 0
+ * repetition, presence and frequency [num_seqs] f32, each NULL for none;
+ * generated, prompt and bias_ids u32, generated_stride etc. the entries of a
+ * row (lengths are clamped to them; a NULL length: all), NULL for none;
+ * draft_ids u32 [num_seqs, rows_per_seq - 1]. Ids >= vocab are ignored.
+ * allowed u32 [num_masks, allowed_stride], bit v % 32 of word v / 32,
+ * allowed_stride >= ceil(vocab / 32); row b * rows_per_seq + i has mask
+ * allowed_rows[row] (one >= num_masks: no mask), or with NULL the mask of its
+ * own index. generated_stride + rows_per_seq at most 2^20, bias_stride at most
+ * 1024 (VPA_ERR_UNSUPPORTED).
+ */
+int vpa_adjust_logits(void* logits, int64_t seq_stride, int64_t row_stride, int32_t num_seqs,
+                      int32_t rows_per_seq, int32_t vocab, int32_t dtype,
+                      const uint32_t* generated, int32_t generated_stride,
+                      const uint32_t* gen_len, const uint32_t* prompt, int32_t prompt_stride,
+                      const uint32_t* prompt_len, const uint32_t* draft_ids,
+                      const float* repetition, const float* presence, const float* frequency,
+                      const uint32_t* bias_ids, const float* bias, int32_t bias_stride,
+                      const uint32_t* bias_len, const uint32_t* allowed, int32_t num_masks,
+                      int32_t allowed_stride, const uint32_t* allowed_rows, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

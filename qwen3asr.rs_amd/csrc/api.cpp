@@ -120,6 +120,39 @@ int check_cache(const char* op, int32_t cache_dtype, int32_t num_kv_heads, int32
   return VPA_OK;
 }
 
+// The scales of a block-scaled cache.
+int check_block_scales(const char* op, const float* key_scales, const float* value_scales,
+                       int64_t scale_block_stride, int32_t num_kv_heads) {
+  if (key_scales == nullptr || value_scales == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: key_scales and value_scales must be non-null", op);
+  if ((reinterpret_cast<uintptr_t>(key_scales) & 3u) != 0 ||
+      (reinterpret_cast<uintptr_t>(value_scales) & 3u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: key_scales / value_scales must be 4-byte aligned",
+                op);
+  if (scale_block_stride < num_kv_heads)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: scale_block_stride=%lld smaller than num_kv_heads=%d",
+                op, (long long)scale_block_stride, num_kv_heads);
+  return VPA_OK;
+}
+
+// The block allocator's state with shared blocks.
+int check_pages(const char* op, const PageState& s, bool needs_positions,
+                bool shared_optional = false) {
+  if (s.num_rows < 0 || s.cols < 0 || s.block_size <= 0 || s.num_blocks <= 0 || s.ring_cap <= 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_rows=%d block_table_stride=%d block_size=%d num_blocks=%lld "
+                "free_ring_capacity=%d",
+                op, s.num_rows, s.cols, s.block_size, (long long)s.num_blocks, s.ring_cap);
+  if (s.ring == nullptr || s.ring_state == nullptr || (s.shared == nullptr && !shared_optional) ||
+      (s.num_rows > 0 && (s.row_blocks == nullptr || (needs_positions && s.positions == nullptr) ||
+                          (s.cols > 0 && s.block_tables == nullptr))))
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: block_tables, row_blocks, %sshared, free_ring and free_ring_state must be "
+                "non-null",
+                op, needs_positions ? "positions, " : "");
+  return VPA_OK;
+}
+
 }  // namespace
 
 int device_cu_count() {
@@ -1209,6 +1242,341 @@ int vpa_verify_draft_tokens(uint32_t* out_ids, uint32_t* out_count, const void* 
                      draft_row_stride, draft_ids, num_drafts, temperature, accept_u, sample_u,
                      num_seqs, max_drafts, vocab, out_ids, out_count, workspace};
   return hip_status(op, launch_verify(dtype, v, static_cast<hipStream_t>(stream)));
+}
+
+int vpa_reshape_and_cache_block_scaled(const void* key, const void* value,
+                                       int64_t key_token_stride, int64_t value_token_stride,
+                                       float* key_scales, float* value_scales,
+                                       int64_t scale_block_stride, void* key_cache,
+                                       void* value_cache, const int64_t* slot_mapping,
+                                       int64_t num_tokens, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t block_size, int64_t num_blocks,
+                                       int64_t cache_block_stride, int64_t cache_head_stride,
+                                       int32_t dtype, void* stream) {
+  clear_error();
+  const char* op = "reshape_and_cache_block_scaled";
+  if (num_tokens < 0) return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_tokens < 0", op);
+  if (!is_float_dtype(dtype))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: unsupported input dtype %s", op, dtype_name(dtype));
+  int rc = check_cache(op, VPA_DTYPE_FP8_E4M3, num_kv_heads, head_dim, block_size, num_blocks,
+                       cache_block_stride, cache_head_stride, key_cache, value_cache);
+  if (rc != VPA_OK) return rc;
+  rc = check_block_scales(op, key_scales, value_scales, scale_block_stride, num_kv_heads);
+  if (rc != VPA_OK) return rc;
+  if (num_tokens == 0) return VPA_OK;
+  if (key == nullptr || value == nullptr || slot_mapping == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: key, value and slot_mapping must be non-null", op);
+  const int64_t row = (int64_t)num_kv_heads * head_dim;
+  if (key_token_stride < row || value_token_stride < row)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: token stride (key=%lld value=%lld) smaller than num_kv_heads*head_dim=%lld",
+                op, (long long)key_token_stride, (long long)value_token_stride, (long long)row);
+  const int eb = dtype_bytes(dtype);
+  if (!aligned16(key) || !aligned16(value) || (key_token_stride * eb) % 16 != 0 ||
+      (value_token_stride * eb) % 16 != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: key/value rows must be 16-byte aligned", op);
+  // (256-lane workgroups on a 1D grid whose lane count must fit in 32 bits)
+  if ((num_tokens + block_size - 1) / block_size > 0xffffffLL / num_kv_heads)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: too many tokens for one launch: %lld", op,
+                (long long)num_tokens);
+  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
+                    cache_head_stride};
+  const ScaledAppendArgs a{key, value, key_token_stride, value_token_stride, key_scales,
+                           value_scales, scale_block_stride, key_cache, value_cache,
+                           slot_mapping, num_tokens};
+  return hip_status(op, launch_scaled_append(dtype, a, g, static_cast<hipStream_t>(stream)));
+}
+
+size_t vpa_paged_attention_block_scaled_workspace_size(int32_t num_seqs, int32_t max_query_len,
+                                                       int32_t max_context_len,
+                                                       int64_t total_query_rows,
+                                                       int32_t num_heads, int32_t num_kv_heads,
+                                                       int32_t head_dim, int32_t dtype) {
+  if (num_seqs <= 0 || max_query_len <= 0 || max_context_len <= 0 || total_query_rows <= 0 ||
+      num_kv_heads <= 0 || num_heads < num_kv_heads || head_dim <= 0)
+    return 0;
+  return scaled_plan(dtype, num_seqs, max_query_len, max_context_len, total_query_rows, num_heads,
+                     num_kv_heads, head_dim)
+      .workspace_bytes;
+}
+
+int vpa_paged_attention_block_scaled(
+    void* out, const void* query, const float* key_scales, const float* value_scales,
+    int64_t scale_block_stride, const void* key_cache, const void* value_cache,
+    const uint32_t* block_tables, int32_t block_table_stride, const uint32_t* cu_seqlens_q,
+    const uint32_t* context_lens, int32_t num_seqs, int32_t max_query_len,
+    int32_t max_context_len, int64_t total_query_rows, float softmax_scale, float denom_eps,
+    int32_t causal, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int64_t num_blocks, int64_t cache_block_stride,
+    int64_t cache_head_stride, int32_t dtype, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  clear_error();
+  const char* op = "paged_attention_block_scaled";
+  if (!is_float_dtype(dtype))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: unsupported query dtype %s", op, dtype_name(dtype));
+  int rc = check_cache(op, VPA_DTYPE_FP8_E4M3, num_kv_heads, head_dim, block_size, num_blocks,
+                       cache_block_stride, cache_head_stride, key_cache, value_cache);
+  if (rc != VPA_OK) return rc;
+  rc = check_block_scales(op, key_scales, value_scales, scale_block_stride, num_kv_heads);
+  if (rc != VPA_OK) return rc;
+  if (num_seqs < 0 || num_heads <= 0 || max_query_len < 0 || max_context_len < 0 ||
+      total_query_rows < 0 || block_table_stride < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_seqs=%d num_heads=%d max_query_len=%d max_context_len=%d "
+                "total_query_rows=%lld block_table_stride=%d",
+                op, num_seqs, num_heads, max_query_len, max_context_len,
+                (long long)total_query_rows, block_table_stride);
+  if (num_heads % num_kv_heads != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_heads=%d not a multiple of num_kv_heads=%d",
+                op, num_heads, num_kv_heads);
+  if (!(denom_eps >= 0.f && denom_eps <= 3.402823466e38f))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: denom_eps must be finite and >= 0, got %g", op,
+                (double)denom_eps);
+  if (num_seqs == 0 || max_query_len == 0 || total_query_rows == 0) return VPA_OK;
+  if (max_context_len > (1 << 28))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: max_context_len=%d exceeds %d", op, max_context_len,
+                1 << 28);
+  const int64_t group = num_heads / num_kv_heads;
+  const ScaledPlan p = [&] {
+    if (max_query_len * group > 0xffffff || (int64_t)num_seqs * num_kv_heads > 0xffffff ||
+        total_query_rows > ((int64_t)1 << 40))
+      return ScaledPlan{};  // (grid 0: refused below)
+    return scaled_plan(dtype, num_seqs, max_query_len, max_context_len, total_query_rows,
+                       num_heads, num_kv_heads, head_dim);
+  }();
+  // (256-lane workgroups: a grid's lane count must fit in 32 bits; the joining launch
+  // has a workgroup per four rows)
+  if (p.grid <= 0 || p.grid > 0xffffff ||
+      (p.max_chunks > 1 &&
+       ((int64_t)max_query_len * num_heads + 3) / 4 > (int64_t)0xffffff / num_seqs))
+    return fail(VPA_ERR_UNSUPPORTED,
+                "%s: num_seqs=%d, num_heads=%d, max_query_len=%d and max_context_len=%d are too "
+                "many rows and tokens for one launch",
+                op, num_seqs, num_heads, max_query_len, max_context_len);
+  if (out == nullptr || query == nullptr || context_lens == nullptr ||
+      (block_tables == nullptr && max_context_len > 0))
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: out, query, block_tables and context_lens must be non-null", op);
+  if (!aligned16(out) || !aligned16(query))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: out and query must be 16-byte aligned", op);
+  if ((int64_t)block_table_stride * block_size < max_context_len)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: block_table_stride=%d too small for max_context_len=%d (block_size=%d)", op,
+                block_table_stride, max_context_len, block_size);
+  if (p.workspace_bytes > 0 && (workspace == nullptr || workspace_bytes < p.workspace_bytes))
+    return fail(VPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", op,
+                p.workspace_bytes, workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", op);
+  const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,
+                    cache_head_stride};
+  const ScaledArgs a{out, query, key_scales, value_scales, scale_block_stride, key_cache,
+                     value_cache, block_tables, block_table_stride, cu_seqlens_q, context_lens,
+                     num_seqs, max_query_len, max_context_len, total_query_rows, softmax_scale,
+                     denom_eps, causal != 0, num_heads, workspace};
+  const auto launch = dtype == VPA_DTYPE_BF16  ? launch_scaled_attention_bf16
+                      : dtype == VPA_DTYPE_F16 ? launch_scaled_attention_f16
+                                               : launch_scaled_attention_f32;
+  return hip_status(op, launch(a, g, p, static_cast<hipStream_t>(stream)));
+}
+
+int vpa_copy_blocks(void** buffers, const int64_t* block_strides, const int64_t* block_bytes,
+                    int32_t num_buffers, const uint32_t* src_blocks, const uint32_t* dst_blocks,
+                    const uint32_t* num_pairs, int32_t max_pairs, int64_t num_blocks,
+                    void* stream) {
+  clear_error();
+  const char* op = "copy_blocks";
+  if (num_buffers < 0 || max_pairs < 0 || num_blocks < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_buffers=%d max_pairs=%d num_blocks=%lld", op, num_buffers,
+                max_pairs, (long long)num_blocks);
+  if (num_buffers == 0 || max_pairs == 0) return VPA_OK;
+  if (buffers == nullptr || block_strides == nullptr || block_bytes == nullptr ||
+      src_blocks == nullptr || dst_blocks == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: buffers, block_strides, block_bytes, src_blocks and dst_blocks must be "
+                "non-null",
+                op);
+  for (int k = 0; k < num_buffers; ++k) {
+    if (buffers[k] == nullptr && block_bytes[k] > 0)
+      return fail(VPA_ERR_INVALID_ARGUMENT, "%s: buffer %d must be non-null", op, k);
+    if (block_bytes[k] < 0 || block_bytes[k] > 0x7fffffffLL || block_strides[k] < block_bytes[k])
+      return fail(VPA_ERR_INVALID_ARGUMENT,
+                  "%s: buffer %d: a block of %lld bytes every %lld (at most 2^31 - 1, and not more "
+                  "than the stride)",
+                  op, k, (long long)block_bytes[k], (long long)block_strides[k]);
+  }
+  for (int first = 0; first < num_buffers; first += kCopyMaxBuffers) {
+    CopyBuffers b{};
+    const int n = std::min(num_buffers - first, kCopyMaxBuffers);
+    for (int k = 0; k < n; ++k) {
+      b.base[k] = static_cast<char*>(buffers[first + k]);
+      b.stride[k] = block_strides[first + k];
+      b.bytes[k] = (uint32_t)block_bytes[first + k];
+    }
+    const int rc = hip_status(op, launch_copy_blocks(b, n, src_blocks, dst_blocks, num_pairs,
+                                                     max_pairs, num_blocks,
+                                                     static_cast<hipStream_t>(stream)));
+    if (rc != VPA_OK) return rc;
+  }
+  return VPA_OK;
+}
+
+int vpa_fork_rows(uint32_t* block_tables, int32_t block_table_stride, uint32_t* row_blocks,
+                  uint32_t* positions, uint32_t* shared, int64_t num_blocks,
+                  const uint32_t* src_rows, const uint32_t* dst_rows, int32_t num_forks,
+                  uint8_t* ok, uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
+                  uint32_t* free_ring, uint32_t* free_ring_state, int32_t free_ring_capacity,
+                  int32_t block_size, int32_t num_rows, void* stream) {
+  clear_error();
+  const char* op = "fork_rows";
+  const PageState s{block_tables, block_table_stride, row_blocks, positions, shared, num_blocks,
+                    free_ring, free_ring_state, free_ring_capacity, block_size, num_rows};
+  const int rc = check_pages(op, s, true);
+  if (rc != VPA_OK) return rc;
+  if (num_forks < 0) return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_forks=%d < 0", op, num_forks);
+  if (num_forks > kMaxForks)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_forks=%d exceeds %d", op, num_forks, kMaxForks);
+  if (copy_count == nullptr || (num_forks > 0 && (src_rows == nullptr || dst_rows == nullptr ||
+                                                  ok == nullptr || copy_src == nullptr ||
+                                                  copy_dst == nullptr)))
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: src_rows, dst_rows, ok, copy_src, copy_dst and copy_count must be non-null",
+                op);
+  return hip_status(op, launch_fork_rows(s, src_rows, dst_rows, num_forks, ok, copy_src, copy_dst,
+                                         copy_count, static_cast<hipStream_t>(stream)));
+}
+
+int vpa_release_shared_blocks(uint32_t* block_tables, int32_t block_table_stride,
+                              uint32_t* row_blocks, uint32_t* shared, int64_t num_blocks,
+                              const uint32_t* keep_blocks, uint32_t* free_ring,
+                              uint32_t* free_ring_state, int32_t free_ring_capacity,
+                              int32_t num_rows, void* stream) {
+  clear_error();
+  const char* op = "release_shared_blocks";
+  const PageState s{block_tables, block_table_stride, row_blocks, nullptr, shared, num_blocks,
+                    free_ring, free_ring_state, free_ring_capacity, 1, num_rows};
+  const int rc = check_pages(op, s, false);
+  if (rc != VPA_OK) return rc;
+  if (num_rows == 0) return VPA_OK;
+  if (keep_blocks == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: keep_blocks must be non-null", op);
+  // (an entry's place in the order is kept in 31 bits)
+  if ((int64_t)num_rows * block_table_stride > 0x7ffffffeLL)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_rows=%d times block_table_stride=%d reaches 2^31 - 1",
+                op, num_rows, block_table_stride);
+  return hip_status(op, launch_release_shared(s, keep_blocks, static_cast<hipStream_t>(stream)));
+}
+
+int vpa_unshare_rows(uint32_t* block_tables, int32_t block_table_stride, uint32_t* row_blocks,
+                     const uint32_t* positions, uint32_t* shared, int64_t num_blocks,
+                     uint8_t* ok, uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
+                     uint32_t* free_ring, uint32_t* free_ring_state, int32_t free_ring_capacity,
+                     int32_t block_size, int32_t num_rows, void* stream) {
+  clear_error();
+  const char* op = "unshare_rows";
+  const PageState s{block_tables, block_table_stride, row_blocks,
+                    const_cast<uint32_t*>(positions),  // (only read)
+                    shared, num_blocks, free_ring, free_ring_state, free_ring_capacity, block_size,
+                    num_rows};
+  const int rc = check_pages(op, s, true);
+  if (rc != VPA_OK) return rc;
+  if (copy_count == nullptr ||
+      (num_rows > 0 && (ok == nullptr || copy_src == nullptr || copy_dst == nullptr)))
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: ok, copy_src, copy_dst and copy_count must be non-null", op);
+  return hip_status(op, launch_unshare_rows(s, ok, copy_src, copy_dst, copy_count,
+                                            static_cast<hipStream_t>(stream)));
+}
+
+size_t vpa_compact_blocks_workspace_size(int64_t num_blocks) {
+  return num_blocks > 0 ? compact_workspace_bytes(num_blocks) : 0;
+}
+
+int vpa_compact_blocks(uint32_t* block_tables, int32_t block_table_stride,
+                       const uint32_t* row_blocks, uint32_t* shared, int64_t num_blocks,
+                       uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
+                       uint32_t* free_ring, uint32_t* free_ring_state,
+                       int32_t free_ring_capacity, int32_t num_rows, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* op = "compact_blocks";
+  const PageState s{block_tables, block_table_stride,
+                    const_cast<uint32_t*>(row_blocks),  // (only read)
+                    nullptr, shared, num_blocks, free_ring, free_ring_state, free_ring_capacity,
+                    1, num_rows};
+  const int rc = check_pages(op, s, false, true);
+  if (rc != VPA_OK) return rc;
+  if (num_blocks > 0x7fffffffLL)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: num_blocks=%lld reaches 2^31", op, (long long)num_blocks);
+  if (copy_src == nullptr || copy_dst == nullptr || copy_count == nullptr)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: copy_src, copy_dst and copy_count must be non-null",
+                op);
+  const size_t need = compact_workspace_bytes(num_blocks);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(VPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", op, need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: workspace must be 256-byte aligned", op);
+  return hip_status(op, launch_compact(s, copy_src, copy_dst, copy_count, workspace,
+                                       static_cast<hipStream_t>(stream)));
+}
+
+int vpa_adjust_logits(void* logits, int64_t seq_stride, int64_t row_stride, int32_t num_seqs,
+                      int32_t rows_per_seq, int32_t vocab, int32_t dtype,
+                      const uint32_t* generated, int32_t generated_stride,
+                      const uint32_t* gen_len, const uint32_t* prompt, int32_t prompt_stride,
+                      const uint32_t* prompt_len, const uint32_t* draft_ids,
+                      const float* repetition, const float* presence, const float* frequency,
+                      const uint32_t* bias_ids, const float* bias, int32_t bias_stride,
+                      const uint32_t* bias_len, const uint32_t* allowed, int32_t num_masks,
+                      int32_t allowed_stride, const uint32_t* allowed_rows, void* stream) {
+  clear_error();
+  const char* op = "adjust_logits";
+  if (!is_float_dtype(dtype))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: unsupported logits dtype %s", op, dtype_name(dtype));
+  if (num_seqs < 0 || rows_per_seq < 0 || vocab < 0 || generated_stride < 0 || prompt_stride < 0 ||
+      bias_stride < 0 || num_masks < 0 || allowed_stride < 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_seqs=%d rows_per_seq=%d vocab=%d generated_stride=%d "
+                "prompt_stride=%d bias_stride=%d num_masks=%d allowed_stride=%d",
+                op, num_seqs, rows_per_seq, vocab, generated_stride, prompt_stride, bias_stride,
+                num_masks, allowed_stride);
+  if (num_seqs == 0 || rows_per_seq == 0 || vocab == 0) return VPA_OK;
+  if ((int64_t)generated_stride + rows_per_seq > (1 << 20))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: generated_stride=%d and rows_per_seq=%d exceed 2^20", op,
+                generated_stride, rows_per_seq);
+  if (bias_stride > kAdjustMaxBias)
+    return fail(VPA_ERR_UNSUPPORTED, "%s: bias_stride=%d exceeds %d", op, bias_stride,
+                kAdjustMaxBias);
+  if (logits == nullptr) return fail(VPA_ERR_INVALID_ARGUMENT, "%s: logits must be non-null", op);
+  if (reinterpret_cast<uintptr_t>(logits) % (uintptr_t)dtype_bytes(dtype) != 0)
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: misaligned logits", op);
+  // (rows are written: none may lie in another)
+  if ((rows_per_seq > 1 && row_stride < vocab) ||
+      (num_seqs > 1 && seq_stride < (rows_per_seq - 1) * row_stride + vocab))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: logits rows overlap: strides %lld and %lld", op,
+                (long long)seq_stride, (long long)row_stride);
+  if ((bias_ids == nullptr) != (bias == nullptr))
+    return fail(VPA_ERR_INVALID_ARGUMENT, "%s: bias_ids and bias go together", op);
+  const int64_t rows = (int64_t)num_seqs * rows_per_seq;
+  if (allowed != nullptr) {
+    if ((int64_t)allowed_stride * 32 < vocab)
+      return fail(VPA_ERR_INVALID_ARGUMENT, "%s: allowed_stride=%d too small for vocab=%d", op,
+                  allowed_stride, vocab);
+    if (allowed_rows == nullptr && num_masks < rows)
+      return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_masks=%d, but %lld rows without allowed_rows",
+                  op, num_masks, (long long)rows);
+  }
+  // (512-lane workgroups: the grid's lane count must fit in 32 bits; a row has at most
+  // one per 16384 tokens for its mask and per 32768 for its lists)
+  if (vocab > (1 << 30) || rows > 0x7fffffLL / (((int64_t)vocab + 16383) / 16384 * 2))
+    return fail(VPA_ERR_UNSUPPORTED, "%s: too many logits for one launch", op);
+  const AdjustArgs a{logits, seq_stride, row_stride, num_seqs, rows_per_seq, vocab, generated,
+                     generated_stride, gen_len, prompt, prompt_stride, prompt_len, draft_ids,
+                     repetition, presence, frequency, bias_ids, bias, bias_stride, bias_len,
+                     allowed, num_masks, allowed_stride, allowed_rows};
+  return hip_status(op, launch_adjust_logits(dtype, a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,780 @@
+// Attention over a paged cache of E4M3 bytes with one scale per (block, kv
+// head), for K and for V (gfx950 MFMA). One kernel serves a decode step, drafted
+// tokens and the rows of a prompt; the files that include it hold its instances
+// for one query type each.
+//
+// For query row r, its sequence's cached tokens t and their block b(t):
+//   s_t = softmax_scale * ks[b(t)] * (q_r . K_t)       K_t, V_t: the bytes' values
+//   out = sum_t p_t vs[b(t)] V_t / (sum_t p_t + eps),  p_t = exp(s_t - max_t s_t)
+// over the tokens the row sees. The scales are applied where they are cheap and
+// exact enough: ks to the f32 scores, vs to the f32 probabilities, so the bytes
+// themselves go through the matrix instructions unscaled (every E4M3 value is
+// exact in f16 and in bf16) and scales of any size neither overflow nor round.
+//
+// Work of a wave: 16 NQ rows (a row is a position and a query head of the kv
+// head; heads fastest, so any group size fills the rows) over 64 keys at a time
+// = 4 tiles of 16 keys. S^T = K Q^T with v_mfma_f32_16x16x32: lane l gives token
+// l % 16 of a tile and, as K's 16-byte vectors hold 16 dims of a token, the dims
+// 16 (l / 16) + 64 i .. + 15, one load for two k-steps; Q is loaded in the same
+// order. The result holds, per lane, column (row of Q) l % 16 and tokens
+// 4 (l / 16) .. + 3 of each tile. O^T += V^T P^T takes V's rows as they lie:
+// lane l holds dim l % 16 and the 16 tokens of tile l / 16, which are two
+// k-steps of 8. P^T has to follow: lane row g needs tile g's 16 tokens where it
+// has 4 tokens of each tile, a transposition of 4 x 4 registers by lane rows,
+// eight v_permlane swaps for 64 keys. So no value of K, V or P goes through LDS
+// and the waves run without barriers; LDS only joins the waves' results at the end.
+//
+// Precision: scores, softmax and sums are f32. P goes through the matrix
+// instructions as f16 (V's bytes are exact in f16 whatever the query's type):
+// rounded to 11 bits, off by at most 2^-11 of itself; f32 queries use two f16
+// values (22 bits), and three bf16 values for Q, which hold an f32 exactly. The
+// probabilities stay below 2^kSlack (the reference maximum moves only when it is
+// exceeded by more) and are scaled by 2^kProbLog2, which keeps f16's smallest
+// step at 2^-31 of a probability of 1. vs enters as its ratio to the largest one
+// met so far (`vref`), so that the ratio is at most 1; like the maximum, vref
+// moving rescales the sums.
+//
+// Few rows (decode): the waves of a workgroup split a chunk's keys, 64 at a time,
+// and are joined in LDS; long contexts are split in chunks over workgroups and
+// joined by a second launch (scaled_merge_kernel). Many rows: every wave has its
+// own rows and all read the same keys, through L2.
+#pragma once
+
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "vpa_device.h"
+#include "vpa_internal.h"
+
+namespace vpa {
+namespace {
+
+typedef __bf16 sa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 sa_f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+template <typename K>
+__device__ __forceinline__ f32x4_t mfma16x16x32(const uint4& a, const uint4& b, const f32x4_t& c) {
+  if constexpr (std::is_same_v<K, f16_t>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sa_f16x8, a),
+                                                  __builtin_bit_cast(sa_f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sa_bf16x8, a),
+                                                   __builtin_bit_cast(sa_bf16x8, b), c, 0, 0, 0);
+}
+
+constexpr int kScaledWaves = 4;
+constexpr int kScaledKeys = 64;  // keys of a step
+constexpr float kScaledSlack = 8.f;
+constexpr int kScaledProbLog2 = 7;
+
+// Maximum / sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_rows(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_rows(float v) { return sum_xor32(sum_xor16(v)); }
+
+// w[b] of lane row g -> w[g] of lane row b (4 x 4, by lane rows).
+__device__ __forceinline__ void transpose_rows(uint32_t (&w)[4]) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(w[b], w[b + 2], false, false);
+    w[b] = r[0];
+    w[b + 2] = r[1];
+  }
+#pragma unroll
+  for (int b = 0; b < 4; b += 2) {
+    const auto r = __builtin_amdgcn_permlane16_swap(w[b], w[b + 1], false, false);
+    w[b] = r[0];
+    w[b + 1] = r[1];
+  }
+}
+
+struct ScaledDev {
+  const void* query;
+  const uint8_t* key_cache;
+  const uint8_t* value_cache;
+  const float* key_scales;
+  const float* value_scales;
+  int64_t scale_block_stride;
+  const uint32_t* block_tables;
+  const uint32_t* cu_seqlens_q;
+  const uint32_t* context_lens;
+  void* out;
+  float* part_out;   // [total rows * heads][max_chunks][D]
+  float* part_stat;  // [total rows * heads][max_chunks][2]: maximum, sum
+  int64_t block_stride, head_stride;  // bytes
+  int64_t num_blocks, total_rows;
+  int32_t block_table_stride, num_seqs, max_query_len, max_ctx;
+  int32_t num_heads, num_kv_heads, group, causal;
+  int32_t tiles, chunk_tokens, max_chunks;
+  int32_t split_keys;  // the waves share 16 NQ rows and split the keys
+  int32_t lds_rows;    // rows kept in LDS then
+  float scale_log2, denom_eps;
+};
+
+// Query types and head dims whose waves may take two tiles of 16 rows.
+template <typename T>
+constexpr bool scaled_two_tiles(int head_dim) {
+  return !std::is_same_v<T, float> && head_dim <= 128;
+}
+
+// Waves per SIMD: O, Q and two tiles' bytes are what a wave holds.
+template <typename T, int D, int NQ>
+constexpr int scaled_waves_per_eu() {
+  return D <= 128 ? 2 : 1;
+}
+
+template <typename T, int D, int BS, int NQ>
+__global__ __launch_bounds__(64 * kScaledWaves)
+__attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scaled_attention_kernel(
+    const ScaledDev a) {
+  constexpr bool kF32 = std::is_same_v<T, float>;
+  using K = std::conditional_t<std::is_same_v<T, f16_t>, f16_t, bf16_t>;  // of S's operands
+  constexpr int QP = kF32 ? 3 : 1;   // parts of Q
+  constexpr int PP = kF32 ? 2 : 1;   // parts of P
+  constexpr int NC = (D + 63) / 64;  // loads of a lane per 16-key tile of K
+  constexpr int DT = D / 16;
+  constexpr int CH = D / 16;  // 16-byte chunks of a key
+  // Where a wave's registers hold two tiles' bytes besides its sums, V is under
+  // way while S is computed and the next K during the softmax; otherwise V
+  // during the softmax and the next K during P.V.
+  constexpr bool kEarly = NQ == 1 && D <= 128;
+
+  extern __shared__ float s_join[];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, kg = lane >> 4;
+  // kv heads vary fastest, then a sequence's row tiles (the last, which see most
+  // keys, first): workgroups that read the same keys are close and, at 8 kv heads,
+  // on one XCD
+  uint32_t w = blockIdx.x;
+  const int j = (int)(w % (uint32_t)a.num_kv_heads);
+  w /= (uint32_t)a.num_kv_heads;
+  const int qt = a.tiles - 1 - (int)(w % (uint32_t)a.tiles);
+  w /= (uint32_t)a.tiles;
+  const int s = (int)(w % (uint32_t)a.num_seqs);
+  const int chunk = (int)(w / (uint32_t)a.num_seqs);
+
+  uint32_t qa = (uint32_t)s, qb = (uint32_t)s + 1u;
+  if (a.cu_seqlens_q != nullptr) {
+    qa = a.cu_seqlens_q[s];
+    qb = a.cu_seqlens_q[s + 1];
+  }
+  int n = qb > qa ? (int)min(qb - qa, (uint32_t)a.max_query_len) : 0;
+  n = (int64_t)qa >= a.total_rows ? 0 : (int)min((int64_t)n, a.total_rows - (int64_t)qa);
+  const int L = (int)min(a.context_lens[s], (uint32_t)a.max_ctx);
+  const int rows = n * a.group;
+  const int wg_rows = (a.split_keys ? 1 : kScaledWaves) * 16 * NQ;
+  if (qt * wg_rows >= rows) return;  // (uniform over the workgroup)
+  const int nchunks = max(1, (L + a.chunk_tokens - 1) / a.chunk_tokens);
+  if (chunk >= nchunks) return;
+  const int r0 = qt * wg_rows + (a.split_keys ? 0 : wave * 16 * NQ);
+
+  // keys that some row of the wave sees, and the part of them here
+  const int shift = L - n;
+  const int last_pos = (min(r0 + 16 * NQ, rows) - 1) / a.group;  // r0 may be past the rows
+  int n_keys = r0 >= rows ? 0 : a.causal ? min(L, last_pos + shift + 1) : L;
+  n_keys = max(n_keys, 0);
+  const int k_end = min(n_keys, (chunk + 1) * a.chunk_tokens);
+  const int k_step = a.split_keys ? kScaledKeys * kScaledWaves : kScaledKeys;
+  const int k_first = chunk * a.chunk_tokens + (a.split_keys ? wave * kScaledKeys : 0);
+  // the last key that every row of the wave sees
+  const int all_see = a.causal ? r0 / a.group + shift : L - 1;
+
+  int limit[NQ];  // last key of this lane's rows (the lane's column of S^T)
+  int64_t orow[NQ];  // their row of `out`, -1: none
+  uint4 qop[NQ][QP][2 * NC];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int r = r0 + 16 * q + c16;
+    const bool ok = r < rows;
+    const int pos = ok ? r / a.group : 0;
+    const int64_t row = ((int64_t)qa + pos) * a.num_heads + (int64_t)j * a.group + (ok ? r % a.group : 0);
+    orow[q] = ok ? row : -1;
+    limit[q] = !ok ? -1 : a.causal ? pos + shift : L - 1;
+    const T* src = static_cast<const T*>(a.query) + row * D;
+#pragma unroll
+    for (int st = 0; st < 2 * NC; ++st) {
+      const int dim = 16 * (kg + 4 * (st / 2)) + 8 * (st % 2);
+      const bool in = dim < D;  // (head dims 96 and 192... end inside a step: zeros)
+      if constexpr (kF32) {
+        uint32_t part[3][4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const float4 v = in ? *reinterpret_cast<const float4*>(src + dim + e)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+          float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+#pragma unroll
+            for (int h = 0; h < 4; h += 2) {
+              const uint32_t pk = pack2_hw<bf16_t>(x[h], x[h + 1]);
+              part[p][(e + h) / 2] = pk;
+              x[h] -= low_half_f32<bf16_t>(pk);
+              x[h + 1] -= high_half_f32<bf16_t>(pk);
+            }
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          qop[q][p][st] = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+      } else {
+        qop[q][0][st] = in ? *reinterpret_cast<const uint4*>(src + dim) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+
+  f32x4_t o[NQ][DT];
+  float m[NQ], mt[NQ], lsum[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    m[q] = mt[q] = -INFINITY;
+    lsum[q] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[q][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  float vref = 1.50463277e-36f;  // 2^-119: 2^kScaledProbLog2 / vref is finite
+
+  if (k_first < k_end) {
+    const uint32_t* bt = a.block_tables + (int64_t)s * a.block_table_stride;
+    const int last_blk = (L - 1) / BS;
+    const uint8_t* kbase = a.key_cache + (int64_t)j * a.head_stride;
+    const uint8_t* vbase = a.value_cache + (int64_t)j * a.head_stride;
+    constexpr int NI = BS == 8 ? 2 : 1;  // blocks of a 16-key tile
+
+    // Ids of this lane row's tile (tile kg of the step; clamped to the last block).
+    struct Ids {
+      uint32_t id[NI];
+    };
+    auto load_ids = [&](int k0) {
+      Ids r;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) r.id[i] = bt[min((k0 + 16 * kg + 8 * i) / BS, last_blk)];
+      return r;
+    };
+    // Scales of that tile; 0 for what is past the context or absent.
+    struct Scales {
+      float k[NI], v[NI];
+    };
+    auto present = [&](uint32_t id) { return (int64_t)id < a.num_blocks; };
+    auto load_scales = [&](const Ids& d, int k0) {
+      Scales r;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const bool ok = present(d.id[i]) && k0 + 16 * kg + 8 * i < L;
+        const int64_t at = (int64_t)(ok ? d.id[i] : 0u) * a.scale_block_stride + j;
+        const float ks = a.key_scales[at], vs = a.value_scales[at];
+        r.k[i] = ok ? ks : 0.f;
+        r.v[i] = ok ? vs : 0.f;
+      }
+      return r;
+    };
+    auto load16 = [](const uint8_t* p) {
+      if constexpr (NQ == 1) return load_stream(reinterpret_cast<const uint4*>(p));
+      else return *reinterpret_cast<const uint4*>(p);
+    };
+    // absent blocks read block 0 (in bounds) and are masked
+    auto load_k = [&](const Ids& d, uint4 (&buf)[4][NC]) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint32_t id0 = (uint32_t)__builtin_amdgcn_readlane((int)d.id[0], 16 * b);
+        int64_t at = (int64_t)(present(id0) ? id0 : 0u) * a.block_stride;
+        if constexpr (NI == 2) {
+          const uint32_t id1 = (uint32_t)__builtin_amdgcn_readlane((int)d.id[1], 16 * b);
+          const int64_t at1 = (int64_t)(present(id1) ? id1 : 0u) * a.block_stride;
+          at = c16 < 8 ? at : at1;
+        }
+        const int off = BS == 8 ? (c16 & 7) : BS == 16 ? c16 : 16 * (b & 1) + c16;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int c = kg + 4 * i;
+          buf[b][i] = load16(kbase + at + ((c < CH ? c : kg) * BS + off) * 16);
+        }
+      }
+    };
+    auto load_v = [&](const Ids& d, uint4 (&buf)[DT]) {
+      const uint8_t* p[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        p[i] = vbase + (int64_t)(present(d.id[i]) ? d.id[i] : 0u) * a.block_stride + c16 * BS +
+               (BS == 32 ? 16 * (kg & 1) : 0);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        if constexpr (NI == 2) {
+          const uint2 lo = *reinterpret_cast<const uint2*>(p[0] + dt * 16 * BS);
+          const uint2 hi = *reinterpret_cast<const uint2*>(p[1] + dt * 16 * BS);
+          buf[dt] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          buf[dt] = load16(p[0] + dt * 16 * BS);
+        }
+      }
+    };
+
+    // Bytes of tokens past the context or in an absent block are stale, NaN among
+    // them, and 0 * NaN is NaN: zeros.
+    struct Keep {
+      uint32_t x[4];
+    };
+    auto keep_of = [&](const Ids& d, int k0) {
+      Keep r;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int left = present(d.id[NI == 2 ? x / 2 : 0]) ? L - (k0 + 16 * kg + 4 * x) : 0;
+        r.x[x] = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+      }
+      return r;
+    };
+    auto kept = [](const uint4& v, const Keep& k) {
+      return make_uint4(v.x & k.x[0], v.y & k.x[1], v.z & k.x[2], v.w & k.x[3]);
+    };
+    // 1 in each byte that is NaN
+    auto nan_bytes = [](uint32_t x) {
+      return (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+    };
+    bool nan_seen = false;
+
+    uint4 kraw[4][NC], vraw[DT];
+    Ids ids = load_ids(k_first), ids1 = load_ids(k_first + k_step);
+    Scales sc = load_scales(ids, k_first);
+    load_k(ids, kraw);
+
+    for (int k0 = k_first; k0 < k_end; k0 += k_step) {
+      if constexpr (kEarly) load_v(ids, vraw);
+      const Ids ids2 = load_ids(k0 + 2 * k_step);
+      const Scales sc1 = load_scales(ids1, k0 + k_step);
+
+      // ---- S^T, tile by tile ----
+      f32x4_t sv[NQ][4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        // (keeps a wave from holding every tile's operands at once)
+        if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) sv[q][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          uint4 op[2];
+          fp8x16_to_pk<K>(kraw[b][i], op[0], op[1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+              for (int p = QP - 1; p >= 0; --p)
+                sv[q][b] = mfma16x16x32<K>(op[h], qop[q][p][2 * i + h], sv[q][b]);
+        }
+      }
+      if constexpr (kEarly) {
+        if (k0 + k_step < k_end) load_k(ids1, kraw);
+      } else {
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(ids, vraw);
+      }
+
+      // ---- scales and masks ----
+      // tile b's scales and presence (8-token blocks: of this lane's half of it)
+      float vsb[4];
+      bool here[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float ksb = readlane_f(sc.k[0], 16 * b);
+        vsb[b] = readlane_f(sc.v[0], 16 * b);
+        here[b] = present((uint32_t)__builtin_amdgcn_readlane((int)ids.id[0], 16 * b));
+        if constexpr (NI == 2) {
+          const float k1 = readlane_f(sc.k[1], 16 * b), v1 = readlane_f(sc.v[1], 16 * b);
+          const bool h1 = present((uint32_t)__builtin_amdgcn_readlane((int)ids.id[1], 16 * b));
+          ksb = kg < 2 ? ksb : k1;
+          vsb[b] = kg < 2 ? vsb[b] : v1;
+          here[b] = kg < 2 ? here[b] : h1;
+        }
+        const float f = ksb * a.scale_log2;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sv[q][b][r] *= f;
+      }
+      // every key inside the context, in a present block, seen by every row
+      bool mine = present(ids.id[0]);
+      if constexpr (NI == 2) mine = mine && present(ids.id[1]);
+      const bool all_here = __ballot(!mine) == 0 && k0 + kScaledKeys <= L;
+      const bool full = all_here && k0 + kScaledKeys - 1 <= all_see;
+      if (!full) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int t = k0 + 16 * b + 4 * kg + r;
+            const bool in = here[b] && t < L;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+              sv[q][b][r] = in && t <= limit[q] ? sv[q][b][r] : -INFINITY;
+          }
+      }
+
+      // ---- online softmax ----
+      float mx[NQ];
+      bool move = false;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        mx[q] = sv[q][0][0];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx[q] = fmaxf(mx[q], sv[q][b][r]);
+        mx[q] = max_rows(mx[q]);
+        mt[q] = fmaxf(mt[q], mx[q]);
+        move = move || mx[q] > m[q] + kScaledSlack || (m[q] == -INFINITY && mx[q] > -INFINITY);
+      }
+      float vmax = fabsf(sc.v[0]);
+      if constexpr (NI == 2) vmax = fmaxf(vmax, fabsf(sc.v[1]));
+      vmax = max_rows(vmax);
+      if (__ballot(move || vmax > vref) != 0) {
+        const float vnew = fmaxf(vref, vmax);
+        const float fv = vref / vnew;
+        vref = vnew;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const float mn = fmaxf(m[q], mx[q]);
+          const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mn);
+          m[q] = mn;
+          lsum[q] *= f;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[q][dt][r] *= f * fv;
+        }
+      }
+      const float ivref = (float)(1 << kScaledProbLog2) / vref;
+
+      // ---- probabilities, as operands of P.V ----
+      uint32_t pw[NQ][PP][2][4];  // [two tokens of a tile's four][tile]
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const float mu = m[q] == -INFINITY ? 0.f : m[q];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const float f = vsb[b] * ivref;
+          float p[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(sv[q][b][r] - mu);
+            lsum[q] += p[r];
+            p[r] *= f;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            pw[q][0][h][b] = pack2_hw<f16_t>(p[2 * h], p[2 * h + 1]);
+            if constexpr (PP == 2)
+              pw[q][1][h][b] = pack2_hw<f16_t>(p[2 * h] - low_half_f32<f16_t>(pw[q][0][h][b]),
+                                               p[2 * h + 1] - high_half_f32<f16_t>(pw[q][0][h][b]));
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < PP; ++p)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) transpose_rows(pw[q][p][h]);
+      }
+
+      // ---- O^T += V^T P^T ----
+      if (!full) {
+        // A NaN value of a token that only later rows see would reach every row
+        // of the tile through 0 * NaN: such bytes count as 0 here and are gone
+        // through once more after the loop.
+        const Keep keep = keep_of(ids, k0);
+        uint32_t any = 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          __builtin_amdgcn_sched_barrier(0);
+          vraw[dt] = kept(vraw[dt], keep);
+          any |= nan_bytes(vraw[dt].x) | nan_bytes(vraw[dt].y) | nan_bytes(vraw[dt].z) |
+                 nan_bytes(vraw[dt].w);
+        }
+        if (a.causal && __ballot(any != 0) != 0) {
+          nan_seen = true;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            __builtin_amdgcn_sched_barrier(0);
+            vraw[dt].x &= ~(nan_bytes(vraw[dt].x) * 0xffu);
+            vraw[dt].y &= ~(nan_bytes(vraw[dt].y) * 0xffu);
+            vraw[dt].z &= ~(nan_bytes(vraw[dt].z) * 0xffu);
+            vraw[dt].w &= ~(nan_bytes(vraw[dt].w) * 0xffu);
+          }
+        }
+      }
+      if constexpr (!kEarly) {
+        // (past the end too, where the clamped ids read one block once more: a
+        // branch here costs the registers of a second copy of the bytes)
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(ids1, kraw);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        if constexpr (!kEarly)
+          if (dt % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        uint4 op[2];
+        fp8x16_to_pk<f16_t>(vraw[dt], op[0], op[1]);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int p = PP - 1; p >= 0; --p)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              o[q][dt] = mfma16x16x32<f16_t>(
+                  op[h],
+                  make_uint4(pw[q][p][0][2 * h], pw[q][p][1][2 * h], pw[q][p][0][2 * h + 1],
+                             pw[q][p][1][2 * h + 1]),
+                  o[q][dt]);
+      }
+      ids = ids1;
+      ids1 = ids2;
+      sc = sc1;
+    }
+
+    // NaN values of the steps that not every row sees whole: a row gets a NaN in
+    // each dim where a token it sees has one, by a product of flags.
+    if (nan_seen) {
+      for (int k0 = k_first; k0 < k_end; k0 += k_step) {
+        if (k0 + kScaledKeys - 1 <= all_see) continue;
+        ids = load_ids(k0);
+        load_v(ids, vraw);
+        const Keep keep = keep_of(ids, k0);
+        uint32_t vis[NQ][2][4];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const int t = k0 + 16 * b + 4 * kg + 2 * h;
+              vis[q][h][b] = (t <= limit[q] ? 0x3c00u : 0u) | (t < limit[q] ? 0x3c000000u : 0u);
+            }
+            transpose_rows(vis[q][h]);
+          }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          __builtin_amdgcn_sched_barrier(0);
+          const uint4 x = kept(vraw[dt], keep);
+          uint4 op[2];
+          fp8x16_to_pk<f16_t>(make_uint4(nan_bytes(x.x) * 0x38u, nan_bytes(x.y) * 0x38u,
+                                         nan_bytes(x.z) * 0x38u, nan_bytes(x.w) * 0x38u),
+                              op[0], op[1]);  // 0x38: 1.0
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            f32x4_t c{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              c = mfma16x16x32<f16_t>(op[h],
+                                      make_uint4(vis[q][0][2 * h], vis[q][1][2 * h],
+                                                 vis[q][0][2 * h + 1], vis[q][1][2 * h + 1]),
+                                      c);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[q][dt][r] = c[r] > 0.f ? NAN : o[q][dt][r];
+          }
+        }
+      }
+    }
+  }
+
+  // ---- to the true maximum, then out: whole rows, a chunk's part, or joined ----
+  float fo[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mt[q]);
+    lsum[q] = sum_rows(lsum[q]) * f;
+    fo[q] = f * (vref * (1.f / (1 << kScaledProbLog2)));
+  }
+  const bool single = nchunks == 1;
+  T* out = static_cast<T*>(a.out);
+  auto store4 = [&](int64_t row, int d, const float (&v)[4], float mx, float sum) {
+    if (single) {
+      const float inv = sum > 0.f || sum != sum ? 1.f / (sum + a.denom_eps) : 0.f;
+      if constexpr (kF32) {
+        *reinterpret_cast<float4*>(out + row * D + d) =
+            make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+      } else {
+        *reinterpret_cast<uint2*>(out + row * D + d) =
+            make_uint2(pack2_hw<T>(v[0] * inv, v[1] * inv), pack2_hw<T>(v[2] * inv, v[3] * inv));
+      }
+    } else {
+      const int64_t at = row * a.max_chunks + chunk;
+      *reinterpret_cast<float4*>(a.part_out + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) *reinterpret_cast<float2*>(a.part_stat + 2 * at) = make_float2(mx, sum);
+    }
+  };
+  if (!a.split_keys) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      if (orow[q] < 0) continue;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const float v[4] = {o[q][dt][0] * fo[q], o[q][dt][1] * fo[q], o[q][dt][2] * fo[q],
+                            o[q][dt][3] * fo[q]};
+        store4(orow[q], 16 * dt + 4 * kg, v, mt[q], lsum[q]);
+      }
+    }
+    return;
+  }
+  // [wave][row][D] sums, then [wave][row][2] maxima and sums
+  const int nr = a.lds_rows;
+  float* s_stat = s_join + kScaledWaves * nr * D;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int r = 16 * q + c16;
+    if (r >= nr) continue;
+    float* dst = s_join + (wave * nr + r) * D + 4 * kg;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<float4*>(dst + 16 * dt) =
+          make_float4(o[q][dt][0] * fo[q], o[q][dt][1] * fo[q], o[q][dt][2] * fo[q],
+                      o[q][dt][3] * fo[q]);
+    if (kg == 0) {
+      s_stat[2 * (wave * nr + r)] = mt[q];
+      s_stat[2 * (wave * nr + r) + 1] = lsum[q];
+    }
+  }
+  __syncthreads();
+  const int live = min(nr, rows - r0);
+  for (int e = threadIdx.x; e < live * (D / 4); e += 64 * kScaledWaves) {
+    const int r = e / (D / 4), d = 4 * (e % (D / 4));
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kScaledWaves; ++x) mx = fmaxf(mx, s_stat[2 * (x * nr + r)]);
+    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < kScaledWaves; ++x) {
+      const float mw = s_stat[2 * (x * nr + r)];
+      if (mw == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(mw - mx);
+      const float4 y = *reinterpret_cast<const float4*>(s_join + (x * nr + r) * D + d);
+      sum = fmaf(f, s_stat[2 * (x * nr + r) + 1], sum);
+      v[0] = fmaf(f, y.x, v[0]);
+      v[1] = fmaf(f, y.y, v[1]);
+      v[2] = fmaf(f, y.z, v[2]);
+      v[3] = fmaf(f, y.w, v[3]);
+    }
+    const int rr = r0 + r;
+    const int64_t row =
+        ((int64_t)qa + rr / a.group) * a.num_heads + (int64_t)j * a.group + rr % a.group;
+    store4(row, d, v, mx, sum);
+  }
+}
+
+// Joins the chunks of the rows whose context has more than one: a wave per row
+// (of a position, heads fastest).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledDev a, int32_t row_tiles) {
+  const int lane = threadIdx.x & 63;
+  const int s = (int)(blockIdx.x / (uint32_t)row_tiles);
+  const int r = (int)(blockIdx.x % (uint32_t)row_tiles) * 4 + (int)(threadIdx.x >> 6);
+  uint32_t qa = (uint32_t)s, qb = (uint32_t)s + 1u;
+  if (a.cu_seqlens_q != nullptr) {
+    qa = a.cu_seqlens_q[s];
+    qb = a.cu_seqlens_q[s + 1];
+  }
+  int n = qb > qa ? (int)min(qb - qa, (uint32_t)a.max_query_len) : 0;
+  n = (int64_t)qa >= a.total_rows ? 0 : (int)min((int64_t)n, a.total_rows - (int64_t)qa);
+  const int L = (int)min(a.context_lens[s], (uint32_t)a.max_ctx);
+  const int nchunks = (L + a.chunk_tokens - 1) / a.chunk_tokens;
+  if (nchunks <= 1 || r >= n * a.num_heads) return;
+  const int64_t row = (int64_t)qa * a.num_heads + r;
+  const float* stat = a.part_stat + row * a.max_chunks * 2;
+  float mx = -INFINITY;
+  for (int c = lane; c < nchunks; c += 64) mx = fmaxf(mx, stat[2 * c]);
+  mx = wave_max_dpp(mx);
+  float sum = 0.f;
+  constexpr int NV = (D + 63) / 64;
+  float v[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) v[k] = 0.f;
+  const float* part = a.part_out + row * a.max_chunks * D + lane;
+  for (int c = 0; c < nchunks; ++c) {
+    const float mc = stat[2 * c];
+    if (mc == -INFINITY) continue;  // (uniform)
+    const float f = __builtin_amdgcn_exp2f(mc - mx);
+    sum = fmaf(f, stat[2 * c + 1], sum);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (lane + 64 * k < D) v[k] = fmaf(f, part[(int64_t)c * D + 64 * k], v[k]);
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / (sum + a.denom_eps) : 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (lane + 64 * k < D)
+      store_from_f32<T>(static_cast<T*>(a.out) + row * D + lane + 64 * k, v[k] * inv);
+}
+
+template <typename T, int D, int BS, int NQ>
+hipError_t launch_scaled_t(const ScaledDev& d, int64_t grid, hipStream_t stream) {
+  const size_t lds = d.split_keys ? (size_t)kScaledWaves * d.lds_rows * (D + 2) * 4 : 0;
+  hipLaunchKernelGGL((scaled_attention_kernel<T, D, BS, NQ>), dim3((unsigned)grid),
+                     dim3(64 * kScaledWaves), lds, stream, d);
+  if (d.max_chunks > 1) {
+    const int tiles = (int)(((int64_t)d.max_query_len * d.num_heads + 3) / 4);
+    hipLaunchKernelGGL((scaled_merge_kernel<T, D>), dim3((unsigned)tiles * d.num_seqs), dim3(256),
+                       0, stream, d, tiles);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int D, int BS>
+hipError_t launch_scaled_q(const ScaledDev& d, int64_t grid, int nq, hipStream_t stream) {
+  if constexpr (scaled_two_tiles<T>(D))
+    if (nq == 2) return launch_scaled_t<T, D, BS, 2>(d, grid, stream);
+  return launch_scaled_t<T, D, BS, 1>(d, grid, stream);
+}
+
+template <typename T>
+hipError_t launch_scaled(const ScaledArgs& a, const CacheGeom& g, const ScaledPlan& p,
+                         hipStream_t stream) {
+  const int64_t rows = a.total_rows * a.num_heads;
+  float* part = static_cast<float*>(a.workspace);
+  const ScaledDev d{a.query,
+                    static_cast<const uint8_t*>(a.key_cache),
+                    static_cast<const uint8_t*>(a.value_cache),
+                    a.key_scales,
+                    a.value_scales,
+                    a.scale_block_stride,
+                    a.block_tables,
+                    a.cu_seqlens_q,
+                    a.context_lens,
+                    a.out,
+                    part,
+                    part == nullptr ? nullptr : part + rows * p.max_chunks * g.head_dim,
+                    g.block_stride,
+                    g.head_stride,
+                    g.num_blocks,
+                    a.total_rows,
+                    a.block_table_stride,
+                    a.num_seqs,
+                    a.max_query_len,
+                    a.max_ctx,
+                    a.num_heads,
+                    g.num_kv_heads,
+                    a.num_heads / g.num_kv_heads,
+                    a.causal,
+                    p.tiles,
+                    p.chunk_tokens,
+                    p.max_chunks,
+                    p.split_keys,
+                    p.lds_rows,
+                    a.scale * 1.4426950408889634f,
+                    a.denom_eps};
+#define VPA_SCALED(DV, BV)                           \
+  if (g.head_dim == DV && g.block_size == BV)        \
+    return launch_scaled_q<T, DV, BV>(d, p.grid, p.nq, stream);
+#define VPA_SCALED_D(DV) VPA_SCALED(DV, 8) VPA_SCALED(DV, 16) VPA_SCALED(DV, 32)
+  VPA_SCALED_D(64) VPA_SCALED_D(96) VPA_SCALED_D(128) VPA_SCALED_D(192) VPA_SCALED_D(256)
+#undef VPA_SCALED_D
+#undef VPA_SCALED
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+}  // namespace vpa

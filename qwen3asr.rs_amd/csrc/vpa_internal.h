@@ -399,6 +399,124 @@ constexpr int kVerifyMaxDrafts = 64;
 size_t verify_workspace_bytes(int32_t num_seqs, int32_t max_drafts, int32_t vocab);
 hipError_t launch_verify(int dtype, const VerifyArgs& a, hipStream_t stream);
 
+// Caches of E4M3 bytes with a scale per (block, kv head), f32 [num_blocks,
+// num_kv_heads], heads contiguous.
+
+// Append (scaled_cache_kernels.hip).
+struct ScaledAppendArgs {
+  const void* key;
+  const void* value;
+  int64_t key_token_stride, value_token_stride;  // elements
+  float* key_scales;
+  float* value_scales;
+  int64_t scale_block_stride;  // elements
+  void* key_cache;
+  void* value_cache;
+  const int64_t* slot_mapping;
+  int64_t num_tokens;
+};
+hipError_t launch_scaled_append(int dtype, const ScaledAppendArgs& a, const CacheGeom& g,
+                                hipStream_t stream);
+
+// Attention (scaled_attention.h and its instances per query type).
+struct ScaledArgs {
+  void* out;
+  const void* query;
+  const float* key_scales;
+  const float* value_scales;
+  int64_t scale_block_stride;
+  const void* key_cache;
+  const void* value_cache;
+  const uint32_t* block_tables;
+  int32_t block_table_stride;
+  const uint32_t* cu_seqlens_q;  // null: one row per sequence
+  const uint32_t* context_lens;
+  int32_t num_seqs, max_query_len, max_ctx;
+  int64_t total_rows;
+  float scale, denom_eps;
+  int32_t causal, num_heads;
+  void* workspace;
+};
+struct ScaledPlan {
+  int32_t nq;  // 16-row tiles of a wave
+  int32_t split_keys, lds_rows;
+  int32_t tiles;  // row tiles of a (sequence, kv head)
+  int32_t chunk_tokens, max_chunks;
+  int64_t grid;  // workgroups
+  size_t workspace_bytes;
+};
+ScaledPlan scaled_plan(int dtype, int32_t num_seqs, int32_t max_query_len, int32_t max_ctx,
+                       int64_t total_rows, int32_t num_heads, int32_t num_kv_heads,
+                       int32_t head_dim);
+hipError_t launch_scaled_attention_bf16(const ScaledArgs& a, const CacheGeom& g,
+                                        const ScaledPlan& p, hipStream_t stream);
+hipError_t launch_scaled_attention_f16(const ScaledArgs& a, const CacheGeom& g,
+                                       const ScaledPlan& p, hipStream_t stream);
+hipError_t launch_scaled_attention_f32(const ScaledArgs& a, const CacheGeom& g,
+                                       const ScaledPlan& p, hipStream_t stream);
+
+// Pages (page_kernels.hip).
+constexpr int kCopyMaxBuffers = 96;  // of one launch
+struct CopyBuffers {
+  char* base[kCopyMaxBuffers];
+  int64_t stride[kCopyMaxBuffers];  // bytes between blocks
+  uint32_t bytes[kCopyMaxBuffers];  // of a block
+};
+// Device state of the block allocator (see vpa_allocate_rows).
+struct PageState {
+  uint32_t* block_tables;
+  int32_t cols;
+  uint32_t* row_blocks;
+  uint32_t* positions;
+  uint32_t* shared;  // [num_blocks]: rows that hold a block besides the first
+  int64_t num_blocks;
+  uint32_t* ring;
+  uint32_t* ring_state;
+  int32_t ring_cap;
+  int32_t block_size;
+  int32_t num_rows;
+};
+constexpr int kMaxForks = 1024;  // of one call
+hipError_t launch_copy_blocks(const CopyBuffers& b, int32_t num_buffers, const uint32_t* src,
+                              const uint32_t* dst, const uint32_t* num_pairs, int32_t max_pairs,
+                              int64_t num_blocks, hipStream_t stream);
+hipError_t launch_fork_rows(const PageState& s, const uint32_t* src_rows, const uint32_t* dst_rows,
+                            int32_t num_forks, uint8_t* ok, uint32_t* copy_src, uint32_t* copy_dst,
+                            uint32_t* copy_count, hipStream_t stream);
+hipError_t launch_release_shared(const PageState& s, const uint32_t* keep_blocks,
+                                 hipStream_t stream);
+hipError_t launch_unshare_rows(const PageState& s, uint8_t* ok, uint32_t* copy_src,
+                               uint32_t* copy_dst, uint32_t* copy_count, hipStream_t stream);
+size_t compact_workspace_bytes(int64_t num_blocks);
+hipError_t launch_compact(const PageState& s, uint32_t* copy_src, uint32_t* copy_dst,
+                          uint32_t* copy_count, void* workspace, hipStream_t stream);
+
+// Logits before a token is chosen (logits_kernels.hip).
+struct AdjustArgs {
+  void* logits;  // [num_seqs, rows_per_seq, vocab]
+  int64_t seq_stride, row_stride;
+  int32_t num_seqs, rows_per_seq, vocab;
+  const uint32_t* generated;  // [num_seqs, generated_stride]
+  int32_t generated_stride;
+  const uint32_t* gen_len;
+  const uint32_t* prompt;  // or null
+  int32_t prompt_stride;
+  const uint32_t* prompt_len;
+  const uint32_t* draft_ids;  // [num_seqs, rows_per_seq - 1] or null
+  const float* repetition;    // [num_seqs] each, or null
+  const float* presence;
+  const float* frequency;
+  const uint32_t* bias_ids;  // [num_seqs, bias_stride] or null
+  const float* bias;
+  int32_t bias_stride;
+  const uint32_t* bias_len;  // or null: bias_stride each
+  const uint32_t* allowed;   // [num_masks, allowed_stride] or null
+  int32_t num_masks, allowed_stride;
+  const uint32_t* allowed_rows;  // [num_seqs, rows_per_seq] or null: row i has mask i
+};
+constexpr int kAdjustMaxBias = 1024;
+hipError_t launch_adjust_logits(int dtype, const AdjustArgs& a, hipStream_t stream);
+
 // True when the MFMA prefill kernel is compiled for this combination.
 bool prefill_supported(int dtype, int cache_dtype, int head_dim, int block_size, int group);
 

@@ -94,6 +94,27 @@ SIGNATURES = {
     "vpa_verify_draft_tokens": (ctypes.c_int, [
         _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p,
         _sz, _p]),
+    "vpa_reshape_and_cache_block_scaled": (ctypes.c_int, [
+        _p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _i64, _i64, _i64,
+        _i32, _p]),
+    "vpa_paged_attention_block_scaled_workspace_size": (_sz, [_i32, _i32, _i32, _i64, _i32, _i32,
+                                                              _i32, _i32]),
+    "vpa_paged_attention_block_scaled": (ctypes.c_int, [
+        _p, _p, _p, _p, _i64, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i64, _f32, _f32, _i32,
+        _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _p, _sz, _p]),
+    "vpa_copy_blocks": (ctypes.c_int, [_p, _p, _p, _i32, _p, _p, _p, _i32, _i64, _p]),
+    "vpa_fork_rows": (ctypes.c_int, [_p, _i32, _p, _p, _p, _i64, _p, _p, _i32, _p, _p, _p, _p, _p,
+                                     _p, _i32, _i32, _i32, _p]),
+    "vpa_release_shared_blocks": (ctypes.c_int, [_p, _i32, _p, _p, _i64, _p, _p, _p, _i32, _i32,
+                                                 _p]),
+    "vpa_unshare_rows": (ctypes.c_int, [_p, _i32, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i32,
+                                        _i32, _i32, _p]),
+    "vpa_compact_blocks_workspace_size": (_sz, [_i64]),
+    "vpa_compact_blocks": (ctypes.c_int, [_p, _i32, _p, _p, _i64, _p, _p, _p, _p, _p, _i32, _i32,
+                                          _p, _sz, _p]),
+    "vpa_adjust_logits": (ctypes.c_int, [
+        _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _i32, _p, _p, _i32, _p, _p, _p, _p, _p, _p,
+        _p, _i32, _p, _p, _i32, _i32, _p, _p]),
     # include/vpa_host.h
     "vpa_bytes_per_paged_block": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _p]),
     "vpa_pool_blocks_for_context": (ctypes.c_int, [_i64, _i32, _p]),

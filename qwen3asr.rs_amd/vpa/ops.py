@@ -21,7 +21,7 @@ launch, as the reference returns ``Err(candle_core::Error::Msg)``.
 from __future__ import annotations
 
 import contextlib
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -462,6 +462,21 @@ class DecodeTokenState:
         """next_ids <- argmax of the step's logits rows (all rows of the batch)."""
         argmax_token_ids_from_logits(logits, out=self.next_ids)
 
+    def adjust(self, logits: torch.Tensor, **rules) -> torch.Tensor:
+        """``adjust_logits`` of the step's logits, in place, with the rows' generated
+        tokens; ``rules`` are its other arguments. Before ``select``."""
+        from .logits import adjust_logits
+
+        return adjust_logits(logits, self.generated[:, :self.capacity], self.gen_len, **rules)
+
+    def fork(self, src_rows: torch.Tensor, dst_rows: torch.Tensor, ok: torch.Tensor) -> None:
+        """Rows dst_rows[f] go on from the state of rows src_rows[f] where ok[f] is set
+        (the arguments and the result of ``DeviceBlockAllocator.fork``)."""
+        take = _fork_map(self.batch, src_rows, dst_rows, ok)
+        for t in (self.next_ids, self.finished, self.generated, self.gen_len, self.input_ids):
+            bits = t.view(torch.int32) if t.dtype == torch.uint32 else t
+            bits.copy_(bits[take])
+
     def consume(self, prev_slot_mapping: Optional[torch.Tensor] = None) -> None:
         """Step start (paged_batch_engine.rs:640-667): pending EOS ids finish
         their rows, other pending ids are appended and become input_ids;
@@ -479,13 +494,27 @@ class DecodeTokenState:
             self.active_count.data_ptr(), self.batch, _stream(self.next_ids)))
 
 
+def _fork_map(batch: int, src_rows: torch.Tensor, dst_rows: torch.Tensor,
+              ok: torch.Tensor) -> torch.Tensor:
+    """The row that each row of the batch goes on from, i64 [batch]."""
+    take = torch.arange(batch + 1, device=ok.device)  # (the last for forks that are not)
+    good = ok != 0
+    src = torch.where(good, src_rows.view(torch.int32).long(), batch)
+    take[torch.where(good, dst_rows.view(torch.int32).long(), batch)] = src
+    return take[:batch]
+
+
 class DeviceBlockAllocator:
     """Device-resident KV block allocation and decode-step metadata for a
     fixed batch of rows (``vpa_allocate_rows`` / ``vpa_decode_step_metadata`` /
     ``vpa_release_blocks``): the PagedBlockManager of
     paged_cache_runtime.rs:217-380 (FIFO free list of ids 1..num_blocks-1)
     and decode_metadata_for_batch_step of paged_kv_cache.rs:924-1059, with
-    every buffer on the device so a captured decode graph can run them."""
+    every buffer on the device so a captured decode graph can run them.
+
+    Rows may share blocks once ``fork`` has been called (or ``enable_sharing``, which
+    has to come before a graph with ``release`` or ``trim`` in it is captured):
+    ``shared`` then counts the rows that hold each block besides the first."""
 
     def __init__(self, num_blocks: int, block_size: int, batch: int, cols: int, device):
         import numpy as np
@@ -505,6 +534,7 @@ class DeviceBlockAllocator:
         self.context_lens = torch.ones(batch, dtype=torch.uint32, device=device)
         self.status = torch.zeros(3, dtype=torch.uint32, device=device)
         self.ok = torch.zeros(batch, dtype=torch.uint8, device=device)
+        self.shared: Optional[torch.Tensor] = None
 
     def _common(self):
         return (self.free_ring.data_ptr(), self.free_ring_state.data_ptr(), self.ring_capacity)
@@ -528,15 +558,108 @@ class DeviceBlockAllocator:
             self.batch, _stream(self.block_tables)))
         return self.slot_mapping, self.context_lens
 
-    def trim(self, num_tokens: torch.Tensor,
-             slot_mapping: Optional[torch.Tensor] = None) -> None:
+    def enable_sharing(self) -> None:
+        """From here on blocks may have several holders (``fork``)."""
+        if self.shared is None:
+            if self.block_tables.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise _err("sharing has to be enabled before the graph is captured")
+            self.shared = torch.zeros(self.ring_capacity, dtype=torch.int32,
+                                      device=self.block_tables.device).view(torch.uint32)
+
+    def fork(self, src_rows: torch.Tensor, dst_rows: torch.Tensor,
+             buffers: Sequence[torch.Tensor]) -> torch.Tensor:
+        """Row dst_rows[f], which holds no blocks, becomes a copy of row src_rows[f] (u32
+        [F], F <= 1024): the blocks that are full are shared, a partly filled one is
+        copied in every one of ``buffers`` (the caches, and scales, of all layers;
+        ``copy_blocks``). Returns ok u8 [F]: 0 where dst_rows[f] held blocks or an earlier
+        fork's, or where no block was left."""
+        from .pages import copy_blocks
+
+        _require_device(src_rows, dst_rows, self.block_tables, *buffers)
+        if src_rows.dtype != torch.uint32 or src_rows.dim() != 1 or \
+                dst_rows.dtype != torch.uint32 or dst_rows.shape != src_rows.shape:
+            raise _err(f"src_rows and dst_rows must be u32 1-d of equal length, got "
+                       f"{src_rows.dtype} {tuple(src_rows.shape)} and {dst_rows.dtype} "
+                       f"{tuple(dst_rows.shape)}")
+        self._check_buffers(buffers)
+        self.enable_sharing()
+        n = src_rows.numel()
+        src_rows, dst_rows = src_rows.contiguous(), dst_rows.contiguous()
+        ok = self.ok.new_empty((n,))
+        src, dst, count = (self.row_blocks.new_empty((m,)) for m in (n, n, 1))
+        ring, state, cap = self._common()
+        with _on_device_of(self.block_tables):
+            check(_lib.load().vpa_fork_rows(
+                self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
+                self.positions.data_ptr(), self.shared.data_ptr(), self.ring_capacity,
+                src_rows.data_ptr(), dst_rows.data_ptr(), n, ok.data_ptr(), src.data_ptr(),
+                dst.data_ptr(), count.data_ptr(), ring, state, cap, self.block_size, self.batch,
+                _stream(self.block_tables)))
+        copy_blocks(buffers, src, dst, count)
+        return ok
+
+    def compact(self, buffers: Sequence[torch.Tensor]
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Brings the n blocks in use to ids 1 .. n: moves them in every one of
+        ``buffers`` (the caches, and scales, of all layers) and rewrites the tables and
+        the ring. Returns (old ids, new ids, count): the first count[0] are the moves,
+        for whoever keeps ids of its own."""
+        from .pages import copy_blocks
+
+        _require_device(self.block_tables, *buffers)
+        self._check_buffers(buffers)
+        n = self.ring_capacity
+        src, dst, count = (self.row_blocks.new_empty((m,)) for m in (n, n, 1))
+        ring, state, cap = self._common()
+        lib = _lib.load()
+        nbytes = lib.vpa_compact_blocks_workspace_size(n)
+        workspace = self.row_blocks.new_empty(((nbytes + 3) // 4,))
+        with _on_device_of(self.block_tables):
+            check(lib.vpa_compact_blocks(
+                self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
+                _ptr(self.shared), n, src.data_ptr(), dst.data_ptr(), count.data_ptr(), ring,
+                state, cap, self.batch, workspace.data_ptr(), nbytes,
+                _stream(self.block_tables)))
+        copy_blocks(buffers, src, dst, count)
+        return src, dst, count
+
+    def _check_buffers(self, buffers: Sequence[torch.Tensor]) -> None:
+        for t in buffers:
+            if t.dim() < 1 or t.shape[0] != self.ring_capacity:
+                raise _err(f"buffers must be pools of {self.ring_capacity} blocks, got "
+                           f"{tuple(t.shape)}")
+
+    def _unshare(self, buffers: Sequence[torch.Tensor]) -> None:
+        from .pages import copy_blocks
+
+        src, dst, count = (self.row_blocks.new_empty((m,)) for m in (self.batch, self.batch, 1))
+        ring, state, cap = self._common()
+        with _on_device_of(self.block_tables):
+            check(_lib.load().vpa_unshare_rows(
+                self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
+                self.positions.data_ptr(), self.shared.data_ptr(), self.ring_capacity,
+                self.ok.data_ptr(), src.data_ptr(), dst.data_ptr(), count.data_ptr(), ring, state,
+                cap, self.block_size, self.batch, _stream(self.block_tables)))
+        copy_blocks(buffers, src, dst, count)
+
+    def trim(self, num_tokens: torch.Tensor, slot_mapping: Optional[torch.Tensor] = None,
+             buffers: Optional[Sequence[torch.Tensor]] = None) -> None:
         """Rows hold num_tokens[r] tokens from here on (u32 [batch], at most what
         they held): the next step appends there, and the blocks past them go
         back (trim_request_to_num_tokens, paged_cache_runtime.rs:320-340). For rows
         whose drafted tokens were rejected or whose cache was cut. With the
         ``slot_mapping`` of the step before (i64 [batch]), a row that did not run in
         it (negative slot: finished, or stalled for lack of a block; its context_lens
-        is 1 whatever it holds) keeps all it holds."""
+        is 1 whatever it holds) keeps all it holds.
+
+        Where rows share blocks, ``buffers`` (the caches, and scales, of all layers) are
+        needed: a row cut back to inside a block that others hold takes a copy of it.
+        ``ok`` is then 0 for a row that found no block for one, which must not go on."""
+        if self.shared is not None:
+            if buffers is None:
+                raise _err("rows may share blocks: trim needs the buffers to copy them in")
+            self._check_buffers(buffers)
+            _require_device(self.block_tables, *buffers)
         if num_tokens.dtype != torch.uint32 or num_tokens.shape != (self.batch,):
             raise _err(f"num_tokens must be u32 [{self.batch}], got {num_tokens.dtype} "
                        f"{tuple(num_tokens.shape)}")
@@ -555,10 +678,21 @@ class DeviceBlockAllocator:
             keep = torch.where(ran, keep, self.cols)  # (no row has more blocks)
         self.positions.view(torch.int32).copy_(tokens)
         self.release(keep.to(torch.int32).view(torch.uint32))
+        if self.shared is not None:
+            self._unshare(buffers)
 
     def release(self, keep_blocks: torch.Tensor) -> None:
-        """Rows keep their first keep_blocks[r] blocks (u32 [batch]), the rest go back."""
+        """Rows keep their first keep_blocks[r] blocks (u32 [batch]), the rest go back
+        (a block that other rows hold: with its last holder)."""
         ring, state, cap = self._common()
+        if self.shared is not None:
+            with _on_device_of(self.block_tables):
+                check(_lib.load().vpa_release_shared_blocks(
+                    self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
+                    self.shared.data_ptr(), self.ring_capacity,
+                    keep_blocks.contiguous().data_ptr(), ring, state, cap, self.batch,
+                    _stream(self.block_tables)))
+            return
         check(_lib.load().vpa_release_blocks(
             self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
             keep_blocks.contiguous().data_ptr(), ring, state, cap, self.batch,

@@ -19,7 +19,9 @@ once as a HIP graph and replayed:
     begin()                    consume the pending ids, grow blocks, build
                                slot_mapping / context_lens, plan the work list
     layer(q, k, v, kc, vc, out) append the step's K/V rows, attend (per layer)
-    end(logits)                next ids = argmax of the step's logits
+    end(logits, **rules)       next ids = argmax of the step's logits, after the
+                               penalties, biases and masks of adjust_logits
+    fork(src, dst, buffers)    between steps: rows go on as several, sharing blocks
 
 Every layer shares the allocator's block tables (one block manager for the
 model, each layer its own cache tensors), as the reference does. Rows that
@@ -37,7 +39,7 @@ from typing import Sequence
 
 import torch
 
-from . import ops
+from . import block_scaled, ops
 
 
 class DeviceDecodeStep:
@@ -53,6 +55,7 @@ class DeviceDecodeStep:
         self.workspace = ops.paged_attention_workspace(batch, num_heads, head_dim,
                                                        self.max_context_len, device)
         self.scale = head_dim ** -0.5
+        self._workspaces = {}
 
     def admit(self, prompt_lens: torch.Tensor) -> torch.Tensor:
         """Rows hold prompt_lens[r] tokens already written to the caches (u32
@@ -81,7 +84,17 @@ class DeviceDecodeStep:
     def layer(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor,
               value_cache: torch.Tensor, out: torch.Tensor, k_scale=None, v_scale=None) -> None:
         """One layer's attention of the step: append the new K/V rows at the
-        step's slots, then attend over the shared block tables."""
+        step's slots, then attend over the shared block tables. Scales of shape
+        [num_blocks, kv_heads] are those of a block-scaled cache, which are set by
+        the append; one-element scales those of an fp8 cache."""
+        if k_scale is not None and k_scale.dim() == 2:
+            block_scaled.reshape_and_cache_block_scaled(k, v, k_scale, v_scale, key_cache,
+                                                        value_cache, self.allocator.slot_mapping)
+            block_scaled.paged_attention_block_scaled(
+                q, k_scale, v_scale, key_cache, value_cache, self.allocator.block_tables,
+                self.allocator.context_lens, self.scale, max_context_len=self.max_context_len,
+                out=out, workspace=self._scaled_workspace(q, key_cache))
+            return
         ops.reshape_and_cache(k, v, k_scale, v_scale, key_cache, value_cache,
                               self.allocator.slot_mapping)
         ops.paged_attention(q, k_scale, v_scale, key_cache, value_cache,
@@ -89,6 +102,31 @@ class DeviceDecodeStep:
                             self.max_context_len, self.scale, 1.0, None, out=out,
                             workspace=self.workspace, planned=True)
 
-    def end(self, logits: torch.Tensor) -> None:
-        """After the forward: next ids = argmax of the step's logits rows."""
+    def _scaled_workspace(self, q: torch.Tensor, key_cache: torch.Tensor):
+        key = (q.dtype, key_cache.shape[1])
+        if key not in self._workspaces:
+            self._workspaces[key] = block_scaled.paged_attention_block_scaled_workspace(
+                self.batch, self.num_heads, key_cache.shape[1], self.head_dim,
+                self.max_context_len, q.dtype, q.device)
+        return self._workspaces[key]
+
+    def end(self, logits: torch.Tensor, **rules) -> None:
+        """After the forward: next ids = argmax of the step's logits rows [batch, V];
+        with ``rules`` (the keyword arguments of ``adjust_logits``) after their
+        adjustment, in place, by them and the rows' generated tokens."""
+        if rules:
+            self.tokens.adjust(logits, **rules)
         self.tokens.select(logits)
+
+    def fork(self, src_rows: torch.Tensor, dst_rows: torch.Tensor,
+             buffers: Sequence[torch.Tensor]) -> torch.Tensor:
+        """Between two steps: rows dst_rows[f], which hold no blocks, go on from what rows
+        src_rows[f] hold and have generated (``DeviceBlockAllocator.fork``, over the
+        caches and scales of all layers). Returns ok u8; a row that is not ok is left as
+        it was."""
+        ok = self.allocator.fork(src_rows, dst_rows, buffers)
+        self.tokens.fork(src_rows, dst_rows, ok)
+        take = ops._fork_map(self.batch, src_rows, dst_rows, ok)
+        slots = self.allocator.slot_mapping
+        slots.copy_(slots[take])  # (whether the row ran in the step before)
+        return ok
