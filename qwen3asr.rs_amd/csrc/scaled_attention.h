@@ -6,10 +6,14 @@
 // For query row r, its sequence's cached tokens t and their block b(t):
 //   s_t = softmax_scale * ks[b(t)] * (q_r . K_t)       K_t, V_t: the bytes' values
 //   out = sum_t p_t vs[b(t)] V_t / (sum_t p_t + eps),  p_t = exp(s_t - max_t s_t)
-// over the tokens the row sees. The scales are applied where they are cheap and
-// exact enough: ks to the f32 scores, vs to the f32 probabilities, so the bytes
-// themselves go through the matrix instructions unscaled (every E4M3 value is
-// exact in f16 and in bf16) and scales of any size neither overflow nor round.
+// over the tokens the row sees. Scales that are powers of two, as the append
+// makes them, cost nothing: the conversion of the bytes for the matrix
+// instructions takes a power of two along, here a block's scale over the largest
+// of the step's (K) or of those met so far (V: `vref`), so that no operand passes
+// 448; that largest one is part of the softmax scale and of the output. Every
+// product is exact as long as the ratio is at least 2^-5 (E4M3's least number,
+// 2^-9, stays normal in f16). Steps with smaller ratios or other scales multiply
+// the f32 scores and probabilities instead.
 //
 // Work of a wave: 16 NQ rows (a row is a position and a query head of the kv
 // head; heads fastest, so any group size fills the rows) over 64 keys at a time
@@ -30,9 +34,8 @@
 // values (22 bits), and three bf16 values for Q, which hold an f32 exactly. The
 // probabilities stay below 2^kSlack (the reference maximum moves only when it is
 // exceeded by more) and are scaled by 2^kProbLog2, which keeps f16's smallest
-// step at 2^-31 of a probability of 1. vs enters as its ratio to the largest one
-// met so far (`vref`), so that the ratio is at most 1; like the maximum, vref
-// moving rescales the sums.
+// step at 2^-31 of a probability of 1. Like the maximum, vref moving rescales the
+// sums.
 //
 // Few rows (decode): the waves of a workgroup split a chunk's keys, 64 at a time,
 // and are joined in LDS; long contexts are split in chunks over workgroups and
@@ -63,6 +66,24 @@ __device__ __forceinline__ f32x4_t mfma16x16x32(const uint4& a, const uint4& b, 
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sa_bf16x8, a),
                                                    __builtin_bit_cast(sa_bf16x8, b), c, 0, 0, 0);
+}
+
+// Sixteen E4M3 bytes times a power of two (f32; the two halves' own) -> sixteen
+// values of K in two operands.
+template <typename K>
+__device__ __forceinline__ void fp8x16_times(const uint4& v, float slo, float shi, uint4& lo,
+                                             uint4& hi) {
+  auto cvt = [](uint32_t w, float s, auto half) -> uint32_t {
+    constexpr bool h = decltype(half)::value;
+    if constexpr (std::is_same_v<K, f16_t>)
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, h));
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, h));
+  };
+  constexpr std::false_type l{};
+  constexpr std::true_type h{};
+  lo = make_uint4(cvt(v.x, slo, l), cvt(v.x, slo, h), cvt(v.y, slo, l), cvt(v.y, slo, h));
+  hi = make_uint4(cvt(v.z, shi, l), cvt(v.z, shi, h), cvt(v.w, shi, l), cvt(v.w, shi, h));
 }
 
 constexpr int kScaledWaves = 4;
@@ -203,7 +224,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 #pragma unroll
     for (int st = 0; st < 2 * NC; ++st) {
       const int dim = 16 * (kg + 4 * (st / 2)) + 8 * (st % 2);
-      const bool in = dim < D;  // (head dims 96 and 192... end inside a step: zeros)
+      const bool in = dim < D;  // (head dim 96 ends inside a step: zeros)
       if constexpr (kF32) {
         uint32_t part[3][4];
 #pragma unroll
@@ -240,7 +261,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[q][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  float vref = 1.50463277e-36f;  // 2^-119: 2^kScaledProbLog2 / vref is finite
+  float vref = 1.50463277e-36f;  // 2^-119 (vref over 2^kScaledProbLog2 is a normal number)
 
   if (k_first < k_end) {
     const uint32_t* bt = a.block_tables + (int64_t)s * a.block_table_stride;
@@ -259,16 +280,17 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
       for (int i = 0; i < NI; ++i) r.id[i] = bt[min((k0 + 16 * kg + 8 * i) / BS, last_blk)];
       return r;
     };
-    // Scales of that tile; 0 for what is past the context or absent.
+    // Scales of that tile; 0 for an absent block's.
     struct Scales {
       float k[NI], v[NI];
     };
-    auto present = [&](uint32_t id) { return (int64_t)id < a.num_blocks; };
-    auto load_scales = [&](const Ids& d, int k0) {
+    const uint32_t max_id = (uint32_t)min(a.num_blocks - 1, (int64_t)0xffffffff);
+    auto present = [&](uint32_t id) { return id <= max_id; };
+    auto load_scales = [&](const Ids& d) {
       Scales r;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const bool ok = present(d.id[i]) && k0 + 16 * kg + 8 * i < L;
+        const bool ok = present(d.id[i]);
         const int64_t at = (int64_t)(ok ? d.id[i] : 0u) * a.scale_block_stride + j;
         const float ks = a.key_scales[at], vs = a.value_scales[at];
         r.k[i] = ok ? ks : 0.f;
@@ -342,13 +364,37 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 
     uint4 kraw[4][NC], vraw[DT];
     Ids ids = load_ids(k_first), ids1 = load_ids(k_first + k_step);
-    Scales sc = load_scales(ids, k_first);
+    Scales sc = load_scales(ids);
     load_k(ids, kraw);
 
     for (int k0 = k_first; k0 < k_end; k0 += k_step) {
       if constexpr (kEarly) load_v(ids, vraw);
       const Ids ids2 = load_ids(k0 + 2 * k_step);
-      const Scales sc1 = load_scales(ids1, k0 + k_step);
+      const Scales sc1 = load_scales(ids1);
+
+      // ---- scales ----
+      float kref = sc.k[0], vmax = fabsf(sc.v[0]);
+      if constexpr (NI == 2) {
+        kref = fmaxf(kref, sc.k[1]);
+        vmax = fmaxf(vmax, fabsf(sc.v[1]));
+      }
+      kref = max_rows(kref);
+      vmax = max_rows(vmax);
+      // x over a power of two `ref`; both are powers of two, x >= 2^-5 ref
+      auto ratio = [](float x, float ref) {
+        return __uint_as_float(__float_as_uint(x) - __float_as_uint(ref) + 0x3f800000u);
+      };
+      auto plain = [](float x, float ref) {
+        return ((__float_as_uint(x) | __float_as_uint(ref)) & 0x7fffffu) == 0 && x >= ref * 0.03125f;
+      };
+      float fs = kref * a.scale_log2;
+      bool odd = !plain(sc.k[0], kref);
+      if constexpr (NI == 2) odd = odd || !plain(sc.k[1], kref);
+      const bool kfast = __ballot(odd) == 0 && fs > 0.f;  // (uniform)
+      if (!kfast) fs = 1.f;
+      float kr[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) kr[i] = kfast ? ratio(sc.k[i], kref) : 1.f;
 
       // ---- S^T, tile by tile ----
       f32x4_t sv[NQ][4];
@@ -358,10 +404,12 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) sv[q][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        float krb = readlane_f(kr[0], 16 * b);
+        if constexpr (NI == 2) krb = c16 < 8 ? krb : readlane_f(kr[1], 16 * b);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
           uint4 op[2];
-          fp8x16_to_pk<K>(kraw[b][i], op[0], op[1]);
+          fp8x16_times<K>(kraw[b][i], krb, krb, op[0], op[1]);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -378,44 +426,40 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         load_v(ids, vraw);
       }
 
-      // ---- scales and masks ----
-      // tile b's scales and presence (8-token blocks: of this lane's half of it)
-      float vsb[4];
-      bool here[4];
+      // ---- other scales, masks ----
+      if (!kfast) {
+        asm volatile("" ::: "memory");  // (a branch, not selects)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float ksb = readlane_f(sc.k[0], 16 * b);
-        vsb[b] = readlane_f(sc.v[0], 16 * b);
-        here[b] = present((uint32_t)__builtin_amdgcn_readlane((int)ids.id[0], 16 * b));
-        if constexpr (NI == 2) {
-          const float k1 = readlane_f(sc.k[1], 16 * b), v1 = readlane_f(sc.v[1], 16 * b);
-          const bool h1 = present((uint32_t)__builtin_amdgcn_readlane((int)ids.id[1], 16 * b));
-          ksb = kg < 2 ? ksb : k1;
-          vsb[b] = kg < 2 ? vsb[b] : v1;
-          here[b] = kg < 2 ? here[b] : h1;
+        for (int b = 0; b < 4; ++b) {
+          float ksb = readlane_f(sc.k[0], 16 * b);
+          if constexpr (NI == 2) ksb = kg < 2 ? ksb : readlane_f(sc.k[1], 16 * b);
+          ksb *= a.scale_log2;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sv[q][b][r] *= ksb;
         }
-        const float f = ksb * a.scale_log2;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sv[q][b][r] *= f;
       }
       // every key inside the context, in a present block, seen by every row
       bool mine = present(ids.id[0]);
       if constexpr (NI == 2) mine = mine && present(ids.id[1]);
-      const bool all_here = __ballot(!mine) == 0 && k0 + kScaledKeys <= L;
-      const bool full = all_here && k0 + kScaledKeys - 1 <= all_see;
+      const bool full = __ballot(!mine) == 0 && k0 + kScaledKeys <= min(L, all_see + 1);
       if (!full) {
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int t = k0 + 16 * b + 4 * kg + r;
-            const bool in = here[b] && t < L;
-#pragma unroll
-            for (int q = 0; q < NQ; ++q)
-              sv[q][b][r] = in && t <= limit[q] ? sv[q][b][r] : -INFINITY;
+        for (int b = 0; b < 4; ++b) {
+          bool here = present((uint32_t)__builtin_amdgcn_readlane((int)ids.id[0], 16 * b));
+          if constexpr (NI == 2) {
+            const bool h1 = present((uint32_t)__builtin_amdgcn_readlane((int)ids.id[1], 16 * b));
+            here = kg < 2 ? here : h1;
           }
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            const int last = here ? limit[q] - (k0 + 16 * b + 4 * kg) : -1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sv[q][b][r] = r <= last ? sv[q][b][r] : -INFINITY;
+          }
+        }
       }
 
       // ---- online softmax ----
@@ -428,13 +472,10 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         for (int b = 0; b < 4; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx[q] = fmaxf(mx[q], sv[q][b][r]);
-        mx[q] = max_rows(mx[q]);
+        mx[q] = max_rows(mx[q]) * fs;
         mt[q] = fmaxf(mt[q], mx[q]);
         move = move || mx[q] > m[q] + kScaledSlack || (m[q] == -INFINITY && mx[q] > -INFINITY);
       }
-      float vmax = fabsf(sc.v[0]);
-      if constexpr (NI == 2) vmax = fmaxf(vmax, fabsf(sc.v[1]));
-      vmax = max_rows(vmax);
       if (__ballot(move || vmax > vref) != 0) {
         const float vnew = fmaxf(vref, vmax);
         const float fv = vref / vnew;
@@ -451,23 +492,45 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
             for (int r = 0; r < 4; ++r) o[q][dt][r] *= f * fv;
         }
       }
-      const float ivref = (float)(1 << kScaledProbLog2) / vref;
+      odd = !plain(sc.v[0], vref);
+      if constexpr (NI == 2) odd = odd || !plain(sc.v[1], vref);
+      const bool vfast = __ballot(odd) == 0;
+      float vr[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) vr[i] = vfast ? ratio(sc.v[i], vref) : 1.f;
 
       // ---- probabilities, as operands of P.V ----
       uint32_t pw[NQ][PP][2][4];  // [two tokens of a tile's four][tile]
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        const float mu = m[q] == -INFINITY ? 0.f : m[q];
+        const float mu = (m[q] == -INFINITY ? 0.f : m[q]) - (float)kScaledProbLog2;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float f = vsb[b] * ivref;
-          float p[4];
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(sv[q][b][r] - mu);
-            lsum[q] += p[r];
-            p[r] *= f;
+            sv[q][b][r] = __builtin_amdgcn_exp2f(fmaf(sv[q][b][r], fs, -mu));
+            lsum[q] += sv[q][b][r];
           }
+      }
+      if (!vfast) {
+        float over = vref;
+        asm volatile("" : "+v"(over));  // (a branch, and nothing of it before)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          float f = readlane_f(sc.v[0], 16 * b);
+          if constexpr (NI == 2) f = kg < 2 ? f : readlane_f(sc.v[1], 16 * b);
+          f /= over;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sv[q][b][r] *= f;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const f32x4_t p = sv[q][b];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             pw[q][0][h][b] = pack2_hw<f16_t>(p[2 * h], p[2 * h + 1]);
@@ -519,7 +582,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         if constexpr (!kEarly)
           if (dt % 2 == 0) __builtin_amdgcn_sched_barrier(0);
         uint4 op[2];
-        fp8x16_to_pk<f16_t>(vraw[dt], op[0], op[1]);
+        fp8x16_times<f16_t>(vraw[dt], vr[0], vr[NI - 1], op[0], op[1]);
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -587,8 +650,9 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mt[q]);
-    lsum[q] = sum_rows(lsum[q]) * f;
-    fo[q] = f * (vref * (1.f / (1 << kScaledProbLog2)));
+    const float f1 = f * (1.f / (1 << kScaledProbLog2));
+    lsum[q] = sum_rows(lsum[q]) * f1;
+    fo[q] = f1 * vref;
   }
   const bool single = nchunks == 1;
   T* out = static_cast<T*>(a.out);

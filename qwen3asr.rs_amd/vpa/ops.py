@@ -573,20 +573,18 @@ class DeviceBlockAllocator:
         copied in every one of ``buffers`` (the caches, and scales, of all layers;
         ``copy_blocks``). Returns ok u8 [F]: 0 where dst_rows[f] held blocks or an earlier
         fork's, or where no block was left."""
-        from .pages import copy_blocks
-
-        _require_device(src_rows, dst_rows, self.block_tables, *buffers)
+        _require_device(src_rows, dst_rows, self.block_tables)
         if src_rows.dtype != torch.uint32 or src_rows.dim() != 1 or \
                 dst_rows.dtype != torch.uint32 or dst_rows.shape != src_rows.shape:
             raise _err(f"src_rows and dst_rows must be u32 1-d of equal length, got "
                        f"{src_rows.dtype} {tuple(src_rows.shape)} and {dst_rows.dtype} "
                        f"{tuple(dst_rows.shape)}")
-        self._check_buffers(buffers)
+        pools = self._pools(buffers)
         self.enable_sharing()
         n = src_rows.numel()
         src_rows, dst_rows = src_rows.contiguous(), dst_rows.contiguous()
         ok = self.ok.new_empty((n,))
-        src, dst, count = (self.row_blocks.new_empty((m,)) for m in (n, n, 1))
+        src, dst, count = self._pairs(n)
         ring, state, cap = self._common()
         with _on_device_of(self.block_tables):
             check(_lib.load().vpa_fork_rows(
@@ -595,7 +593,7 @@ class DeviceBlockAllocator:
                 src_rows.data_ptr(), dst_rows.data_ptr(), n, ok.data_ptr(), src.data_ptr(),
                 dst.data_ptr(), count.data_ptr(), ring, state, cap, self.block_size, self.batch,
                 _stream(self.block_tables)))
-        copy_blocks(buffers, src, dst, count)
+            pools.copy(src, dst, count)
         return ok
 
     def compact(self, buffers: Sequence[torch.Tensor]
@@ -604,12 +602,10 @@ class DeviceBlockAllocator:
         ``buffers`` (the caches, and scales, of all layers) and rewrites the tables and
         the ring. Returns (old ids, new ids, count): the first count[0] are the moves,
         for whoever keeps ids of its own."""
-        from .pages import copy_blocks
-
-        _require_device(self.block_tables, *buffers)
-        self._check_buffers(buffers)
+        _require_device(self.block_tables)
+        pools = self._pools(buffers)
         n = self.ring_capacity
-        src, dst, count = (self.row_blocks.new_empty((m,)) for m in (n, n, 1))
+        src, dst, count = self._pairs(n)
         ring, state, cap = self._common()
         lib = _lib.load()
         nbytes = lib.vpa_compact_blocks_workspace_size(n)
@@ -620,27 +616,17 @@ class DeviceBlockAllocator:
                 _ptr(self.shared), n, src.data_ptr(), dst.data_ptr(), count.data_ptr(), ring,
                 state, cap, self.batch, workspace.data_ptr(), nbytes,
                 _stream(self.block_tables)))
-        copy_blocks(buffers, src, dst, count)
+            pools.copy(src, dst, count)
         return src, dst, count
 
-    def _check_buffers(self, buffers: Sequence[torch.Tensor]) -> None:
-        for t in buffers:
-            if t.dim() < 1 or t.shape[0] != self.ring_capacity:
-                raise _err(f"buffers must be pools of {self.ring_capacity} blocks, got "
-                           f"{tuple(t.shape)}")
+    def _pools(self, buffers: Sequence[torch.Tensor]):
+        from .pages import _Pools
 
-    def _unshare(self, buffers: Sequence[torch.Tensor]) -> None:
-        from .pages import copy_blocks
+        return _Pools(buffers, self.ring_capacity, self.block_tables.get_device())
 
-        src, dst, count = (self.row_blocks.new_empty((m,)) for m in (self.batch, self.batch, 1))
-        ring, state, cap = self._common()
-        with _on_device_of(self.block_tables):
-            check(_lib.load().vpa_unshare_rows(
-                self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
-                self.positions.data_ptr(), self.shared.data_ptr(), self.ring_capacity,
-                self.ok.data_ptr(), src.data_ptr(), dst.data_ptr(), count.data_ptr(), ring, state,
-                cap, self.block_size, self.batch, _stream(self.block_tables)))
-        copy_blocks(buffers, src, dst, count)
+    def _pairs(self, n: int):
+        """Room for n pairs of copied blocks and their number."""
+        return tuple(self.row_blocks.new_empty((m,)) for m in (n, n, 1))
 
     def trim(self, num_tokens: torch.Tensor, slot_mapping: Optional[torch.Tensor] = None,
              buffers: Optional[Sequence[torch.Tensor]] = None) -> None:
@@ -658,8 +644,7 @@ class DeviceBlockAllocator:
         if self.shared is not None:
             if buffers is None:
                 raise _err("rows may share blocks: trim needs the buffers to copy them in")
-            self._check_buffers(buffers)
-            _require_device(self.block_tables, *buffers)
+            pools = self._pools(buffers)
         if num_tokens.dtype != torch.uint32 or num_tokens.shape != (self.batch,):
             raise _err(f"num_tokens must be u32 [{self.batch}], got {num_tokens.dtype} "
                        f"{tuple(num_tokens.shape)}")
@@ -679,7 +664,15 @@ class DeviceBlockAllocator:
         self.positions.view(torch.int32).copy_(tokens)
         self.release(keep.to(torch.int32).view(torch.uint32))
         if self.shared is not None:
-            self._unshare(buffers)
+            src, dst, count = self._pairs(self.batch)
+            ring, state, cap = self._common()
+            with _on_device_of(self.block_tables):
+                check(_lib.load().vpa_unshare_rows(
+                    self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
+                    self.positions.data_ptr(), self.shared.data_ptr(), self.ring_capacity,
+                    self.ok.data_ptr(), src.data_ptr(), dst.data_ptr(), count.data_ptr(), ring,
+                    state, cap, self.block_size, self.batch, _stream(self.block_tables)))
+                pools.copy(src, dst, count)
 
     def release(self, keep_blocks: torch.Tensor) -> None:
         """Rows keep their first keep_blocks[r] blocks (u32 [batch]), the rest go back

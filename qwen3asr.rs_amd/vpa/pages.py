@@ -3,7 +3,7 @@ blocks need them."""
 
 from __future__ import annotations
 
-import ctypes
+from array import array
 from typing import Optional, Sequence
 
 import torch
@@ -13,6 +13,47 @@ from ._lib import check
 from .ops import _err, _on_device_of, _ptr, _require_device, _stream
 
 
+class _Pools:
+    """Addresses, strides and sizes of the blocks of ``buffers``, checked, in the host
+    arrays that ``vpa_copy_blocks`` reads."""
+
+    def __init__(self, buffers: Sequence[torch.Tensor], blocks: int, device: int):
+        # (a hundred or more tensors per call: few calls for each)
+        base, size, stride = [], [], []
+        for t in buffers:
+            if t.get_device() != device:
+                _require_device(t)
+                raise _err(f"device mismatch: a buffer on {t.device}, ids on cuda:{device}")
+            if t.dim() < 1 or t.shape[0] != blocks:
+                raise _err(f"buffers must be pools of {blocks} blocks, got {tuple(t.shape)}")
+            if blocks and t.is_contiguous():
+                n = t.nbytes // blocks
+                stride.append(n)
+            elif blocks:
+                if not t[0].is_contiguous():
+                    raise _err(f"buffers must have contiguous blocks, got {tuple(t.shape)} of "
+                               f"strides {t.stride()}")
+                n = t.numel() // blocks * t.element_size()
+                stride.append(t.stride(0) * t.element_size() if blocks > 1 else n)
+            if blocks and n:
+                base.append(t.data_ptr())
+                size.append(n)
+            elif blocks:
+                stride.pop()
+        self.blocks, self.count = blocks, len(base)
+        self.base, self.stride, self.size = array("Q", base), array("q", stride), array("q", size)
+
+    def copy(self, src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
+             num_pairs: Optional[torch.Tensor]) -> None:
+        """The copies of contiguous u32 pairs, on the current device and stream."""
+        if self.count == 0:
+            return
+        check(_lib.load().vpa_copy_blocks(
+            self.base.buffer_info()[0], self.stride.buffer_info()[0], self.size.buffer_info()[0],
+            self.count, src_blocks.data_ptr(), dst_blocks.data_ptr(), _ptr(num_pairs),
+            src_blocks.numel(), self.blocks, _stream(src_blocks)))
+
+
 def copy_blocks(buffers: Sequence[torch.Tensor], src_blocks: torch.Tensor,
                 dst_blocks: torch.Tensor, num_pairs: Optional[torch.Tensor] = None) -> None:
     """Copies block src_blocks[p] to block dst_blocks[p] (u32 [P]) in each of ``buffers``,
@@ -20,7 +61,7 @@ def copy_blocks(buffers: Sequence[torch.Tensor], src_blocks: torch.Tensor,
     layer) and whose blocks are contiguous. ``num_pairs`` (u32 [1], on the device) tells
     how many of the pairs there are. The destinations are distinct and none of them is a
     source; ids past the pool copy nothing."""
-    _require_device(src_blocks, dst_blocks, num_pairs, *buffers)
+    _require_device(src_blocks, dst_blocks, num_pairs)
     if src_blocks.dtype != torch.uint32 or src_blocks.dim() != 1 or \
             dst_blocks.dtype != torch.uint32 or dst_blocks.shape != src_blocks.shape:
         raise _err(f"src_blocks and dst_blocks must be u32 1-d of equal length, got "
@@ -28,22 +69,12 @@ def copy_blocks(buffers: Sequence[torch.Tensor], src_blocks: torch.Tensor,
                    f"{tuple(dst_blocks.shape)}")
     if num_pairs is not None and (num_pairs.dtype != torch.uint32 or num_pairs.numel() != 1):
         raise _err(f"num_pairs must be u32 [1], got {num_pairs.dtype} {tuple(num_pairs.shape)}")
-    n = len(buffers)
-    if n == 0 or src_blocks.numel() == 0:
+    if len(buffers) == 0:
         return
-    blocks = buffers[0].shape[0] if buffers[0].dim() else -1
-    base, stride, size = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int64 * n)()
-    for k, t in enumerate(buffers):
-        if t.dim() < 1 or t.shape[0] != blocks or not (blocks == 0 or t[0].is_contiguous()):
-            raise _err(f"buffer {k} must be [{blocks}, ...] with contiguous blocks, got "
-                       f"{tuple(t.shape)} of strides {t.stride()}")
-        base[k], e = t.data_ptr(), t.element_size()
-        size[k] = t.numel() // max(blocks, 1) * e
-        stride[k] = t.stride(0) * e if blocks > 1 else size[k]
-    if blocks == 0 or all(b == 0 for b in size):
+    blocks = buffers[0].shape[0] if buffers[0].dim() else 0
+    pools = _Pools(buffers, blocks, src_blocks.get_device())
+    if src_blocks.numel() == 0:
         return
     src_blocks, dst_blocks = src_blocks.contiguous(), dst_blocks.contiguous()
     with _on_device_of(src_blocks):
-        check(_lib.load().vpa_copy_blocks(
-            base, stride, size, n, src_blocks.data_ptr(), dst_blocks.data_ptr(), _ptr(num_pairs),
-            src_blocks.numel(), blocks, _stream(src_blocks)))
+        pools.copy(src_blocks, dst_blocks, num_pairs)
