@@ -34,6 +34,18 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_tmp, uint
   return before + incl - v;
 }
 
+// Waits for this wave's memory operations, atomics among them (a barrier alone
+// does not); then the workgroup's, which all go to one L2, are done for each other.
+__device__ __forceinline__ void finish_and_sync() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// Place `at` + `more` of the ring (32-bit: the capacity is below 2^31).
+__device__ __forceinline__ uint32_t ring_at(const PageState& s, uint32_t at, uint32_t more) {
+  return (at % (uint32_t)s.ring_cap + more) % (uint32_t)s.ring_cap;
+}
+
 // (past the L1 cache, which other compute units' atomics do not update)
 __device__ __forceinline__ uint32_t load_fresh(const uint32_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -96,7 +108,7 @@ __global__ __launch_bounds__(kPageThreads) void fork_decide_kernel(
     uint32_t* __restrict__ copy_src, uint32_t* __restrict__ copy_dst,
     uint32_t* __restrict__ copy_count) {
   __shared__ uint32_t s_tmp[kPageThreads / 64];
-  __shared__ uint32_t s_dst[kMaxForks];
+  __shared__ __align__(16) uint32_t s_dst[kMaxForks];
   const int f = threadIdx.x;
   const uint32_t head = s.ring_state[0], avail = s.ring_state[1];
   uint32_t src = 0xffffffffu, dst = 0xffffffffu, tokens = 0, last = 0;
@@ -111,8 +123,17 @@ __global__ __launch_bounds__(kPageThreads) void fork_decide_kernel(
     const uint32_t have = min(s.row_blocks[src], (uint32_t)s.cols);
     tokens = (uint32_t)min((uint64_t)s.positions[src], (uint64_t)have * (uint32_t)s.block_size);
     can = s.row_blocks[dst] == 0;
-    for (int e = 0; can && e < f; ++e) can = s_dst[e] != dst;
   }
+  // an earlier fork of the same row? (four at a time, the reads not waiting on each other)
+  bool claimed = false;
+  const int before = min((int)(threadIdx.x | 63u), num_forks);
+#pragma unroll 4
+  for (int e = 0; e < before; e += 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(&s_dst[e]);
+    claimed = claimed || (v.x == dst && e < f) || (v.y == dst && e + 1 < f) ||
+              (v.z == dst && e + 2 < f) || (v.w == dst && e + 3 < f);
+  }
+  can = can && !claimed;
   const uint32_t full = tokens / (uint32_t)s.block_size;
   const bool part = can && tokens % (uint32_t)s.block_size != 0;
   if (part) last = s.block_tables[(int64_t)src * s.cols + full];
@@ -125,7 +146,7 @@ __global__ __launch_bounds__(kPageThreads) void fork_decide_kernel(
     s.positions[dst] = tokens;
     s.row_blocks[dst] = full + (part ? 1u : 0u);
     if (part) {
-      const uint32_t id = s.ring[(uint32_t)(((uint64_t)head + rank) % (uint32_t)s.ring_cap)];
+      const uint32_t id = s.ring[ring_at(s, head, rank)];
       s.block_tables[(int64_t)dst * s.cols + full] = id;
       copy_src[rank] = last;
       copy_dst[rank] = id;
@@ -134,7 +155,7 @@ __global__ __launch_bounds__(kPageThreads) void fork_decide_kernel(
   if (f == 0) {
     const uint32_t used = min(total, avail);
     *copy_count = used;
-    s.ring_state[0] = (uint32_t)(((uint64_t)head + used) % (uint32_t)s.ring_cap);
+    s.ring_state[0] = ring_at(s, head, used);
     s.ring_state[1] = avail - used;
   }
 }
@@ -169,61 +190,86 @@ __global__ __launch_bounds__(kPageThreads) void release_shared_kernel(
     const PageState s, const uint32_t* __restrict__ keep_blocks) {
   __shared__ uint32_t s_tmp[kPageThreads / 64];
   __shared__ uint32_t s_count[kPageThreads];
+  __shared__ uint32_t s_rows[kPageThreads], s_keep[kPageThreads], s_have[kPageThreads];
   constexpr int kWaves = kPageThreads / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t head = s.ring_state[0], count = s.ring_state[1];
-  auto code_of = [&](int r, uint32_t i) {
-    return 0xfffffffeu - ((uint32_t)r * (uint32_t)s.cols + ((uint32_t)s.cols - 1u - i));
+  auto code_of = [&](uint32_t r, uint32_t i) {
+    return 0xfffffffeu - (r * (uint32_t)s.cols + ((uint32_t)s.cols - 1u - i));
   };
-  auto held = [&](int r) { return min(s.row_blocks[r], (uint32_t)s.cols); };
-  auto kept = [&](int r) { return min(keep_blocks[r], held(r)); };
   auto counted = [&](uint32_t id) { return id != 0 && (int64_t)id < s.num_blocks; };
-  for (int r = wave; r < s.num_rows; r += kWaves) {
-    const uint32_t have = held(r);
-    for (uint32_t i = kept(r) + lane; i < have; i += 64) {
-      const uint32_t id = s.block_tables[(int64_t)r * s.cols + i];
+  auto entry = [&](uint32_t r, uint32_t i) { return s.block_tables[(int64_t)r * s.cols + i]; };
+  // The rows among base .. base + 1023 that give something back, in order; a wave
+  // takes each of them, a lane each of its entries. Every pass lists them again
+  // unless one list holds them all.
+  auto list_rows = [&](int base) -> int {
+    const int r = base + threadIdx.x;
+    uint32_t have = 0, keep = 0;
+    if (r < s.num_rows) {
+      have = min(s.row_blocks[r], (uint32_t)s.cols);
+      keep = min(keep_blocks[r], have);
+    }
+    uint32_t total;
+    const uint32_t rank = group_scan(keep < have ? 1u : 0u, s_tmp, &total);
+    if (keep < have) {
+      s_rows[rank] = (uint32_t)r;
+      s_keep[rank] = keep;
+      s_have[rank] = have;
+    }
+    __syncthreads();
+    return (int)total;
+  };
+  const bool one_list = s.num_rows <= kPageThreads;
+  int rows = 0;
+  auto pass = [&](auto&& body) {
+    for (int base = 0; base < s.num_rows; base += kPageThreads) {
+      if (!one_list) rows = list_rows(base);
+      for (int k = wave; k < rows; k += kWaves) body(s_rows[k], s_keep[k], s_have[k], k);
+      finish_and_sync();
+    }
+  };
+  if (one_list) rows = list_rows(0);
+  if (one_list && rows == 0) return;  // (uniform)
+  pass([&](uint32_t r, uint32_t keep, uint32_t have, int) {
+    for (uint32_t i = keep + lane; i < have; i += 64) {
+      const uint32_t id = entry(r, i);
       if (counted(id)) atomicSub(&s.shared[id], 1u);
     }
-  }
-  __threadfence();  // (a barrier alone does not wait for atomics in flight)
-  __syncthreads();
-  for (int r = wave; r < s.num_rows; r += kWaves) {
-    const uint32_t have = held(r);
-    for (uint32_t i = kept(r) + lane; i < have; i += 64) {
-      const uint32_t id = s.block_tables[(int64_t)r * s.cols + i];
+  });
+  pass([&](uint32_t r, uint32_t keep, uint32_t have, int) {
+    for (uint32_t i = keep + lane; i < have; i += 64) {
+      const uint32_t id = entry(r, i);
       if (counted(id) && load_fresh(&s.shared[id]) >= 0x80000000u)
         atomicMin(&s.shared[id], code_of(r, i));
     }
-  }
-  __threadfence();
-  __syncthreads();
+  });
   uint32_t added = 0;
   for (int base = 0; base < s.num_rows; base += kPageThreads) {
-    const int end = min(base + kPageThreads, s.num_rows);
-    auto gives = [&](int r, uint32_t i, uint32_t& id) {
-      id = s.block_tables[(int64_t)r * s.cols + i];
+    if (!one_list) rows = list_rows(base);
+    auto gives = [&](uint32_t r, uint32_t i, uint32_t& id) {
+      id = entry(r, i);
       return counted(id) && load_fresh(&s.shared[id]) == code_of(r, i);
     };
     s_count[threadIdx.x] = 0;
     __syncthreads();
-    for (int r = base + wave; r < end; r += kWaves) {
-      const uint32_t have = held(r), keep = kept(r);
+    for (int k = wave; k < rows; k += kWaves) {
+      const uint32_t r = s_rows[k], keep = s_keep[k], have = s_have[k];
       uint32_t n = 0, id;
       for (uint32_t at = keep; at < have; at += 64) {
         const bool mine = at + lane < have && gives(r, at + lane, id);
         n += (uint32_t)__builtin_popcountll(__ballot(mine));
       }
-      if (lane == 0) s_count[r - base] = n;
+      if (lane == 0) s_count[k] = n;
     }
     __syncthreads();
     uint32_t total;
     const uint32_t before = group_scan(s_count[threadIdx.x], s_tmp, &total);
     s_count[threadIdx.x] = before;
     __syncthreads();
-    for (int r = base + wave; r < end; r += kWaves) {
-      const uint32_t have = held(r), keep = kept(r);
-      if (keep >= have) continue;
-      uint64_t at_ring = (uint64_t)head + count + added + s_count[r - base];
+    for (int k = wave; k < rows; k += kWaves) {
+      const uint32_t r = s_rows[k], keep = s_keep[k], have = s_have[k];
+      uint32_t at_ring = (uint32_t)(((uint64_t)head + count + added + s_count[k]) %
+                                    (uint32_t)s.ring_cap);
       for (uint32_t upto = have; upto > keep; upto = upto >= keep + 64 ? upto - 64 : keep) {
         // lane 0 takes the last block
         uint32_t id = 0;
@@ -232,11 +278,11 @@ __global__ __launch_bounds__(kPageThreads) void release_shared_kernel(
         if (mine) {
           const uint32_t rank = __builtin_amdgcn_mbcnt_hi(
               (uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
-          s.ring[(at_ring + rank) % (uint32_t)s.ring_cap] = id;
+          s.ring[ring_at(s, at_ring, rank)] = id;
           // (no other entry of this block compares equal, before or after)
           __hip_atomic_store(&s.shared[id], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        at_ring += (uint32_t)__builtin_popcountll(mask);
+        at_ring = ring_at(s, at_ring, (uint32_t)__builtin_popcountll(mask));
       }
       if (lane == 0) s.row_blocks[r] = keep;
     }
@@ -325,22 +371,41 @@ __global__ __launch_bounds__(256) void compact_clear_kernel(CompactSpace c) {
 __global__ __launch_bounds__(256) void compact_mark_kernel(const PageState s, CompactSpace c) {
   const uint32_t head = s.ring_state[0], count = min(s.ring_state[1], (uint32_t)s.ring_cap);
   for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) {
-    const uint32_t id = s.ring[(uint32_t)(((uint64_t)head + i) % (uint32_t)s.ring_cap)];
+    const uint32_t id = s.ring[ring_at(s, head, i)];
     if (id != 0 && (int64_t)id < s.num_blocks) atomicOr(&c.free_bits[id / 32], 1u << (id % 32));
   }
 }
 
+// Pools of at most this many blocks have their free bits collected by the pairing
+// workgroup itself, in LDS: three launches become one (a few us each). A larger
+// pool's ring is read faster by many workgroups.
+constexpr int kCompactOneGroup = 65536;
+
 // The k-th block in use past the front takes the k-th free place in it; the front
 // is as long as there are blocks in use, so there are as many of the one as of the
 // other. One workgroup, a run of words per lane.
+template <bool kMark>
 __global__ __launch_bounds__(kPageThreads) void compact_pair_kernel(
     const PageState s, CompactSpace c, uint32_t* __restrict__ copy_src,
     uint32_t* __restrict__ copy_dst, uint32_t* __restrict__ copy_count) {
   __shared__ uint32_t s_tmp[kPageThreads / 64];
+  __shared__ uint32_t s_bits[kMark ? kCompactOneGroup / 32 : 1];
+  if constexpr (kMark) {
+    for (int i = threadIdx.x; i < c.words; i += kPageThreads) s_bits[i] = 0;
+    __syncthreads();
+    const uint32_t head = s.ring_state[0], count = min(s.ring_state[1], (uint32_t)s.ring_cap);
+    for (uint32_t i = threadIdx.x; i < count; i += kPageThreads) {
+      const uint32_t id = s.ring[ring_at(s, head, i)];
+      if (id != 0 && (int64_t)id < s.num_blocks) atomicOr(&s_bits[id / 32], 1u << (id % 32));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < c.words; i += kPageThreads) c.free_bits[i] = s_bits[i];
+  }
+  const uint32_t* bits = kMark ? s_bits : c.free_bits;
   const int per = (c.words + kPageThreads - 1) / kPageThreads;
   const int a = min(threadIdx.x * per, (unsigned)c.words), b = min(a + per, c.words);
   uint32_t n = 0;
-  for (int i = a; i < b; ++i) n += (uint32_t)__builtin_popcount(c.free_bits[i]);
+  for (int i = a; i < b; ++i) n += (uint32_t)__builtin_popcount(bits[i]);
   uint32_t free_blocks;
   group_scan(n, s_tmp, &free_blocks);
   const uint32_t nb = (uint32_t)s.num_blocks, front = nb - 1 - free_blocks;
@@ -349,8 +414,8 @@ __global__ __launch_bounds__(kPageThreads) void compact_pair_kernel(
     const int64_t left = (int64_t)id + 1 - 32 * (int64_t)i;
     return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
   };
-  auto holes_of = [&](int i) { return c.free_bits[i] & upto(front, i); };
-  auto moved_of = [&](int i) { return ~c.free_bits[i] & upto(nb - 1, i) & ~upto(front, i); };
+  auto holes_of = [&](int i) { return bits[i] & upto(front, i); };
+  auto moved_of = [&](int i) { return ~bits[i] & upto(nb - 1, i) & ~upto(front, i); };
   uint32_t holes = 0, moved = 0, total;
   for (int i = a; i < b; ++i) {
     holes += (uint32_t)__builtin_popcount(holes_of(i));
@@ -452,10 +517,16 @@ size_t compact_workspace_bytes(int64_t num_blocks) {
 hipError_t launch_compact(const PageState& s, uint32_t* copy_src, uint32_t* copy_dst,
                           uint32_t* copy_count, void* workspace, hipStream_t stream) {
   const CompactSpace c = compact_space(workspace, s.num_blocks);
-  hipLaunchKernelGGL(compact_clear_kernel, dim3(grid_of(c.words)), dim3(256), 0, stream, c);
-  hipLaunchKernelGGL(compact_mark_kernel, dim3(grid_of(s.num_blocks)), dim3(256), 0, stream, s, c);
-  hipLaunchKernelGGL(compact_pair_kernel, dim3(1), dim3(kPageThreads), 0, stream, s, c, copy_src,
-                     copy_dst, copy_count);
+  if (s.num_blocks <= kCompactOneGroup) {
+    hipLaunchKernelGGL((compact_pair_kernel<true>), dim3(1), dim3(kPageThreads), 0, stream, s, c,
+                       copy_src, copy_dst, copy_count);
+  } else {
+    hipLaunchKernelGGL(compact_clear_kernel, dim3(grid_of(c.words)), dim3(256), 0, stream, c);
+    hipLaunchKernelGGL(compact_mark_kernel, dim3(grid_of(s.num_blocks)), dim3(256), 0, stream, s,
+                       c);
+    hipLaunchKernelGGL((compact_pair_kernel<false>), dim3(1), dim3(kPageThreads), 0, stream, s, c,
+                       copy_src, copy_dst, copy_count);
+  }
   int64_t lanes = (int64_t)s.num_rows * s.cols;
   if (lanes < s.num_blocks) lanes = s.num_blocks;
   hipLaunchKernelGGL(compact_apply_kernel, dim3(grid_of(lanes)), dim3(256), 0, stream, s, c,

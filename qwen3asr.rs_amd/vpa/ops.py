@@ -21,6 +21,7 @@ launch, as the reference returns ``Err(candle_core::Error::Msg)``.
 from __future__ import annotations
 
 import contextlib
+from array import array
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -494,6 +495,60 @@ class DecodeTokenState:
             self.active_count.data_ptr(), self.batch, _stream(self.next_ids)))
 
 
+class _Pools:
+    """Addresses, strides and sizes of the blocks of ``buffers``, checked, in the host
+    arrays that ``vpa_copy_blocks`` reads."""
+
+    def __init__(self, buffers: Sequence[torch.Tensor], blocks: int, device: int):
+        # (a hundred or more tensors per call: few calls for each)
+        self.blocks = blocks
+        try:
+            plain = all([t.is_contiguous() and t.get_device() == device and t.shape[0] == blocks
+                         for t in buffers])
+        except IndexError:  # a tensor without dimensions
+            plain = False
+        if plain and blocks:
+            size = [t.nbytes // blocks for t in buffers]
+            if 0 not in size:
+                self.count = len(size)
+                self.base = array("Q", [t.data_ptr() for t in buffers])
+                self.size = self.stride = array("q", size)
+                return
+        base, size, stride = [], [], []
+        for t in buffers:
+            if t.get_device() != device:
+                _require_device(t)
+                raise _err(f"device mismatch: a buffer on {t.device}, ids on cuda:{device}")
+            if t.dim() < 1 or t.shape[0] != blocks:
+                raise _err(f"buffers must be pools of {blocks} blocks, got {tuple(t.shape)}")
+            if blocks and t.is_contiguous():
+                n = t.nbytes // blocks
+                stride.append(n)
+            elif blocks:
+                if not t[0].is_contiguous():
+                    raise _err(f"buffers must have contiguous blocks, got {tuple(t.shape)} of "
+                               f"strides {t.stride()}")
+                n = t.numel() // blocks * t.element_size()
+                stride.append(t.stride(0) * t.element_size() if blocks > 1 else n)
+            if blocks and n:
+                base.append(t.data_ptr())
+                size.append(n)
+            elif blocks:
+                stride.pop()
+        self.count = len(base)
+        self.base, self.stride, self.size = array("Q", base), array("q", stride), array("q", size)
+
+    def copy(self, src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
+             num_pairs: Optional[torch.Tensor]) -> None:
+        """The copies of contiguous u32 pairs, on the current device and stream."""
+        if self.count == 0:
+            return
+        check(_lib.load().vpa_copy_blocks(
+            self.base.buffer_info()[0], self.stride.buffer_info()[0], self.size.buffer_info()[0],
+            self.count, src_blocks.data_ptr(), dst_blocks.data_ptr(), _ptr(num_pairs),
+            src_blocks.numel(), self.blocks, _stream(src_blocks)))
+
+
 def _fork_map(batch: int, src_rows: torch.Tensor, dst_rows: torch.Tensor,
               ok: torch.Tensor) -> torch.Tensor:
     """The row that each row of the batch goes on from, i64 [batch]."""
@@ -620,8 +675,6 @@ class DeviceBlockAllocator:
         return src, dst, count
 
     def _pools(self, buffers: Sequence[torch.Tensor]):
-        from .pages import _Pools
-
         return _Pools(buffers, self.ring_capacity, self.block_tables.get_device())
 
     def _pairs(self, n: int):
