@@ -1568,8 +1568,8 @@ int vpa_adjust_logits(void* logits, int64_t seq_stride, int64_t row_stride, int3
       return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_masks=%d, but %lld rows without allowed_rows",
                   op, num_masks, (long long)rows);
   }
-  // (512-lane workgroups: the grid's lane count must fit in 32 bits; a row has at most
-  // one per 16384 tokens for its mask and per 32768 for its lists)
+  // (512-lane workgroups: the grid's lane count must fit in 32 bits; beyond about 512 in
+  // all, a row has at most one per 32760 tokens)
   if (vocab > (1 << 30) || rows > 0x7fffffLL / (((int64_t)vocab + 16383) / 16384 * 2))
     return fail(VPA_ERR_UNSUPPORTED, "%s: too many logits for one launch", op);
   const AdjustArgs a{logits, seq_stride, row_stride, num_seqs, rows_per_seq, vocab, generated,
