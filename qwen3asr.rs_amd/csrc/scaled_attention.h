@@ -148,7 +148,7 @@ constexpr bool scaled_two_tiles(int head_dim) {
 // Waves per SIMD: O, Q and two tiles' bytes are what a wave holds.
 template <typename T, int D, int NQ>
 constexpr int scaled_waves_per_eu() {
-  return D <= 128 ? 2 : 1;
+  return D <= 128 || (D == 192 && !std::is_same_v<T, float>) ? 2 : 1;
 }
 
 template <typename T, int D, int BS, int NQ>
@@ -253,6 +253,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
   }
 
   f32x4_t o[NQ][DT];
+  float kref = 1.f;
   float m[NQ], mt[NQ], lsum[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
@@ -373,25 +374,31 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
       const Scales sc1 = load_scales(ids1);
 
       // ---- scales ----
-      float kref = sc.k[0], vmax = fabsf(sc.v[0]);
-      if constexpr (NI == 2) {
-        kref = fmaxf(kref, sc.k[1]);
-        vmax = fmaxf(vmax, fabsf(sc.v[1]));
-      }
-      kref = max_rows(kref);
-      vmax = max_rows(vmax);
-      // x over a power of two `ref`; both are powers of two, x >= 2^-5 ref
+      // x over a power of two `ref`; both are powers of two, 2^-5 ref <= x <= ref
       auto ratio = [](float x, float ref) {
         return __uint_as_float(__float_as_uint(x) - __float_as_uint(ref) + 0x3f800000u);
       };
       auto plain = [](float x, float ref) {
-        return ((__float_as_uint(x) | __float_as_uint(ref)) & 0x7fffffu) == 0 && x >= ref * 0.03125f;
+        return ((__float_as_uint(x) | __float_as_uint(ref)) & 0x7fffffu) == 0 &&
+               x >= ref * 0.03125f && x <= ref;
       };
-      float fs = kref * a.scale_log2;
-      bool odd = !plain(sc.k[0], kref);
-      if constexpr (NI == 2) odd = odd || !plain(sc.k[1], kref);
-      const bool kfast = __ballot(odd) == 0 && fs > 0.f;  // (uniform)
-      if (!kfast) fs = 1.f;
+      auto all_plain = [&](const float(&x)[NI], float ref) {
+        bool odd = !plain(x[0], ref);
+        if constexpr (NI == 2) odd = odd || !plain(x[1], ref);
+        return __ballot(odd) == 0;  // (uniform)
+      };
+      auto largest = [&](const float(&x)[NI]) {
+        float v = fabsf(x[0]);
+        if constexpr (NI == 2) v = fmaxf(v, fabsf(x[1]));
+        return max_rows(v);
+      };
+      bool kfast = all_plain(sc.k, kref);
+      if (!kfast) {  // (rare where scales are powers of two of one size)
+        kref = largest(sc.k);
+        kfast = all_plain(sc.k, kref);
+      }
+      kfast = kfast && kref * a.scale_log2 > 0.f;  // (a maximum goes through the scale)
+      const float fs = kfast ? kref * a.scale_log2 : 1.f;
       float kr[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) kr[i] = kfast ? ratio(sc.k[i], kref) : 1.f;
@@ -463,6 +470,8 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
       }
 
       // ---- online softmax ----
+      // Each lane looks at its own 16 keys of a row; only where one passes the
+      // reference maximum by more than the slack are the row's four lanes compared.
       float mx[NQ];
       bool move = false;
 #pragma unroll
@@ -472,17 +481,19 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         for (int b = 0; b < 4; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx[q] = fmaxf(mx[q], sv[q][b][r]);
-        mx[q] = max_rows(mx[q]) * fs;
+        mx[q] *= fs;
         mt[q] = fmaxf(mt[q], mx[q]);
-        move = move || mx[q] > m[q] + kScaledSlack || (m[q] == -INFINITY && mx[q] > -INFINITY);
+        move = move || mx[q] > m[q] + kScaledSlack;  // (m is -inf before the first key)
       }
-      if (__ballot(move || vmax > vref) != 0) {
-        const float vnew = fmaxf(vref, vmax);
+      bool vmore = fabsf(sc.v[0]) > vref;
+      if constexpr (NI == 2) vmore = vmore || fabsf(sc.v[1]) > vref;
+      if (__ballot(move || vmore) != 0) {
+        const float vnew = fmaxf(vref, largest(sc.v));
         const float fv = vref / vnew;
         vref = vnew;
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          const float mn = fmaxf(m[q], mx[q]);
+          const float mn = fmaxf(m[q], max_rows(mx[q]));
           const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mn);
           m[q] = mn;
           lsum[q] *= f;
@@ -492,9 +503,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
             for (int r = 0; r < 4; ++r) o[q][dt][r] *= f * fv;
         }
       }
-      odd = !plain(sc.v[0], vref);
-      if constexpr (NI == 2) odd = odd || !plain(sc.v[1], vref);
-      const bool vfast = __ballot(odd) == 0;
+      const bool vfast = all_plain(sc.v, vref);
       float vr[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) vr[i] = vfast ? ratio(sc.v[i], vref) : 1.f;
@@ -649,6 +658,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
   float fo[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
+    mt[q] = max_rows(mt[q]);
     const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mt[q]);
     const float f1 = f * (1.f / (1 << kScaledProbLog2));
     lsum[q] = sum_rows(lsum[q]) * f1;
@@ -748,24 +758,40 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledDev a, in
   const int nchunks = (L + a.chunk_tokens - 1) / a.chunk_tokens;
   if (nchunks <= 1 || r >= n * a.num_heads) return;
   const int64_t row = (int64_t)qa * a.num_heads + r;
-  const float* stat = a.part_stat + row * a.max_chunks * 2;
-  float mx = -INFINITY;
-  for (int c = lane; c < nchunks; c += 64) mx = fmaxf(mx, stat[2 * c]);
-  mx = wave_max_dpp(mx);
-  float sum = 0.f;
-  constexpr int NV = (D + 63) / 64;
-  float v[NV];
+  // eight chunks' parts at a time, all of them under way before one is used
+  const float2* stat = reinterpret_cast<const float2*>(a.part_stat) + row * a.max_chunks;
+  const float* part = a.part_out + row * a.max_chunks * D;
+  constexpr int NV = (D + 63) / 64, U = 8;
+  float mx = -INFINITY, sum = 0.f, v[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) v[k] = 0.f;
-  const float* part = a.part_out + row * a.max_chunks * D + lane;
-  for (int c = 0; c < nchunks; ++c) {
-    const float mc = stat[2 * c];
-    if (mc == -INFINITY) continue;  // (uniform)
-    const float f = __builtin_amdgcn_exp2f(mc - mx);
-    sum = fmaf(f, stat[2 * c + 1], sum);
+  for (int c0 = 0; c0 < nchunks; c0 += U) {
+    float2 st[U];
+    float x[U][NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (lane + 64 * k < D) v[k] = fmaf(f, part[(int64_t)c * D + 64 * k], v[k]);
+    for (int u = 0; u < U; ++u) {
+      const int c = min(c0 + u, nchunks - 1);
+      st[u] = stat[c];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) x[u][k] = part[(int64_t)c * D + min(lane + 64 * k, D - 1)];
+    }
+    float top = mx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, c0 + u < nchunks ? st[u].x : -INFINITY);
+    if (top == -INFINITY) continue;  // (uniform; rows that saw no key so far)
+    const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
+    mx = top;
+    sum *= f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] *= f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool have = c0 + u < nchunks && st[u].x != -INFINITY;
+      const float g = have ? __builtin_amdgcn_exp2f(st[u].x - mx) : 0.f;
+      sum = fmaf(g, have ? st[u].y : 0.f, sum);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) v[k] = have ? fmaf(g, x[u][k], v[k]) : v[k];
+    }
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / (sum + a.denom_eps) : 0.f;
 #pragma unroll

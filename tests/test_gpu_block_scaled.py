@@ -319,6 +319,37 @@ def test_scales_far_apart(device):
             p.check()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 0.3])
+@pytest.mark.parametrize("rows", [None, [300, 20]])
+def test_any_softmax_scale(device, dtype, scale, rows):
+    """Negative, zero and tiny softmax scales, over scales of 1 and of other sizes, in contexts
+    of many steps."""
+    for ks in (None, 1.0, 2.0 ** -3):
+        p = Problem(device, 9, dtype, 4, 2, 64, 16, [1500, 700], rows=rows)
+        p.scale = scale
+        if ks is not None:
+            p.ks[:] = ks
+            p.ks[p.tables[0, 40:]] = 2.0 ** -7
+        p.q = (p.q.float() / 64).to(dtype)
+        p.check()
+
+
+def test_scales_that_turn_odd(device):
+    """Powers of two, then others, then smaller ones, absent blocks among them."""
+    for rows in (None, [250, 40]):
+        p = Problem(device, 19, torch.bfloat16, 4, 2, 64, 8, [1300, 600], rows=rows)
+        cols = p.tables.shape[1]
+        for s in (p.ks, p.vs):
+            s[p.tables[0, 30:60]] *= 0.7
+            s[p.tables[0, 90:95]] *= 2.0 ** -12
+            s[p.tables[0, 100:]] *= 2.0 ** -4
+            s[p.tables[1, 10]] = 0.0
+        p.tables[0, 70] = 0xFFFFFFFF
+        assert cols > 100
+        p.check()
+
+
 def test_zero_scales_and_negative_softmax_scale(device):
     p = Problem(device, 9, torch.bfloat16, 4, 2, 64, 16, [100, 50])
     p.scale = -0.2

@@ -33,11 +33,11 @@ def test_append_rejects(over, code, needle):
     refused("vpa_reshape_and_cache_block_scaled", AP, over, code, needle)
 
 
-def aws(n=4, mq=3, mc=2000, rows=9, h=16, kvh=8, d=128, dtype=BF16):
+def aws(n=4, mq=3, mc=20000, rows=9, h=16, kvh=8, d=128, dtype=BF16):
     return _lib.load().vpa_paged_attention_block_scaled_workspace_size(n, mq, mc, rows, h, kvh, d, dtype)
 
 
-AT = dict(out=P, q=P, ks=P, vs=P, sst=8, kc=P, vc=P, bt=P, bts=125, cu=P, cl=P, n=4, mq=3, mc=2000,
+AT = dict(out=P, q=P, ks=P, vs=P, sst=8, kc=P, vc=P, bt=P, bts=1250, cu=P, cl=P, n=4, mq=3, mc=20000,
           rows=9, scale=0.1, eps=0.0, causal=1, h=16, kvh=8, d=128, bs=16, nb=200, bst=8 * 2048, hst=2048,
           dtype=BF16, ws=P, wsb=1 << 30, stream=None)
 
@@ -52,7 +52,7 @@ AT = dict(out=P, q=P, ks=P, vs=P, sst=8, kc=P, vc=P, bt=P, bts=125, cu=P, cl=P, 
     (dict(mq=1 << 30), UNS, "too many"), (dict(n=1 << 22, mc=1 << 16, bts=1 << 12), UNS, "too many"),
     (dict(out=None), INV, "non-null"), (dict(q=None), INV, "non-null"), (dict(bt=None), INV, "non-null"),
     (dict(cl=None), INV, "non-null"), (dict(q=P + 2), INV, "16-byte"), (dict(out=P + 8), INV, "16-byte"),
-    (dict(bts=124), INV, "too small"), (dict(ws=None), WS, "bytes needed"),
+    (dict(bts=1249), INV, "too small"), (dict(ws=None), WS, "bytes needed"),
     (dict(wsb=aws() - 1), WS, "bytes needed"), (dict(ws=P + 16), INV, "256-byte"),
 ])
 def test_attention_rejects(over, code, needle):
@@ -66,7 +66,7 @@ def test_attention_of_nothing():
 
 def test_attention_workspace():
     assert aws(n=0) == aws(mq=0) == aws(mc=0) == aws(rows=0) == aws(kvh=0) == 0
-    assert aws(n=512, mc=2048, rows=512, mq=1) == 0  # one chunk of keys: nothing to join
+    assert aws(n=512, mc=4096, rows=512, mq=1) == aws(mc=512) == 0  # one chunk of keys: nothing to join
     # every row's parts: head_dim sums, a maximum and a sum
     assert aws() % (9 * 16 * 130 * 4) == 0 and aws() > 0
     assert aws(n=1, mq=1 << 20, mc=1 << 28, rows=1 << 20) >= 0  # in 64 bits
