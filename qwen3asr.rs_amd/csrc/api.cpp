@@ -1275,7 +1275,8 @@ int vpa_reshape_and_cache_block_scaled(const void* key, const void* value,
   if (!aligned16(key) || !aligned16(value) || (key_token_stride * eb) % 16 != 0 ||
       (value_token_stride * eb) % 16 != 0)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: key/value rows must be 16-byte aligned", op);
-  // (256-lane workgroups on a 1D grid whose lane count must fit in 32 bits)
+  // (two 64-lane workgroups per block's worth of tokens and kv head on a 1D grid, whose
+  // lane count must fit in 32 bits)
   if ((num_tokens + block_size - 1) / block_size > 0xffffffLL / num_kv_heads)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: too many tokens for one launch: %lld", op,
                 (long long)num_tokens);
@@ -1568,9 +1569,9 @@ int vpa_adjust_logits(void* logits, int64_t seq_stride, int64_t row_stride, int3
       return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_masks=%d, but %lld rows without allowed_rows",
                   op, num_masks, (long long)rows);
   }
-  // (512-lane workgroups: the grid's lane count must fit in 32 bits; beyond about 512 in
+  // (1024-lane workgroups: the grid's lane count must fit in 32 bits; beyond about 512 in
   // all, a row has at most one per 32760 tokens)
-  if (vocab > (1 << 30) || rows > 0x7fffffLL / (((int64_t)vocab + 16383) / 16384 * 2))
+  if (vocab > (1 << 30) || rows > 0x3fffffLL / (((int64_t)vocab + 16383) / 16384 * 2))
     return fail(VPA_ERR_UNSUPPORTED, "%s: too many logits for one launch", op);
   const AdjustArgs a{logits, seq_stride, row_stride, num_seqs, rows_per_seq, vocab, generated,
                      generated_stride, gen_len, prompt, prompt_stride, prompt_len, draft_ids,

@@ -29,7 +29,7 @@
 namespace vpa {
 namespace {
 
-constexpr int kAdjustThreads = 512;
+constexpr int kAdjustThreads = 1024;
 constexpr uint32_t kCountMask = (1u << 20) - 1;  // occurrences
 constexpr uint32_t kInPrompt = 1u << 20;
 constexpr int kBiasShift = 21;      // entry + 1, at most kAdjustMaxBias

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import VpaError, check
-from .ops import _err, _on_device_of, _ptr, _require_device, _stream, cache_geometry, dtype_code
+from .ops import _err, _on_device_of, _ptr, _same_device, _stream, cache_geometry, dtype_code
 
 
 def block_scales(num_blocks: int, num_kv_heads: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -20,6 +20,21 @@ def block_scales(num_blocks: int, num_kv_heads: int, device) -> Tuple[torch.Tens
 
 
 def _geometry(key_cache, value_cache, key_scales, value_scales):
+    """``cache_geometry`` of an fp8 cache and the scales' block stride. (Called for every
+    layer of a step: one look at each shape and stride, the messages where one is wrong.)"""
+    kd, vd = key_cache.dtype, value_cache.dtype
+    if kd is vd and (kd is torch.float8_e4m3fn or kd is torch.uint8) and key_cache.dim() == 5 \
+            and value_cache.dim() == 4:
+        nb, kvh, dx, bs, x = key_cache.shape
+        s0, s1, s2, s3, s4 = key_cache.stride()
+        d = dx * 16
+        if x == 16 and value_cache.shape == (nb, kvh, d, bs) and s4 == 1 and s3 == 16 and \
+                s2 == bs * 16 and value_cache.stride() == (s0, s1, bs, 1) and s1 >= d * bs and \
+                key_scales.dtype is value_scales.dtype is torch.float32 and \
+                key_scales.shape == value_scales.shape == (nb, kvh):
+            stride = key_scales.stride()
+            if value_scales.stride() == stride and stride[1] == 1 and nb > 1:
+                return nb, kvh, d, bs, s0, s1, stride[0]
     geometry = cache_geometry(key_cache, value_cache)
     nb, kvh = geometry[:2]
     if dtype_code(key_cache.dtype) != _lib.DTYPE_FP8_E4M3:
@@ -47,26 +62,29 @@ def reshape_and_cache_block_scaled(key: torch.Tensor, value: torch.Tensor,
     token at offset 0 of a block opens it (what it held no longer counts); a larger
     element later rescales the bytes that are there. Tokens of one block are neighbours
     in the call."""
-    _require_device(key, value, key_cache, value_cache, slot_mapping, key_scales, value_scales)
+    _same_device(key_cache, key, value, value_cache, slot_mapping, key_scales, value_scales)
     nb, kvh, d, bs, bstride, hstride, sstride = _geometry(key_cache, value_cache, key_scales,
                                                           value_scales)
-    if key.dim() != 3 or value.shape != key.shape:
+    shape = key.shape
+    if len(shape) != 3 or value.shape != shape:
         raise _err(f"key/value must be [T, KVH, D] of equal shape, got {tuple(key.shape)} and "
                    f"{tuple(value.shape)}")
-    t, kh, kd = key.shape
-    if (kh, kd) != (kvh, d):
+    t, kh, kd = shape
+    if kh != kvh or kd != d:
         raise _err(f"key shape {tuple(key.shape)} does not match cache heads={kvh} dim={d}")
-    if key.dtype != value.dtype:
+    if key.dtype is not value.dtype:
         raise _err(f"key/value dtype mismatch: {key.dtype} vs {value.dtype}")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != t:
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (t,):
         raise _err(f"slot_mapping must be i64 [{t}], got {slot_mapping.dtype} "
                    f"{tuple(slot_mapping.shape)}")
-    if key.stride(2) != 1 or key.stride(1) != d:
-        key = key.contiguous()
-    if value.stride(2) != 1 or value.stride(1) != d:
-        value = value.contiguous()
-    # (one token: its stride is free)
-    ks, vs = (key.stride(0), value.stride(0)) if t > 1 else (kvh * d, kvh * d)
+    ks, kh, kd = key.stride()
+    if kd != 1 or kh != d:
+        key, ks = key.contiguous(), kvh * d
+    vs, kh, kd = value.stride()
+    if kd != 1 or kh != d:
+        value, vs = value.contiguous(), kvh * d
+    if t <= 1:  # (one token: its stride is free)
+        ks = vs = kvh * d
     slot_mapping = slot_mapping.contiguous()
     with _on_device_of(key_cache):
         check(_lib.load().vpa_reshape_and_cache_block_scaled(
@@ -108,18 +126,19 @@ def paged_attention_block_scaled(q: torch.Tensor, key_scales: torch.Tensor,
     The maxima size the grid; a caller that knows them on the host passes them to skip a
     device read. ``denom_eps`` is added to the softmax denominator: by default as
     ``paged_attention`` (1e-6) and ``paged_attention_varlen_prefill`` (0 where causal) do."""
-    _require_device(q, key_cache, value_cache, key_scales, value_scales, block_tables,
-                    context_lens, cu_seqlens_q, out, workspace)
+    _same_device(q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens,
+                 cu_seqlens_q, out, workspace)
     nb, kvh, d, bs, bstride, hstride, sstride = _geometry(key_cache, value_cache, key_scales,
                                                           value_scales)
-    if q.dim() != 3 or q.shape[2] != d:
+    shape, tables = q.shape, block_tables.shape
+    if len(shape) != 3 or shape[2] != d:
         raise _err(f"q must be [total_q, H, {d}], got {tuple(q.shape)}")
-    rows, h, _ = q.shape
-    if block_tables.dtype != torch.uint32 or block_tables.dim() != 2:
+    rows, h, _ = shape
+    if block_tables.dtype is not torch.uint32 or len(tables) != 2:
         raise _err(f"block_tables must be u32 2-d, got {block_tables.dtype} "
                    f"{tuple(block_tables.shape)}")
-    b = block_tables.shape[0]
-    if context_lens.dtype != torch.uint32 or context_lens.shape != (b,):
+    b, cols = tables
+    if context_lens.dtype is not torch.uint32 or context_lens.shape != (b,):
         raise _err(f"context_lens must be u32 [{b}], got {context_lens.dtype} "
                    f"{tuple(context_lens.shape)}")
     if cu_seqlens_q is None:
@@ -158,7 +177,7 @@ def paged_attention_block_scaled(q: torch.Tensor, key_scales: torch.Tensor,
         check(lib.vpa_paged_attention_block_scaled(
             out.data_ptr(), q.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), sstride,
             key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-            block_tables.shape[1], _ptr(cu_seqlens_q), context_lens.data_ptr(), b,
+            cols, _ptr(cu_seqlens_q), context_lens.data_ptr(), b,
             int(max_query_len), int(max_context_len), rows, float(softmax_scale),
             float(denom_eps), int(bool(causal)), h, kvh, d, bs, nb, bstride, hstride, code,
             _ptr(workspace), nbytes, _stream(q)))

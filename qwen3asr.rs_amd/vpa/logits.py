@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .ops import _err, _on_device_of, _ptr, _require_device, _stream, dtype_code
+from .ops import _err, _on_device_of, _ptr, _same_device, _stream, dtype_code
 
 
 def _list(name: str, ids: Optional[torch.Tensor], lengths: Optional[torch.Tensor], b: int):
@@ -61,13 +61,16 @@ def adjust_logits(logits: torch.Tensor, generated: Optional[torch.Tensor] = None
     ``allowed`` u32 [M, >= ceil(V / 32)] are masks of one bit per token: a row takes mask
     allowed_rows[b] or allowed_rows[b, i] (u32; one >= M: none; None: the mask of its
     index) and what its mask leaves out becomes -inf."""
-    _require_device(logits, generated, gen_len, prompt, prompt_len, draft_ids, repetition,
-                    presence, frequency, bias_ids, bias, bias_len, allowed, allowed_rows)
-    if logits.dim() not in (2, 3):
+    _same_device(logits, generated, gen_len, prompt, prompt_len, draft_ids, repetition, presence,
+                 frequency, bias_ids, bias, bias_len, allowed, allowed_rows)
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) == 3:
+        b, k1, v = shape
+    elif len(shape) == 2:
+        (b, v), k1 = shape, 1
+    else:
         raise _err(f"logits must be [B, V] or [B, K + 1, V], got {tuple(logits.shape)}")
-    b, v = logits.shape[0], logits.shape[-1]
-    k1 = logits.shape[1] if logits.dim() == 3 else 1
-    if v > 1 and logits.stride(-1) != 1:
+    if v > 1 and strides[-1] != 1:
         raise _err("logits must be contiguous along the vocabulary")
     gen, gen_cap, gen_len = _list("generated", generated, gen_len, b)
     pro, pro_cap, prompt_len = _list("prompt", prompt, prompt_len, b)
@@ -100,8 +103,8 @@ def adjust_logits(logits: torch.Tensor, generated: Optional[torch.Tensor] = None
                        f"{allowed_rows.dtype} {tuple(allowed_rows.shape)}")
         allowed_rows = allowed_rows.contiguous()
     # (a dimension of one row has a free stride)
-    row = logits.stride(1) if logits.dim() == 3 and k1 > 1 else v
-    seq = logits.stride(0) if b > 1 else row * k1
+    row = strides[1] if k1 > 1 else v
+    seq = strides[0] if b > 1 else row * k1
     with _on_device_of(logits):
         check(_lib.load().vpa_adjust_logits(
             logits.data_ptr(), seq, row, b, k1, v, dtype_code(logits.dtype), _ptr(gen), gen_cap,

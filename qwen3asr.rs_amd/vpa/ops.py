@@ -87,6 +87,14 @@ def _require_device(*ts: torch.Tensor) -> None:
             raise _err(f"device mismatch: {first.device} vs {t.device}")
 
 
+def _same_device(first: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
+    """The index of the one GPU that all of them (None aside) are on."""
+    dev = first.get_device()
+    if dev < 0 or [dev] * len(ts) != [dev if t is None else t.get_device() for t in ts]:
+        _require_device(first, *ts)
+    return dev
+
+
 def cache_geometry(key_cache: torch.Tensor, value_cache: torch.Tensor):
     """(num_blocks, num_kv_heads, head_dim, block_size, block_stride, head_stride)
     of a key/value cache pair in the reference layout."""
