@@ -1275,9 +1275,10 @@ int vpa_reshape_and_cache_block_scaled(const void* key, const void* value,
   if (!aligned16(key) || !aligned16(value) || (key_token_stride * eb) % 16 != 0 ||
       (value_token_stride * eb) % 16 != 0)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: key/value rows must be 16-byte aligned", op);
-  // (two 64-lane workgroups per block's worth of tokens and kv head on a 1D grid, whose
-  // lane count must fit in 32 bits)
-  if ((num_tokens + block_size - 1) / block_size > 0xffffffLL / num_kv_heads)
+  // (two 64-lane workgroups per kv head and block's worth of tokens, or token of few, on a
+  // 1D grid, whose lane count must fit in 32 bits)
+  if (std::max(std::min<int64_t>(num_tokens, 2048), (num_tokens + block_size - 1) / block_size) >
+      0x1ffffffLL / num_kv_heads)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: too many tokens for one launch: %lld", op,
                 (long long)num_tokens);
   const CacheGeom g{num_kv_heads, head_dim, block_size, num_blocks, cache_block_stride,

@@ -723,9 +723,9 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
     float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < kScaledWaves; ++x) {
+      // (a wave without a maximum has seen no key: zeros; or nothing but NaN, which stays)
       const float mw = s_stat[2 * (x * nr + r)];
-      if (mw == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(mw - mx);
+      const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mx);
       const float4 y = *reinterpret_cast<const float4*>(s_join + (x * nr + r) * D + d);
       sum = fmaf(f, s_stat[2 * (x * nr + r) + 1], sum);
       v[0] = fmaf(f, y.x, v[0]);
@@ -778,7 +778,7 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledDev a, in
     float top = mx;
 #pragma unroll
     for (int u = 0; u < U; ++u) top = fmaxf(top, c0 + u < nchunks ? st[u].x : -INFINITY);
-    if (top == -INFINITY) continue;  // (uniform; rows that saw no key so far)
+    // (a part without a maximum has seen no key: zeros; or nothing but NaN, which stays)
     const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
     mx = top;
     sum *= f;
@@ -786,8 +786,8 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledDev a, in
     for (int k = 0; k < NV; ++k) v[k] *= f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool have = c0 + u < nchunks && st[u].x != -INFINITY;
-      const float g = have ? __builtin_amdgcn_exp2f(st[u].x - mx) : 0.f;
+      const bool have = c0 + u < nchunks;
+      const float g = st[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[u].x - mx);
       sum = fmaf(g, have ? st[u].y : 0.f, sum);
 #pragma unroll
       for (int k = 0; k < NV; ++k) v[k] = have ? fmaf(g, x[u][k], v[k]) : v[k];

@@ -87,7 +87,7 @@ class DeviceDecodeStep:
         step's slots, then attend over the shared block tables. Scales of shape
         [num_blocks, kv_heads] are those of a block-scaled cache, which are set by
         the append; one-element scales those of an fp8 cache."""
-        if k_scale is not None and k_scale.dim() == 2:
+        if k_scale is not None and k_scale.numel() > 1:
             block_scaled.reshape_and_cache_block_scaled(k, v, k_scale, v_scale, key_cache,
                                                         value_cache, self.allocator.slot_mapping)
             block_scaled.paged_attention_block_scaled(

@@ -307,6 +307,21 @@ def test_nan_of_a_later_token_stays_there(device, rows):
     assert np.isnan(got[n - 7:]).all() and not np.isnan(got[:n - 7]).any()
 
 
+@pytest.mark.parametrize("rows", [None, [40, 3], [300, 2]])
+@pytest.mark.parametrize("size", [60, 900, 6000])
+def test_nan_queries_and_keys(device, rows, size):
+    """NaN wherever a row's query, or a key that it sees, holds one: also where every key of
+    a wave's or of a chunk's is such."""
+    p = Problem(device, 16, torch.bfloat16, 2, 1, 64, 16, [size, 100], rows=rows)
+    p.q[0, 1, 7] = float("nan")
+    got = p.check()
+    seen = rows is None or size >= rows[0]
+    assert np.isnan(got[0, 1]).all() == seen and not np.isnan(got[0, 0]).any()
+    p.kc[p.tables[1, :4], :, 1, :, 3] = 0x7F
+    got = p.check()
+    assert np.isnan(got[-1]).all()
+
+
 def test_scales_far_apart(device):
     """Blocks whose values differ by 2^40: the small ones vanish in the sum, nothing else
     does; values and scales that f16 cannot hold."""

@@ -297,3 +297,23 @@ def test_side_stream(device):
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_a_step_over_a_cache_of_one_scale(device):
+    """One-element scales are an fp8 cache's, whatever their shape."""
+    rng = np.random.default_rng(6)
+    step = vpa.DeviceDecodeStep(2, 8, BS, 64, H, D, [EOS], 8, device)
+    assert step.admit(u32([5, 20], device)).cpu().all()
+    q, k, v = (torch.from_numpy(rng.standard_normal((2, n, D)).astype(np.float32)).to(device)
+               for n in (H, KVH, KVH))
+    outs = []
+    for shape in ((1,), (1, 1)):
+        kc = torch.zeros((8, KVH, D // 16, BS, 16), dtype=torch.uint8, device=device)
+        vc = torch.zeros((8, KVH, D, BS), dtype=torch.uint8, device=device)
+        if not outs:
+            step.begin(kc, vc, torch.float32)
+        one = torch.full(shape, 0.25, device=device)
+        outs.append(torch.empty((2, H, D), device=device))
+        step.layer(q, k, v, kc, vc, outs[-1], one, one)
+    torch.cuda.synchronize()
+    assert outs[0].any() and torch.equal(outs[0], outs[1])
