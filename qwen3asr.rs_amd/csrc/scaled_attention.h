@@ -86,6 +86,15 @@ __device__ __forceinline__ void fp8x16_times(const uint4& v, float slo, float sh
   hi = make_uint4(cvt(v.z, shi, l), cvt(v.z, shi, h), cvt(v.w, shi, l), cvt(v.w, shi, h));
 }
 
+// Four times: a matrix instruction, then two vector instructions in its shadow.
+__device__ __forceinline__ void alternate() {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+  }
+}
+
 constexpr int kScaledWaves = 4;
 constexpr int kScaledKeys = 64;  // keys of a step
 constexpr float kScaledSlack = 8.f;
@@ -136,6 +145,7 @@ struct ScaledDev {
   int32_t tiles, chunk_tokens, max_chunks;
   int32_t split_keys;  // the waves share 16 NQ rows and split the keys
   int32_t lds_rows;    // rows kept in LDS then
+  int32_t row_waves;   // waves of a workgroup with rows of their own (1: shared)
   float scale_log2, denom_eps;
 };
 
@@ -192,7 +202,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
   n = (int64_t)qa >= a.total_rows ? 0 : (int)min((int64_t)n, a.total_rows - (int64_t)qa);
   const int L = (int)min(a.context_lens[s], (uint32_t)a.max_ctx);
   const int rows = n * a.group;
-  const int wg_rows = (a.split_keys ? 1 : kScaledWaves) * 16 * NQ;
+  const int wg_rows = a.row_waves * 16 * NQ;
   if (qt * wg_rows >= rows) return;  // (uniform over the workgroup)
   const int nchunks = max(1, (L + a.chunk_tokens - 1) / a.chunk_tokens);
   if (chunk >= nchunks) return;
@@ -403,28 +413,39 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 #pragma unroll
       for (int i = 0; i < NI; ++i) kr[i] = kfast ? ratio(sc.k[i], kref) : 1.f;
 
-      // ---- S^T, tile by tile ----
+      // ---- S^T, 64 dims of a tile at a time, the next ones' bytes converted meanwhile ----
       f32x4_t sv[NQ][4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        // (keeps a wave from holding every tile's operands at once)
-        if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) sv[q][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      auto tile_ratio = [&](int b) {
         float krb = readlane_f(kr[0], 16 * b);
         if constexpr (NI == 2) krb = c16 < 8 ? krb : readlane_f(kr[1], 16 * b);
+        return krb;
+      };
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          uint4 op[2];
-          fp8x16_times<K>(kraw[b][i], krb, krb, op[0], op[1]);
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int q = 0; q < NQ; ++q) sv[q][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      uint4 kop[2][2];
+      {
+        const float krb = tile_ratio(0);
+        fp8x16_times<K>(kraw[0][0], krb, krb, kop[0][0], kop[0][1]);
+      }
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
-#pragma unroll
-              for (int p = QP - 1; p >= 0; --p)
-                sv[q][b] = mfma16x16x32<K>(op[h], qop[q][p][2 * i + h], sv[q][b]);
+      for (int t = 0; t < 4 * NC; ++t) {
+        if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
+        if (t + 1 < 4 * NC) {
+          const float krb = tile_ratio((t + 1) / NC);
+          fp8x16_times<K>(kraw[(t + 1) / NC][(t + 1) % NC], krb, krb, kop[(t + 1) % 2][0],
+                          kop[(t + 1) % 2][1]);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int p = QP - 1; p >= 0; --p)
+              sv[q][t / NC] =
+                  mfma16x16x32<K>(kop[t % 2][h], qop[q][p][2 * (t % NC) + h], sv[q][t / NC]);
+        if constexpr (NQ == 2) alternate();
       }
       if constexpr (kEarly) {
         if (k0 + k_step < k_end) load_k(ids1, kraw);
@@ -554,7 +575,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
           for (int h = 0; h < 2; ++h) transpose_rows(pw[q][p][h]);
       }
 
-      // ---- O^T += V^T P^T ----
+      // ---- O^T += V^T P^T, the next dims' bytes converted meanwhile ----
       if (!full) {
         // A NaN value of a token that only later rows see would reach every row
         // of the tile through 0 * NaN: such bytes count as 0 here and are gone
@@ -586,23 +607,26 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         __builtin_amdgcn_sched_barrier(0);
         load_k(ids1, kraw);
       }
+      uint4 vop[2][2];
+      fp8x16_times<f16_t>(vraw[0], vr[0], vr[NI - 1], vop[0][0], vop[0][1]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        if constexpr (!kEarly)
-          if (dt % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-        uint4 op[2];
-        fp8x16_times<f16_t>(vraw[dt], vr[0], vr[NI - 1], op[0], op[1]);
+        if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
+        if (dt + 1 < DT)
+          fp8x16_times<f16_t>(vraw[dt + 1], vr[0], vr[NI - 1], vop[(dt + 1) % 2][0],
+                              vop[(dt + 1) % 2][1]);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
+        for (int p = PP - 1; p >= 0; --p)
 #pragma unroll
-          for (int p = PP - 1; p >= 0; --p)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int q = 0; q < NQ; ++q)
               o[q][dt] = mfma16x16x32<f16_t>(
-                  op[h],
+                  vop[dt % 2][h],
                   make_uint4(pw[q][p][0][2 * h], pw[q][p][1][2 * h], pw[q][p][0][2 * h + 1],
                              pw[q][p][1][2 * h + 1]),
                   o[q][dt]);
+        if constexpr (NQ == 2) alternate();
       }
       ids = ids1;
       ids1 = ids2;
@@ -804,7 +828,7 @@ template <typename T, int D, int BS, int NQ>
 hipError_t launch_scaled_t(const ScaledDev& d, int64_t grid, hipStream_t stream) {
   const size_t lds = d.split_keys ? (size_t)kScaledWaves * d.lds_rows * (D + 2) * 4 : 0;
   hipLaunchKernelGGL((scaled_attention_kernel<T, D, BS, NQ>), dim3((unsigned)grid),
-                     dim3(64 * kScaledWaves), lds, stream, d);
+                     dim3(64 * (d.split_keys ? kScaledWaves : d.row_waves)), lds, stream, d);
   if (d.max_chunks > 1) {
     const int tiles = (int)(((int64_t)d.max_query_len * d.num_heads + 3) / 4);
     hipLaunchKernelGGL((scaled_merge_kernel<T, D>), dim3((unsigned)tiles * d.num_seqs), dim3(256),
@@ -854,6 +878,7 @@ hipError_t launch_scaled(const ScaledArgs& a, const CacheGeom& g, const ScaledPl
                     p.max_chunks,
                     p.split_keys,
                     p.lds_rows,
+                    p.row_waves,
                     a.scale * 1.4426950408889634f,
                     a.denom_eps};
 #define VPA_SCALED(DV, BV)                           \
