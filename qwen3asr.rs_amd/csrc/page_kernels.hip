@@ -126,12 +126,12 @@ __global__ __launch_bounds__(kPageThreads) void fork_decide_kernel(
   }
   // an earlier fork of the same row? (four at a time, the reads not waiting on each other)
   bool claimed = false;
-  const int before = min((int)(threadIdx.x | 63u), num_forks);
+  const int before = (int)(threadIdx.x & ~63u) < num_forks ? min(f | 63, num_forks) : 0;
 #pragma unroll 4
   for (int e = 0; e < before; e += 4) {
     const uint4 v = *reinterpret_cast<const uint4*>(&s_dst[e]);
-    claimed = claimed || (v.x == dst && e < f) || (v.y == dst && e + 1 < f) ||
-              (v.z == dst && e + 2 < f) || (v.w == dst && e + 3 < f);
+    claimed |= ((v.x == dst) & (e < f)) | ((v.y == dst) & (e + 1 < f)) |
+               ((v.z == dst) & (e + 2 < f)) | ((v.w == dst) & (e + 3 < f));
   }
   can = can && !claimed;
   const uint32_t full = tokens / (uint32_t)s.block_size;
@@ -185,110 +185,139 @@ __global__ __launch_bounds__(256) void fork_share_kernel(const PageState s,
 // are subtracted, which leaves -1 where none is left; there, the entry that comes
 // last in that order is found by an atomic minimum over codes that fall with the
 // order, in the same word; that entry gives the block back, at a place in the
-// ring by a prefix sum.
+// ring by a prefix sum. The entries are numbered in that order, so a lane takes
+// four of any rows at a time: with a wave per row instead, 96 rows of 40 blocks
+// took 28 us, each waiting for its own loads.
 __global__ __launch_bounds__(kPageThreads) void release_shared_kernel(
     const PageState s, const uint32_t* __restrict__ keep_blocks) {
   __shared__ uint32_t s_tmp[kPageThreads / 64];
-  __shared__ uint32_t s_count[kPageThreads];
-  __shared__ uint32_t s_rows[kPageThreads], s_keep[kPageThreads], s_have[kPageThreads];
-  constexpr int kWaves = kPageThreads / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ uint32_t s_rows[kPageThreads], s_first[kPageThreads], s_have[kPageThreads];
+  constexpr int U = 4;
   const uint32_t head = s.ring_state[0], count = s.ring_state[1];
-  auto code_of = [&](uint32_t r, uint32_t i) {
-    return 0xfffffffeu - (r * (uint32_t)s.cols + ((uint32_t)s.cols - 1u - i));
+  // Of the rows base .. base + 1023 those that give something back, in order, and the
+  // number of each one's first entry; every pass lists them again unless one list
+  // holds them all.
+  struct List {
+    uint32_t rows, entries;
   };
-  auto counted = [&](uint32_t id) { return id != 0 && (int64_t)id < s.num_blocks; };
-  auto entry = [&](uint32_t r, uint32_t i) { return s.block_tables[(int64_t)r * s.cols + i]; };
-  // The rows among base .. base + 1023 that give something back, in order; a wave
-  // takes each of them, a lane each of its entries. Every pass lists them again
-  // unless one list holds them all.
-  auto list_rows = [&](int base) -> int {
+  auto list_rows = [&](int base) {
     const int r = base + threadIdx.x;
     uint32_t have = 0, keep = 0;
     if (r < s.num_rows) {
       have = min(s.row_blocks[r], (uint32_t)s.cols);
       keep = min(keep_blocks[r], have);
     }
-    uint32_t total;
-    const uint32_t rank = group_scan(keep < have ? 1u : 0u, s_tmp, &total);
+    List l;
+    const uint32_t rank = group_scan(keep < have ? 1u : 0u, s_tmp, &l.rows);
+    const uint32_t first = group_scan(have - keep, s_tmp, &l.entries);
     if (keep < have) {
       s_rows[rank] = (uint32_t)r;
-      s_keep[rank] = keep;
+      s_first[rank] = first;
       s_have[rank] = have;
     }
     __syncthreads();
-    return (int)total;
+    return l;
+  };
+  // The blocks of entries e .. e + U - 1 of the list, 0: none or not counted. Their rows
+  // are the last ones whose entries begin at or before them (found together, so that no
+  // search waits for another's reads).
+  auto blocks_of = [&](const List& l, uint32_t e, uint32_t (&id)[U]) {
+    uint32_t row[U] = {};
+    for (uint32_t step = l.rows > 1 ? 1u << (31 - __builtin_clz(l.rows - 1)) : 0u; step != 0;
+         step /= 2) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t next = row[u] + step;
+        if (next < l.rows && s_first[next] <= e + u) row[u] = next;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      id[u] = 0;
+      if (e + u >= l.entries) continue;
+      const uint32_t i = s_have[row[u]] - 1u - (e + u - s_first[row[u]]);
+      id[u] = s.block_tables[(int64_t)s_rows[row[u]] * s.cols + i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = (int64_t)id[u] < s.num_blocks ? id[u] : 0u;
   };
   const bool one_list = s.num_rows <= kPageThreads;
-  int rows = 0;
-  auto pass = [&](auto&& body) {
+  List l{};
+  // few entries are looked up once
+  uint32_t held[U] = {};
+  bool few = false;
+  // body(id[U], number of the first of these entries): consecutive entries of a lane
+  auto pass = [&](auto&& body, auto&& done) {
+    uint32_t before = 0;
     for (int base = 0; base < s.num_rows; base += kPageThreads) {
-      if (!one_list) rows = list_rows(base);
-      for (int k = wave; k < rows; k += kWaves) body(s_rows[k], s_keep[k], s_have[k], k);
-      finish_and_sync();
+      if (!one_list) l = list_rows(base);
+      for (uint32_t at = 0; at < l.entries; at += U * kPageThreads) {
+        const uint32_t e = at + U * threadIdx.x;
+        if (few) {
+          body(held, before + e);
+        } else {
+          uint32_t id[U];
+          blocks_of(l, e, id);
+          body(id, before + e);
+        }
+      }
+      before += l.entries;
+      done();
     }
   };
-  if (one_list) rows = list_rows(0);
-  if (one_list && rows == 0) return;  // (uniform)
-  pass([&](uint32_t r, uint32_t keep, uint32_t have, int) {
-    for (uint32_t i = keep + lane; i < have; i += 64) {
-      const uint32_t id = entry(r, i);
-      if (counted(id)) atomicSub(&s.shared[id], 1u);
-    }
-  });
-  pass([&](uint32_t r, uint32_t keep, uint32_t have, int) {
-    for (uint32_t i = keep + lane; i < have; i += 64) {
-      const uint32_t id = entry(r, i);
-      if (counted(id) && load_fresh(&s.shared[id]) >= 0x80000000u)
-        atomicMin(&s.shared[id], code_of(r, i));
-    }
-  });
-  uint32_t added = 0;
-  for (int base = 0; base < s.num_rows; base += kPageThreads) {
-    if (!one_list) rows = list_rows(base);
-    auto gives = [&](uint32_t r, uint32_t i, uint32_t& id) {
-      id = entry(r, i);
-      return counted(id) && load_fresh(&s.shared[id]) == code_of(r, i);
-    };
-    s_count[threadIdx.x] = 0;
-    __syncthreads();
-    for (int k = wave; k < rows; k += kWaves) {
-      const uint32_t r = s_rows[k], keep = s_keep[k], have = s_have[k];
-      uint32_t n = 0, id;
-      for (uint32_t at = keep; at < have; at += 64) {
-        const bool mine = at + lane < have && gives(r, at + lane, id);
-        n += (uint32_t)__builtin_popcountll(__ballot(mine));
-      }
-      if (lane == 0) s_count[k] = n;
-    }
-    __syncthreads();
-    uint32_t total;
-    const uint32_t before = group_scan(s_count[threadIdx.x], s_tmp, &total);
-    s_count[threadIdx.x] = before;
-    __syncthreads();
-    for (int k = wave; k < rows; k += kWaves) {
-      const uint32_t r = s_rows[k], keep = s_keep[k], have = s_have[k];
-      uint32_t at_ring = (uint32_t)(((uint64_t)head + count + added + s_count[k]) %
-                                    (uint32_t)s.ring_cap);
-      for (uint32_t upto = have; upto > keep; upto = upto >= keep + 64 ? upto - 64 : keep) {
-        // lane 0 takes the last block
-        uint32_t id = 0;
-        const bool mine = upto >= keep + 1 + lane && gives(r, upto - 1 - lane, id);
-        const uint64_t mask = __ballot(mine);
-        if (mine) {
-          const uint32_t rank = __builtin_amdgcn_mbcnt_hi(
-              (uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
-          s.ring[ring_at(s, at_ring, rank)] = id;
-          // (no other entry of this block compares equal, before or after)
-          __hip_atomic_store(&s.shared[id], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        at_ring = ring_at(s, at_ring, (uint32_t)__builtin_popcountll(mask));
-      }
-      if (lane == 0) s.row_blocks[r] = keep;
-    }
-    added += total;
-    __syncthreads();
+  auto code_of = [](uint32_t e) { return 0xfffffffeu - e; };
+  if (one_list) {
+    l = list_rows(0);
+    if (l.rows == 0) return;  // (uniform)
+    few = l.entries <= U * kPageThreads;
+    if (few) blocks_of(l, U * threadIdx.x, held);
   }
+  pass(
+      [&](const uint32_t(&id)[U], uint32_t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (id[u] != 0) atomicSub(&s.shared[id[u]], 1u);
+      },
+      [] { finish_and_sync(); });
+  pass(
+      [&](const uint32_t(&id)[U], uint32_t e) {
+        uint32_t left[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) left[u] = id[u] != 0 ? load_fresh(&s.shared[id[u]]) : 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (left[u] >= 0x80000000u) atomicMin(&s.shared[id[u]], code_of(e + u));
+      },
+      [] { finish_and_sync(); });
+  uint32_t added = 0;
+  pass(
+      [&](const uint32_t(&id)[U], uint32_t e) {
+        uint32_t last[U], n = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) last[u] = id[u] != 0 ? load_fresh(&s.shared[id[u]]) : 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) n += last[u] == code_of(e + u) ? 1u : 0u;
+        uint32_t total;
+        uint32_t at = (uint32_t)(((uint64_t)head + count + added + group_scan(n, s_tmp, &total)) %
+                                 (uint32_t)s.ring_cap);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (last[u] == code_of(e + u)) {
+            s.ring[at] = id[u];
+            at = ring_at(s, at, 1u);
+            // (no other entry of this block compares equal, before or after)
+            __hip_atomic_store(&s.shared[id[u]], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+        added += total;
+      },
+      [&] {
+        const uint32_t k = threadIdx.x;
+        if (k < l.rows) {
+          const uint32_t end = k + 1 < l.rows ? s_first[k + 1] : l.entries;
+          s.row_blocks[s_rows[k]] = s_have[k] - (end - s_first[k]);
+        }
+        __syncthreads();
+      });
   if (threadIdx.x == 0) s.ring_state[1] = count + added;
 }
 

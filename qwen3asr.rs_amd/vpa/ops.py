@@ -510,16 +510,18 @@ class _Pools:
     def __init__(self, buffers: Sequence[torch.Tensor], blocks: int, device: int):
         # (a hundred or more tensors per call: few calls for each)
         self.blocks = blocks
+        cls = torch.Tensor
         try:
-            plain = all([t.is_contiguous() and t.get_device() == device and t.shape[0] == blocks
-                         for t in buffers])
+            plain = all(map(cls.is_contiguous, buffers)) and \
+                set(map(cls.get_device, buffers)) == {device} and \
+                {s[0] for s in map(cls.shape.__get__, buffers)} == {blocks}
         except IndexError:  # a tensor without dimensions
             plain = False
         if plain and blocks:
-            size = [t.nbytes // blocks for t in buffers]
+            size = [n // blocks for n in map(cls.nbytes.__get__, buffers)]
             if 0 not in size:
                 self.count = len(size)
-                self.base = array("Q", [t.data_ptr() for t in buffers])
+                self.base = array("Q", map(cls.data_ptr, buffers))
                 self.size = self.stride = array("q", size)
                 return
         base, size, stride = [], [], []

@@ -71,12 +71,16 @@ class DeviceDecodeStep:
         return ok
 
     def begin(self, key_cache: torch.Tensor, value_cache: torch.Tensor,
-              query_dtype: torch.dtype) -> None:
+              query_dtype: torch.dtype, block_scaled: bool = False) -> None:
         """Step start: pending ids consumed (EOS rows finish), blocks grown,
         this step's slot_mapping / context_lens and the decode work list
-        built (the caches of any layer give the geometry and cache type)."""
+        built (the caches of any layer give the geometry and cache type).
+        Layers over a block-scaled cache need no work list: ``block_scaled``
+        leaves it out, for a step of such layers alone."""
         self.tokens.consume(self.allocator.slot_mapping)
         self.allocator.step(self.tokens.finished)
+        if block_scaled:
+            return
         ops.paged_attention_plan(self.allocator.context_lens, self.max_context_len, self.cols,
                                  self.num_heads, key_cache, value_cache, query_dtype,
                                  self.workspace)

@@ -137,6 +137,21 @@ def test_many_forks(device):
     b.check()
 
 
+@pytest.mark.parametrize("rows,tokens", [(200, 164), (200, 165), (512, 80), (1024, 40), (1000, 99)])
+def test_release_entries_beyond_a_lane_s_few(device, rows, tokens):
+    """About 4096 entries of one list of rows, more, and blocks of their own in between."""
+    b = Both(device, 7000, 8, rows, 22, seed=rows)
+    b.shuffle()
+    b.allocate([tokens, tokens // 2] + [0] * (rows - 2))
+    b.fork(list(b.rng.integers(0, 2, size=rows - 2)), list(range(2, rows)))
+    b.check()
+    b.release(list(b.rng.integers(0, 3, size=rows)))
+    b.check()
+    b.release([0] * rows)
+    b.check()
+    assert b.ref.count == 6999
+
+
 def test_release_more_rows_than_a_pass_takes(device):
     b = Both(device, 6000, 4, 2100, 5, seed=2)
     b.allocate(list(b.rng.integers(0, 9, size=2000)) + [0] * 100)

@@ -317,3 +317,20 @@ def test_a_step_over_a_cache_of_one_scale(device):
         step.layer(q, k, v, kc, vc, outs[-1], one, one)
     torch.cuda.synchronize()
     assert outs[0].any() and torch.equal(outs[0], outs[1])
+
+
+def test_a_block_scaled_step_needs_no_work_list(device):
+    rng = np.random.default_rng(7)
+    prompts = [list(rng.integers(0, V - 1, size=n)) for n in (20, 5)]
+    chosen = []
+    for skip in (False, True):
+        loop = Loop(device)
+        if skip:
+            begin = loop.step.begin
+            loop.step.begin = lambda *a: begin(*a, block_scaled=True)
+        loop.admit(prompts)
+        for _ in range(4):
+            loop.decode()
+        torch.cuda.synchronize()
+        chosen.append(loop.step.tokens.next_ids.cpu().numpy()[:2].tolist())
+    assert chosen[0] == chosen[1]
