@@ -20,6 +20,12 @@
 // a range of the vocabulary, of which only the listed entries are cleared. A word per
 // token holds its count, whether it is in the prompt and which bias it has; integers,
 // so the order of atomics does not show.
+//
+// 256 rows of 151936 bf16 logits, masks that leave every other token out: 29 us, 155 MB
+// read and written (5.3 TB/s; 33 us with workgroups of 512; 47 with workgroups for the
+// sweep and others for the lists of a row). Masked elements stored one by one, without
+// reading their neighbours: 43 us. The sweep's first loads issued before the lists are
+// counted: no difference. One row without a mask: 6 us, the chain of its lists' loads.
 
 #include <algorithm>
 

@@ -18,6 +18,10 @@
 // token lie in every 16-byte vector of its tile, so a partly filled tile is read and
 // written whole: contiguous vectors instead of single bytes in every 32-byte sector;
 // the tile's loads are under way before the rows' largest element is known.
+// A prompt's append is bound by HBM (8 kv heads of 128 dims, bf16: 32768 tokens 39 us
+// for 202 MB, 5.2 TB/s read and written), a decode step's by the chain of its loads and
+// the tiles read and written around single tokens (256 tokens 7.4 us for 17 MB; with a
+// workgroup of 256 lanes for K and V of a block, and its barriers, 9.4 and 69 us).
 
 #include <algorithm>
 #include <type_traits>
@@ -312,22 +316,28 @@ hipError_t launch_scaled_append(int dtype, const ScaledAppendArgs& a, const Cach
   }
 }
 
-// Rows: up to 256 of a (sequence, kv head) go 16 or 32 at a time to a workgroup whose
-// waves split the keys, more have a wave per 16 or 32 of them (8000 keys, 128 rows:
-// 19 us split, 24 not; a batch of 64 with 1024 rows each keeps its waves busy without).
-// Workgroups of such waves are four, which find each other's keys in the L1 cache (32
-// sequences of up to 4000 keys, 512 rows of head dim 192: 629 us, 718 one by one; a
-// chunk of 512 rows over 6000 tokens: 54, 56), but one where there are two tiles a wave
-// and the rows of a workgroup end at different keys, as in a prompt's first chunk (512
-// tokens: 20.4 and 19.4 us; 1000: 33.2 and 31.9), or where more than an eighth of the
-// fours' rows would be missing (64 times 400 rows, 12.5 waves each: 69 and 55 us).
+// Rows: a wave takes 16 or 32 of a (sequence, kv head). Of up to 256 rows the waves of a
+// workgroup share each such tile and split the keys, unless there are enough tiles for
+// waves of their own: 1024 for contexts of up to 512 keys (32 times 200 rows over 100
+// keys: 33 us split, 14 not; 128 decode steps of 60 to 128 keys 10.8, 7.6), 2048 beyond
+// (64 times 200 rows over 2000 keys: 184, 173; 40 rows each, 1024 tiles: 61, 66), where
+// one tile alone is always split (a decode). Contexts of one step of 64 keys have nothing
+// to split (256 of them: 17 us, 8), and more than 256 rows go without (8000 keys, 128
+// rows: 19 us split, 24 not; a batch of 64 with 1024 rows each keeps its waves busy).
+// Workgroups of waves with rows of their own are four, which find each other's keys in
+// the L1 cache (32 sequences of up to 4000 keys, 512 rows of head dim 192: 629 us, 718
+// one by one; a chunk of 512 rows over 6000 tokens: 54, 56), but one where there are two
+// tiles a wave and the rows of a workgroup end at different keys, as in a prompt's first
+// chunk (512 tokens: 20.4 and 19.4 us; 1000: 33.2 and 31.9), or where more than an eighth
+// of the fours' rows would be missing (64 times 400 rows, 12.5 waves each: 69 and 55 us).
 // Keys: chunks over workgroups until there is one workgroup of four waves (split keys)
 // or are two (a wave per rows, which finish at different times) per compute unit of an
-// MI355X, of at least 256 keys where the waves split them; where there are enough
+// MI355X, of at least 256 keys; where the waves split the keys and there are enough
 // workgroups at most 4096, so that a batch's long contexts do not run on alone. Contexts
-// of up to 512 keys stay whole: the second launch costs what it saves. (Twice as many
-// chunks of a prompt's rows pay where contexts differ, 3 of 2000 to 8000: 146 us for
-// 197, and cost as much where they do not, 129 for 109; the lengths are the device's.)
+// of up to 512 keys stay whole, as the second launch costs what it saves or more (a
+// prompt of 512 rows: 19.4 us in two chunks, 15.8 whole). (Twice as many chunks of a
+// prompt's rows pay where contexts differ, 3 of 2000 to 8000: 146 us for 197, and cost as
+// much where they do not, 129 for 109; the lengths are the device's.)
 // The numbers are constants, not the device's: results and workspace do not depend on a
 // partition's size.
 ScaledPlan scaled_plan(int dtype, int32_t num_seqs, int32_t max_query_len, int32_t max_ctx,
@@ -338,17 +348,20 @@ ScaledPlan scaled_plan(int dtype, int32_t num_seqs, int32_t max_query_len, int32
   const int64_t rows = (int64_t)max_query_len * (num_heads / num_kv_heads);
   const bool two = dtype != VPA_DTYPE_F32 && head_dim <= 128;
   p.nq = two && rows > 16 ? 2 : 1;
-  p.split_keys = rows <= 256 ? 1 : 0;
+  const int64_t row_tiles = (rows + 16 * p.nq - 1) / (16 * p.nq);
+  const bool few = row_tiles * num_seqs * num_kv_heads < (max_ctx <= kWhole ? 1024 : 2048) ||
+                   (row_tiles == 1 && max_ctx > kWhole);
+  p.split_keys = rows <= 256 && max_ctx > 64 && few ? 1 : 0;
   p.lds_rows = p.split_keys ? (int32_t)(rows < 16 * p.nq ? rows : 16 * p.nq) : 0;
   const int64_t four = 64 * p.nq, over = (rows + four - 1) / four * four - rows;
-  const bool apart = p.nq == 2 && ((int64_t)max_query_len * 4 > max_ctx || over * 8 > rows);
+  const bool apart = over * 8 > rows || (p.nq == 2 && (int64_t)max_query_len * 4 > max_ctx);
   p.row_waves = p.split_keys || apart ? 1 : 4;
   const int64_t per = 16 * p.nq * p.row_waves;
   const int64_t tiles = (rows + per - 1) / per;
   p.tiles = (int32_t)tiles;
   const int64_t units = (int64_t)num_seqs * num_kv_heads * tiles;
   int64_t tokens = max_ctx;
-  if (!(p.split_keys && max_ctx <= kWhole)) {
+  if (max_ctx > kWhole) {
     const int64_t wanted = p.split_keys ? 256 : 2048 / p.row_waves;
     const int64_t chunks = units >= wanted ? 1
                            : p.split_keys  ? (wanted + units - 1) / units

@@ -270,6 +270,19 @@ def test_batches_of_many_short_contexts(device):
     Problem(device, 1, torch.bfloat16, 4, 2, 64, 16, rng.integers(0, 90, size=300)).check()
 
 
+@pytest.mark.parametrize("dtype,batch,hi,rows,causal", [
+    (torch.bfloat16, 700, 64, 0, True), (torch.float32, 700, 120, 0, True),
+    (torch.float16, 40, 500, 110, True), (torch.float32, 60, 64, 70, False),
+    (torch.bfloat16, 200, 130, 25, False)])
+def test_batches_whose_waves_have_rows_of_their_own(device, dtype, batch, hi, rows, causal):
+    """Short contexts of many sequences, whose keys are not split."""
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, hi + 1, size=batch)
+    lens[0] = hi
+    n = None if rows == 0 else rng.integers(0, rows + 1, size=batch)
+    Problem(device, 5, dtype, 4, 2, 64, 16, lens, rows=n, any_scale=True).check(causal)
+
+
 def test_more_rows_than_tokens(device):
     """The first rows see nothing and are zeros."""
     p = Problem(device, 2, torch.bfloat16, 4, 2, 64, 16, [5, 0, 20], rows=[12, 3, 20])
