@@ -47,7 +47,7 @@
 // tokens by its two launches and their dependent loads (8.0 us, 6.0 + 2.4 on their own);
 // rows of prompts by the issue of vector instructions, about 460 beside 64 matrix
 // instructions for 32 rows and 64 keys (512 rows each of 64 prompts of 560 to 1600 tokens:
-// 339 us, 708 TFLOP/s; matrix units busy 30 % of the time, vector issue 67 %). There the
+// 341 us, 704 TFLOP/s; matrix units busy 31 % of the time, vector issue 70 %). There the
 // next operands' bytes are converted between the matrix instructions (1 to 5 % of a
 // prompt's time); without any conversion the same call takes 12 % less, without
 // exponentials 7 %, without loads 5 %. Not kept: 8 waves that split the keys (97 us for the
