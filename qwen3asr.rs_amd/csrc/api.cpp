@@ -1346,9 +1346,9 @@ int vpa_paged_attention_block_scaled(
     return scaled_plan(dtype, num_seqs, max_query_len, max_context_len, total_query_rows,
                        num_heads, num_kv_heads, head_dim);
   }();
-  // (256-lane workgroups: a grid's lane count must fit in 32 bits; the joining launch
-  // has a workgroup per four rows)
-  if (p.grid <= 0 || p.grid > 0xffffff ||
+  // (workgroups of 256 lanes, or 64 with rows of their own: a grid's lane count must fit in
+  // 32 bits; the joining launch has a workgroup of 256 per four rows)
+  if (p.grid <= 0 || p.grid > (p.split_keys ? 0xffffff : 0x3ffffff) ||
       (p.max_chunks > 1 &&
        ((int64_t)max_query_len * num_heads + 3) / 4 > (int64_t)0xffffff / num_seqs))
     return fail(VPA_ERR_UNSUPPORTED,

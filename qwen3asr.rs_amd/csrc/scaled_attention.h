@@ -39,8 +39,8 @@
 //
 // Few rows (decode): the waves of a workgroup split a chunk's keys, 64 at a time,
 // and are joined in LDS; long contexts are split in chunks over workgroups and
-// joined by a second launch (scaled_merge_kernel). Many rows: every wave has its
-// own rows and all read the same keys, through L1 and L2.
+// joined by a second launch (scaled_merge_kernel). Many rows: a workgroup is one
+// wave with its own rows, and all of them read the same keys, through L1 and L2.
 //
 // Bounds, with 16 query and 8 kv heads of 128 dims: a decode of 256 sequences of 800 to
 // 4096 tokens by HBM (77 us, 5.3 TB/s; a read-only kernel reaches as much); one of 1500
@@ -106,7 +106,7 @@ __device__ __forceinline__ void alternate() {
   }
 }
 
-constexpr int kScaledWaves = 4;
+constexpr int kScaledWaves = 4;  // of a workgroup that splits the keys
 constexpr int kScaledKeys = 64;  // keys of a step
 constexpr float kScaledSlack = 8.f;
 constexpr int kScaledProbLog2 = 7;
@@ -156,20 +156,23 @@ struct ScaledDev {
   int32_t tiles, chunk_tokens, max_chunks;
   int32_t split_keys;  // the waves share 16 NQ rows and split the keys
   int32_t lds_rows;    // rows kept in LDS then
-  int32_t row_waves;   // waves of a workgroup with rows of their own (1: shared)
   float scale_log2, denom_eps;
 };
 
-// Query types and head dims whose waves may take two tiles of 16 rows.
+// Query types whose waves may take two tiles of 16 rows. (f32 queries' parts leave no
+// registers for a second one: 1000 rows of 8 prompts 200 us with one tile, 222 with two.)
 template <typename T>
-constexpr bool scaled_two_tiles(int head_dim) {
-  return !std::is_same_v<T, float> && head_dim <= 128;
+constexpr bool scaled_two_tiles() {
+  return !std::is_same_v<T, float>;
 }
 
-// Waves per SIMD: O, Q and two tiles' bytes are what a wave holds.
+// Waves per SIMD: O, Q and two tiles' bytes are what a wave holds. Two row tiles of head
+// dims 192 and 256 fill it alone, and share each conversion: 512 rows each of 32 prompts
+// of 1000 to 2000 tokens, head dim 256, 487 us, 714 with one tile. (Four row tiles of
+// head dim 128, alone too, are slower than two waves of two: 450 us for 340.)
 template <typename T, int D, int NQ>
 constexpr int scaled_waves_per_eu() {
-  return D <= 128 || (D == 192 && !std::is_same_v<T, float>) ? 2 : 1;
+  return D <= 128 || (D == 192 && NQ == 1 && !std::is_same_v<T, float>) ? 2 : 1;
 }
 
 template <typename T, int D, int BS, int NQ>
@@ -187,6 +190,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
   // way while S is computed and the next K during the softmax; otherwise V
   // during the softmax and the next K during P.V.
   constexpr bool kEarly = NQ == 1 && D <= 128;
+  constexpr bool kLate = NQ == 2 && D == 256;  // where half of V's have been used
 
   extern __shared__ float s_join[];
 
@@ -213,16 +217,15 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
   n = (int64_t)qa >= a.total_rows ? 0 : (int)min((int64_t)n, a.total_rows - (int64_t)qa);
   const int L = (int)min(a.context_lens[s], (uint32_t)a.max_ctx);
   const int rows = n * a.group;
-  const int wg_rows = a.row_waves * 16 * NQ;
-  if (qt * wg_rows >= rows) return;  // (uniform over the workgroup)
+  const int r0 = qt * 16 * NQ;
+  if (r0 >= rows) return;  // (uniform over the workgroup)
   const int nchunks = max(1, (L + a.chunk_tokens - 1) / a.chunk_tokens);
   if (chunk >= nchunks) return;
-  const int r0 = qt * wg_rows + (a.split_keys ? 0 : wave * 16 * NQ);
 
   // keys that some row of the wave sees, and the part of them here
   const int shift = L - n;
-  const int last_pos = (min(r0 + 16 * NQ, rows) - 1) / a.group;  // r0 may be past the rows
-  int n_keys = r0 >= rows ? 0 : a.causal ? min(L, last_pos + shift + 1) : L;
+  const int last_pos = (min(r0 + 16 * NQ, rows) - 1) / a.group;
+  int n_keys = a.causal ? min(L, last_pos + shift + 1) : L;
   n_keys = max(n_keys, 0);
   const int k_end = min(n_keys, (chunk + 1) * a.chunk_tokens);
   const int k_step = a.split_keys ? kScaledKeys * kScaledWaves : kScaledKeys;
@@ -612,9 +615,9 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
           }
         }
       }
-      if constexpr (!kEarly) {
-        // (past the end too, where the clamped ids read one block once more: a
-        // branch here costs the registers of a second copy of the bytes)
+      // (past the end too, where the clamped ids read one block once more: a branch here
+      // costs the registers of a second copy of the bytes)
+      if constexpr (!kEarly && !kLate) {
         __builtin_amdgcn_sched_barrier(0);
         load_k(ids1, kraw);
       }
@@ -623,6 +626,8 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kLate)
+          if (dt == DT / 2) load_k(ids1, kraw);
         if (dt + 1 < DT)
           fp8x16_times<f16_t>(vraw[dt + 1], vr[0], vr[NI - 1], vop[(dt + 1) % 2][0],
                               vop[(dt + 1) % 2][1]);
@@ -839,7 +844,7 @@ template <typename T, int D, int BS, int NQ>
 hipError_t launch_scaled_t(const ScaledDev& d, int64_t grid, hipStream_t stream) {
   const size_t lds = d.split_keys ? (size_t)kScaledWaves * d.lds_rows * (D + 2) * 4 : 0;
   hipLaunchKernelGGL((scaled_attention_kernel<T, D, BS, NQ>), dim3((unsigned)grid),
-                     dim3(64 * (d.split_keys ? kScaledWaves : d.row_waves)), lds, stream, d);
+                     dim3(d.split_keys ? 64 * kScaledWaves : 64), lds, stream, d);
   if (d.max_chunks > 1) {
     const int tiles = (int)(((int64_t)d.max_query_len * d.num_heads + 3) / 4);
     hipLaunchKernelGGL((scaled_merge_kernel<T, D>), dim3((unsigned)tiles * d.num_seqs), dim3(256),
@@ -850,7 +855,7 @@ hipError_t launch_scaled_t(const ScaledDev& d, int64_t grid, hipStream_t stream)
 
 template <typename T, int D, int BS>
 hipError_t launch_scaled_q(const ScaledDev& d, int64_t grid, int nq, hipStream_t stream) {
-  if constexpr (scaled_two_tiles<T>(D))
+  if constexpr (scaled_two_tiles<T>())
     if (nq == 2) return launch_scaled_t<T, D, BS, 2>(d, grid, stream);
   return launch_scaled_t<T, D, BS, 1>(d, grid, stream);
 }
@@ -889,7 +894,6 @@ hipError_t launch_scaled(const ScaledArgs& a, const CacheGeom& g, const ScaledPl
                     p.max_chunks,
                     p.split_keys,
                     p.lds_rows,
-                    p.row_waves,
                     a.scale * 1.4426950408889634f,
                     a.denom_eps};
 #define VPA_SCALED(DV, BV)                           \

@@ -324,15 +324,12 @@ hipError_t launch_scaled_append(int dtype, const ScaledAppendArgs& a, const Cach
 // one tile alone is always split (a decode). Contexts of one step of 64 keys have nothing
 // to split (256 of them: 17 us, 8), and more than 256 rows go without (8000 keys, 128
 // rows: 19 us split, 24 not; a batch of 64 with 1024 rows each keeps its waves busy).
-// Workgroups of waves with rows of their own are four, which find each other's keys in
-// the L1 cache (32 sequences of up to 4000 keys, 512 rows of head dim 192: 629 us, 718
-// one by one; a chunk of 512 rows over 6000 tokens: 54, 56), but one where there are two
-// tiles a wave and the rows of a workgroup end at different keys, as in a prompt's first
-// chunk (512 tokens: 20.4 and 19.4 us; 1000: 33.2 and 31.9), or where more than an eighth
-// of the fours' rows would be missing (64 times 400 rows, 12.5 waves each: 69 and 55 us).
-// Keys: chunks over workgroups until there is one workgroup of four waves (split keys)
-// or are two (a wave per rows, which finish at different times) per compute unit of an
-// MI355X, of at least 256 keys; where the waves split the keys and there are enough
+// Waves with rows of their own are a workgroup each: four to one end at different keys
+// and leave the last one's without rows (64 times 400 rows: 68 us for 53; 512 rows each
+// of 32 prompts, head dim 256: 548, 496; never more than 2 % faster).
+// Keys: chunks over workgroups until an MI355X has one of four waves (split keys) per
+// compute unit or two waves (with rows of their own, which finish at different times) per
+// SIMD, of at least 256 keys; where the waves split the keys and there are enough
 // workgroups at most 4096, so that a batch's long contexts do not run on alone. Contexts
 // of up to 512 keys stay whole, as the second launch costs what it saves or more (a
 // prompt of 512 rows: 19.4 us in two chunks, 15.8 whole). (Twice as many chunks of a
@@ -346,23 +343,17 @@ ScaledPlan scaled_plan(int dtype, int32_t num_seqs, int32_t max_query_len, int32
   constexpr int64_t kLeast = 256, kWhole = 512, kMost = 4096;
   ScaledPlan p{};
   const int64_t rows = (int64_t)max_query_len * (num_heads / num_kv_heads);
-  const bool two = dtype != VPA_DTYPE_F32 && head_dim <= 128;
-  p.nq = two && rows > 16 ? 2 : 1;
+  p.nq = dtype != VPA_DTYPE_F32 && rows > 16 ? 2 : 1;
   const int64_t row_tiles = (rows + 16 * p.nq - 1) / (16 * p.nq);
-  const bool few = row_tiles * num_seqs * num_kv_heads < (max_ctx <= kWhole ? 1024 : 2048) ||
+  const int64_t units = row_tiles * num_seqs * num_kv_heads;
+  const bool few = units < (max_ctx <= kWhole ? 1024 : 2048) ||
                    (row_tiles == 1 && max_ctx > kWhole);
   p.split_keys = rows <= 256 && max_ctx > 64 && few ? 1 : 0;
   p.lds_rows = p.split_keys ? (int32_t)(rows < 16 * p.nq ? rows : 16 * p.nq) : 0;
-  const int64_t four = 64 * p.nq, over = (rows + four - 1) / four * four - rows;
-  const bool apart = over * 8 > rows || (p.nq == 2 && (int64_t)max_query_len * 4 > max_ctx);
-  p.row_waves = p.split_keys || apart ? 1 : 4;
-  const int64_t per = 16 * p.nq * p.row_waves;
-  const int64_t tiles = (rows + per - 1) / per;
-  p.tiles = (int32_t)tiles;
-  const int64_t units = (int64_t)num_seqs * num_kv_heads * tiles;
+  p.tiles = (int32_t)row_tiles;
   int64_t tokens = max_ctx;
   if (max_ctx > kWhole) {
-    const int64_t wanted = p.split_keys ? 256 : 2048 / p.row_waves;
+    const int64_t wanted = p.split_keys ? 256 : 2048;
     const int64_t chunks = units >= wanted ? 1
                            : p.split_keys  ? (wanted + units - 1) / units
                                            : wanted / units;

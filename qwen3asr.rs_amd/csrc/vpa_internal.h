@@ -440,7 +440,6 @@ struct ScaledArgs {
 struct ScaledPlan {
   int32_t nq;  // 16-row tiles of a wave
   int32_t split_keys, lds_rows;
-  int32_t row_waves;  // waves of a workgroup with rows of their own
   int32_t tiles;  // row tiles of a (sequence, kv head)
   int32_t chunk_tokens, max_chunks;
   int64_t grid;  // workgroups
