@@ -818,7 +818,8 @@ int vpa_paged_attention_block_scaled(
  * vpa_decode_step_metadata go on as they are (their blocks are fresh); rows
  * give blocks back with vpa_release_shared_blocks in place of
  * vpa_release_blocks. A shared block is full for all its holders, so nobody
- * writes to it, unless a row is cut back (vpa_unshare_rows). Block 0 is not
+ * writes to it, unless a row is cut back (vpa_unshare_rows); vpa_evict_kv_cache,
+ * which rewrites a row's blocks, is not for rows that share any. Block 0 is not
  * counted. No counterparts in the reference, whose blocks have one owner.
  */
 

@@ -7,6 +7,7 @@ Hand-written HIP kernels for gfx950 behind the C ABI of ``include/vpa.h``
 
 from ._lib import VpaError  # noqa: F401
 from .ops import (  # noqa: F401
+    BlockBuffers,
     DecodeTokenState,
     DeviceBlockAllocator,
     argmax_token_ids_from_logits,
@@ -41,6 +42,7 @@ from .verify import verify_draft_tokens, verify_draft_tokens_workspace  # noqa: 
 
 __all__ = [
     "DecodeGraphCache",
+    "BlockBuffers",
     "DecodeTokenState",
     "DeviceBlockAllocator",
     "DeviceDecodeStep",

@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import contextlib
 from array import array
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -503,13 +503,25 @@ class DecodeTokenState:
             self.active_count.data_ptr(), self.batch, _stream(self.next_ids)))
 
 
-class _Pools:
-    """Addresses, strides and sizes of the blocks of ``buffers``, checked, in the host
-    arrays that ``vpa_copy_blocks`` reads."""
+class BlockBuffers:
+    """Tensors whose first dimension counts a pool's blocks (K, V and scales of every
+    layer), looked at once: the addresses, strides and sizes of their blocks in the host
+    arrays that ``vpa_copy_blocks`` reads. In place of the list of tensors in calls that
+    copy blocks, it spares each of them the checks (half a microsecond per tensor). It
+    holds the tensors, which keep their storage."""
 
-    def __init__(self, buffers: Sequence[torch.Tensor], blocks: int, device: int):
+    def __init__(self, buffers: Sequence[torch.Tensor], num_blocks: Optional[int] = None,
+                 device: Optional[int] = None):
         # (a hundred or more tensors per call: few calls for each)
-        self.blocks = blocks
+        self.tensors = buffers = tuple(buffers)
+        if device is None:
+            if not buffers:
+                raise _err("buffers are empty")
+            _require_device(*buffers)
+            device = buffers[0].get_device()
+        if num_blocks is None:
+            num_blocks = buffers[0].shape[0] if buffers and buffers[0].dim() else 0
+        self.blocks, self.device = blocks, device = num_blocks, device
         cls = torch.Tensor
         try:
             plain = all(map(cls.is_contiguous, buffers)) and \
@@ -548,6 +560,17 @@ class _Pools:
         self.count = len(base)
         self.base, self.stride, self.size = array("Q", base), array("q", stride), array("q", size)
 
+    @classmethod
+    def of(cls, buffers, num_blocks: Optional[int], device: int) -> "BlockBuffers":
+        """``buffers``, a list of tensors or one of these, for a pool of that many blocks
+        (None: as many as it has)."""
+        if not isinstance(buffers, cls):
+            return cls(buffers, num_blocks, device)
+        if buffers.device != device or num_blocks not in (None, buffers.blocks):
+            raise _err(f"buffers of {buffers.blocks} blocks on cuda:{buffers.device} for a pool "
+                       f"of {num_blocks} on cuda:{device}")
+        return buffers
+
     def copy(self, src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
              num_pairs: Optional[torch.Tensor]) -> None:
         """The copies of contiguous u32 pairs, on the current device and stream."""
@@ -557,6 +580,9 @@ class _Pools:
             self.base.buffer_info()[0], self.stride.buffer_info()[0], self.size.buffer_info()[0],
             self.count, src_blocks.data_ptr(), dst_blocks.data_ptr(), _ptr(num_pairs),
             src_blocks.numel(), self.blocks, _stream(src_blocks)))
+
+
+Buffers = Union[Sequence[torch.Tensor], BlockBuffers]
 
 
 def _fork_map(batch: int, src_rows: torch.Tensor, dst_rows: torch.Tensor,
@@ -579,7 +605,9 @@ class DeviceBlockAllocator:
 
     Rows may share blocks once ``fork`` has been called (or ``enable_sharing``, which
     has to come before a graph with ``release`` or ``trim`` in it is captured):
-    ``shared`` then counts the rows that hold each block besides the first."""
+    ``shared`` then counts the rows that hold each block besides the first. What
+    rewrites a row's blocks in place (``evict_kv_cache``) is not for rows that share
+    any. ``buffers`` are lists of tensors, or ``BlockBuffers`` made of one once."""
 
     def __init__(self, num_blocks: int, block_size: int, batch: int, cols: int, device):
         import numpy as np
@@ -632,7 +660,7 @@ class DeviceBlockAllocator:
                                       device=self.block_tables.device).view(torch.uint32)
 
     def fork(self, src_rows: torch.Tensor, dst_rows: torch.Tensor,
-             buffers: Sequence[torch.Tensor]) -> torch.Tensor:
+             buffers: Buffers) -> torch.Tensor:
         """Row dst_rows[f], which holds no blocks, becomes a copy of row src_rows[f] (u32
         [F], F <= 1024): the blocks that are full are shared, a partly filled one is
         copied in every one of ``buffers`` (the caches, and scales, of all layers;
@@ -661,7 +689,7 @@ class DeviceBlockAllocator:
             pools.copy(src, dst, count)
         return ok
 
-    def compact(self, buffers: Sequence[torch.Tensor]
+    def compact(self, buffers: Buffers
                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Brings the n blocks in use to ids 1 .. n: moves them in every one of
         ``buffers`` (the caches, and scales, of all layers) and rewrites the tables and
@@ -684,15 +712,15 @@ class DeviceBlockAllocator:
             pools.copy(src, dst, count)
         return src, dst, count
 
-    def _pools(self, buffers: Sequence[torch.Tensor]):
-        return _Pools(buffers, self.ring_capacity, self.block_tables.get_device())
+    def _pools(self, buffers: Buffers) -> BlockBuffers:
+        return BlockBuffers.of(buffers, self.ring_capacity, self.block_tables.get_device())
 
     def _pairs(self, n: int):
         """Room for n pairs of copied blocks and their number."""
         return tuple(self.row_blocks.new_empty((m,)) for m in (n, n, 1))
 
     def trim(self, num_tokens: torch.Tensor, slot_mapping: Optional[torch.Tensor] = None,
-             buffers: Optional[Sequence[torch.Tensor]] = None) -> None:
+             buffers: Optional[Buffers] = None) -> None:
         """Rows hold num_tokens[r] tokens from here on (u32 [batch], at most what
         they held): the next step appends there, and the blocks past them go
         back (trim_request_to_num_tokens, paged_cache_runtime.rs:320-340). For rows

@@ -123,7 +123,7 @@ class DeviceDecodeStep:
         self.tokens.select(logits)
 
     def fork(self, src_rows: torch.Tensor, dst_rows: torch.Tensor,
-             buffers: Sequence[torch.Tensor]) -> torch.Tensor:
+             buffers: ops.Buffers) -> torch.Tensor:
         """Between two steps: rows dst_rows[f], which hold no blocks, go on from what rows
         src_rows[f] hold and have generated (``DeviceBlockAllocator.fork``, over the
         caches and scales of all layers). Returns ok u8; a row that is not ok is left as

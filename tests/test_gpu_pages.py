@@ -312,6 +312,30 @@ def test_copy_without_pairs_or_buffers(device):
     assert torch.equal(b, torch.arange(12, device=device, dtype=torch.float32).view(3, 4))
 
 
+def test_buffers_looked_at_once(device):
+    """BlockBuffers in place of the tensors: the same copies, and refused for another pool."""
+    b = Both(device, 40, 8, 6, 6)
+    tensors = b.buffers
+    once = vpa.BlockBuffers(tensors)
+    b.shuffle()
+    b.allocate([21, 30, 0, 0, 0, 0])
+    b.buffers = once
+    b.fork([0, 1, 0], [2, 3, 4])
+    b.release([99, 0, 99, 99, 99, 99])
+    b.trim([21, 0, 10, 30, 21, 0])
+    b.compact()
+    b.buffers = tensors
+    b.check()
+    vpa.copy_blocks(once, u32([1], device), u32([39], device))
+    assert all(torch.equal(t[1], t[39]) for t in tensors)
+    with pytest.raises(vpa.VpaError, match="40 blocks"):
+        vpa.DeviceBlockAllocator(41, 8, 2, 2, device).compact(once)
+    for bad, match in (([], "empty"), ([torch.zeros(3)], "GPU only"),
+                       ([tensors[0], torch.zeros((41, 2), device=device)], "pools of 40")):
+        with pytest.raises(vpa.VpaError, match=match):
+            vpa.BlockBuffers(bad)
+
+
 def test_refusals(device):
     a = vpa.DeviceBlockAllocator(10, 16, 4, 3, device)
     b = torch.zeros((10, 4), device=device)
