@@ -456,7 +456,7 @@ hipError_t launch_scaled_attention_f32(const ScaledArgs& a, const CacheGeom& g,
                                        const ScaledPlan& p, hipStream_t stream);
 
 // Pages (page_kernels.hip).
-constexpr int kCopyMaxBuffers = 96;  // of one launch
+constexpr int kCopyMaxBuffers = 192;  // of one launch, whose arguments end at 4 KiB
 struct CopyBuffers {
   char* base[kCopyMaxBuffers];
   int64_t stride[kCopyMaxBuffers];  // bytes between blocks

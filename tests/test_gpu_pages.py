@@ -312,6 +312,18 @@ def test_copy_without_pairs_or_buffers(device):
     assert torch.equal(b, torch.arange(12, device=device, dtype=torch.float32).view(3, 4))
 
 
+@pytest.mark.parametrize("n", [1, 191, 192, 193, 400])
+def test_any_number_of_buffers(device, n):
+    """More than a launch takes, of sizes in vectors, words and bytes."""
+    rng = np.random.default_rng(n)
+    host = [rng.integers(0, 255, (6, (16, 4, 3)[k % 3] * (1 + k % 5)), dtype=np.uint8) for k in range(n)]
+    bufs = [torch.from_numpy(h).to(device) for h in host]
+    vpa.copy_blocks(bufs, u32([1, 4], device), u32([5, 2], device))
+    for h, b in zip(host, bufs):
+        h[5], h[2] = h[1], h[4]
+        assert np.array_equal(b.cpu().numpy(), h)
+
+
 def test_buffers_looked_at_once(device):
     """BlockBuffers in place of the tensors: the same copies, and refused for another pool."""
     b = Both(device, 40, 8, 6, 6)
