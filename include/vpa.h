@@ -791,7 +791,10 @@ size_t vpa_paged_attention_block_scaled_workspace_size(int32_t num_seqs, int32_t
  * n_s for its r-th row. A row that sees none is zeros; block ids >= num_blocks
  * are absent. vpa_paged_attention adds a denom_eps of 1e-6,
  * vpa_chunked_prefill_paged_attention the caller's. Scales may be any finite
- * numbers, not only powers of two.
+ * numbers, not only powers of two; those of blocks that a row does not see have
+ * no part in its result. Of those it sees, a token counts as long as p_t
+ * value_scales is above 2^-27 of the largest (probabilities are 16-bit numbers,
+ * for f32 queries pairs of them).
  * Any number of query heads per kv head, head_dim 64, 96, 128, 192 or 256,
  * block_size 8, 16 or 32. n_s and L_s are clamped to max_query_len and
  * max_context_len, which size the grid; rows at or past total_query_rows are

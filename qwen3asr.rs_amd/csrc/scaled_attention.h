@@ -9,11 +9,13 @@
 // over the tokens the row sees. Scales that are powers of two, as the append
 // makes them, cost nothing: the conversion of the bytes for the matrix
 // instructions takes a power of two along, here a block's scale over the largest
-// of the step's (K) or of those met so far (V: `vref`), so that no operand passes
+// of the step's (K) or of those met so far (V: `vrow`), so that no operand passes
 // 448; that largest one is part of the softmax scale and of the output. Every
 // product is exact as long as the ratio is at least 2^-5 (E4M3's least number,
 // 2^-9, stays normal in f16). Steps with smaller ratios or other scales multiply
-// the f32 scores and probabilities instead.
+// the f32 scores and probabilities instead. V's reference is a row's own, at most 2^5
+// above the largest scale that it sees: blocks that it does not see, louder by any factor,
+// do not push its weights p_t vs_t / vrow out of f16's range.
 //
 // Work of a wave: 16 NQ rows (a row is a position and a query head of the kv
 // head; heads fastest, so any group size fills the rows) over 64 keys at a time
@@ -34,7 +36,7 @@
 // values (22 bits), and three bf16 values for Q, which hold an f32 exactly. The
 // probabilities stay below 2^kSlack (the reference maximum moves only when it is
 // exceeded by more) and are scaled by 2^kProbLog2, which keeps f16's smallest
-// step at 2^-31 of a probability of 1. Like the maximum, vref moving rescales the
+// step at 2^-31 of a probability of 1. Like the maximum, vrow moving rescales the
 // sums.
 //
 // Few rows (decode): the waves of a workgroup split a chunk's keys, 64 at a time,
@@ -110,6 +112,9 @@ constexpr int kScaledWaves = 4;  // of a workgroup that splits the keys
 constexpr int kScaledKeys = 64;  // keys of a step
 constexpr float kScaledSlack = 8.f;
 constexpr int kScaledProbLog2 = 7;
+// How far above a row's own the wave's reference of V's scales may be taken for it: what the
+// conversion takes along exactly.
+constexpr float kScaledReach = 32.f;
 
 // Maximum / sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_rows(float v) {
@@ -170,14 +175,15 @@ constexpr bool scaled_two_tiles() {
 // dims 192 and 256 fill it alone, and share each conversion: 512 rows each of 32 prompts
 // of 1000 to 2000 tokens, head dim 256, 487 us, 714 with one tile. (Four row tiles of
 // head dim 128, alone too, are slower than two waves of two: 450 us for 340.)
-template <typename T, int D, int NQ>
+template <typename T, int D, int BS, int NQ>
 constexpr int scaled_waves_per_eu() {
+  if (D == 64 && NQ == 2 && BS > 8) return 3;  // (168 registers)
   return D <= 128 || (D == 192 && NQ == 1 && !std::is_same_v<T, float>) ? 2 : 1;
 }
 
 template <typename T, int D, int BS, int NQ>
 __global__ __launch_bounds__(64 * kScaledWaves)
-__attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scaled_attention_kernel(
+__attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, BS, NQ>()))) void scaled_attention_kernel(
     const ScaledDev a) {
   constexpr bool kF32 = std::is_same_v<T, float>;
   using K = std::conditional_t<std::is_same_v<T, f16_t>, f16_t, bf16_t>;  // of S's operands
@@ -234,7 +240,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
   const int all_see = a.causal ? r0 / a.group + shift : L - 1;
 
   int limit[NQ];  // last key of this lane's rows (the lane's column of S^T)
-  int64_t orow[NQ];  // their row of `out`, -1: none
+  int64_t orow[NQ];  // their row of `out`
   uint4 qop[NQ][QP][2 * NC];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
@@ -242,7 +248,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
     const bool ok = r < rows;
     const int pos = ok ? r / a.group : 0;
     const int64_t row = ((int64_t)qa + pos) * a.num_heads + (int64_t)j * a.group + (ok ? r % a.group : 0);
-    orow[q] = ok ? row : -1;
+    orow[q] = row;
     limit[q] = !ok ? -1 : a.causal ? pos + shift : L - 1;
     const T* src = static_cast<const T*>(a.query) + row * D;
 #pragma unroll
@@ -286,7 +292,14 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[q][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  float vref = 1.50463277e-36f;  // 2^-119 (vref over 2^kScaledProbLog2 is a normal number)
+  // V's reference: the largest scale of all that the wave's steps held or, for a row whose own
+  // do not reach that far (kScaledReach), the largest that it has seen. Rows of a wave differ
+  // in it only where the wave is `apart`.
+  float vrow[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) vrow[q] = 1.50463277e-36f;  // 2^-119 (over 2^kScaledProbLog2 normal)
+  constexpr int kApart = 1, kNan = 2;
+  int state = 0;  // (uniform)
 
   if (k_first < k_end) {
     const uint32_t* bt = a.block_tables + (int64_t)s * a.block_table_stride;
@@ -364,6 +377,17 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
       }
     };
 
+    // x of tile b's tokens, the second of its blocks where `second`. (Both lanes are read by
+    // the whole wave: under a branch of some lanes the one read might not be written.)
+    auto of_tile = [](const float(&x)[NI], int b, bool second) {
+      const float lo = readlane_f(x[0], 16 * b);
+      if constexpr (NI == 2) {
+        const float hi = readlane_f(x[1], 16 * b);
+        return second ? hi : lo;
+      }
+      return lo;
+    };
+
     // Bytes of tokens past the context or in an absent block are stale, NaN among
     // them, and 0 * NaN is NaN: zeros.
     struct Keep {
@@ -385,8 +409,6 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
     auto nan_bytes = [](uint32_t x) {
       return (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
     };
-    bool nan_seen = false;
-
     uint4 kraw[4][NC], vraw[DT];
     Ids ids = load_ids(k_first), ids1 = load_ids(k_first + k_step);
     Scales sc = load_scales(ids);
@@ -429,11 +451,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 
       // ---- S^T, 64 dims of a tile at a time, the next ones' bytes converted meanwhile ----
       f32x4_t sv[NQ][4];
-      auto tile_ratio = [&](int b) {
-        float krb = readlane_f(kr[0], 16 * b);
-        if constexpr (NI == 2) krb = c16 < 8 ? krb : readlane_f(kr[1], 16 * b);
-        return krb;
-      };
+      auto tile_ratio = [&](int b) { return of_tile(kr, b, c16 >= 8); };
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -473,9 +491,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         asm volatile("" ::: "memory");  // (a branch, not selects)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          float ksb = readlane_f(sc.k[0], 16 * b);
-          if constexpr (NI == 2) ksb = kg < 2 ? ksb : readlane_f(sc.k[1], 16 * b);
-          ksb *= a.scale_log2;
+          const float ksb = of_tile(sc.k, b, kg >= 2) * a.scale_log2;
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -520,28 +536,49 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
         mt[q] = fmaxf(mt[q], mx[q]);
         move = move || mx[q] > m[q] + kScaledSlack;  // (m is -inf before the first key)
       }
-      bool vmore = fabsf(sc.v[0]) > vref;
-      if constexpr (NI == 2) vmore = vmore || fabsf(sc.v[1]) > vref;
+      // (a row that is apart sees nothing of the steps to come: it may look in vain)
+      bool vmore = fabsf(sc.v[0]) > vrow[0];
+      if constexpr (NI == 2) vmore = vmore || fabsf(sc.v[1]) > vrow[0];
       if (__ballot(move || vmore) != 0) {
-        const float vnew = fmaxf(vref, largest(sc.v));
-        const float fv = vref / vnew;
-        vref = vnew;
+        float fix[NQ];
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
           const float mn = fmaxf(m[q], max_rows(mx[q]));
-          const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mn);
+          fix[q] = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mn);
           m[q] = mn;
-          lsum[q] *= f;
+          lsum[q] *= fix[q];
+        }
+        if (__ballot(vmore) != 0) {
+          float vref = fmaxf(fabsf(sc.v[0]), fabsf(sc.v[NI - 1]));
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) vref = fmaxf(vref, vrow[q]);
+          vref = wave_max_dpp(vref);
+          bool off = false;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            float seen = k0 + 16 * kg <= limit[q] ? fabsf(sc.v[0]) : 0.f;
+            if constexpr (NI == 2)
+              seen = fmaxf(seen, k0 + 16 * kg + 8 <= limit[q] ? fabsf(sc.v[1]) : 0.f);
+            seen = fmaxf(vrow[q], max_rows(seen));
+            // (a row that sees nothing at all takes any)
+            const float to = limit[q] < k_first || seen * kScaledReach >= vref ? vref : seen;
+            fix[q] *= vrow[q] / to;
+            vrow[q] = to;
+            off = off || to != vref;
+          }
+          state = (state & kNan) | (__ballot(off) != 0 ? kApart : 0);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[q][dt][r] *= f * fv;
-        }
+            for (int r = 0; r < 4; ++r) o[q][dt][r] *= fix[q];
       }
-      const bool vfast = all_plain(sc.v, vref);
+      const bool vfast = all_plain(sc.v, vrow[0]) && (state & kApart) == 0;
       float vr[NI];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) vr[i] = vfast ? ratio(sc.v[i], vref) : 1.f;
+      for (int i = 0; i < NI; ++i) vr[i] = vfast ? ratio(sc.v[i], vrow[0]) : 1.f;
 
       // ---- probabilities, as operands of P.V ----
       uint32_t pw[NQ][PP][2][4];  // [two tokens of a tile's four][tile]
@@ -557,17 +594,19 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
           }
       }
       if (!vfast) {
-        float over = vref;
-        asm volatile("" : "+v"(over));  // (a branch, and nothing of it before)
+        asm volatile("" ::: "memory");  // (a branch, and nothing of it before)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          float f = readlane_f(sc.v[0], 16 * b);
-          if constexpr (NI == 2) f = kg < 2 ? f : readlane_f(sc.v[1], 16 * b);
-          f /= over;
+        for (int q = 0; q < NQ; ++q) {
+          const float over = 1.f / vrow[q];
 #pragma unroll
-          for (int q = 0; q < NQ; ++q)
+          for (int b = 0; b < 4; ++b) {
+            // (of a block that the row does not see: perhaps infinite, times 0)
+            const int t0 = k0 + 16 * b + (NI == 2 ? 8 * (kg / 2) : 0);
+            const float vs = of_tile(sc.v, b, kg >= 2);
+            const float f = t0 <= limit[q] ? vs * over : 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) sv[q][b][r] *= f;
+          }
         }
       }
 #pragma unroll
@@ -604,7 +643,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
                  nan_bytes(vraw[dt].w);
         }
         if (a.causal && __ballot(any != 0) != 0) {
-          nan_seen = true;
+          state |= kNan;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             __builtin_amdgcn_sched_barrier(0);
@@ -651,7 +690,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
 
     // NaN values of the steps that not every row sees whole: a row gets a NaN in
     // each dim where a token it sees has one, by a product of flags.
-    if (nan_seen) {
+    if ((state & kNan) != 0) {
       for (int k0 = k_first; k0 < k_end; k0 += k_step) {
         if (k0 + kScaledKeys - 1 <= all_see) continue;
         ids = load_ids(k0);
@@ -702,7 +741,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
     const float f = m[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[q] - mt[q]);
     const float f1 = f * (1.f / (1 << kScaledProbLog2));
     lsum[q] = sum_rows(lsum[q]) * f1;
-    fo[q] = f1 * vref;
+    fo[q] = f1 * vrow[q];
   }
   const bool single = nchunks == 1;
   T* out = static_cast<T*>(a.out);
@@ -722,10 +761,13 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, NQ>()))) void scale
       if (d == 0) *reinterpret_cast<float2*>(a.part_stat + 2 * at) = make_float2(mx, sum);
     }
   };
-  if (!a.split_keys) {
+  // (compared here: kept from above, each would hold a pair of registers over the loop)
+  int split = a.split_keys, end = rows;
+  asm volatile("" : "+s"(split), "+s"(end));
+  if (split == 0) {
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      if (orow[q] < 0) continue;
+      if (r0 + 16 * q + c16 >= end) continue;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const float v[4] = {o[q][dt][0] * fo[q], o[q][dt][1] * fo[q], o[q][dt][2] * fo[q],
