@@ -688,11 +688,11 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, BS, NQ>()))) void s
       sc = sc1;
     }
 
-    // NaN values of the steps that not every row sees whole: a row gets a NaN in
-    // each dim where a token it sees has one, by a product of flags.
+    // NaN values, which the steps that were not full left out (masked rows, the context's
+    // end, an absent block; the other steps' come out the same): a row gets a NaN in each
+    // dim where a token it sees has one, by a product of flags.
     if ((state & kNan) != 0) {
       for (int k0 = k_first; k0 < k_end; k0 += k_step) {
-        if (k0 + kScaledKeys - 1 <= all_see) continue;
         ids = load_ids(k0);
         load_v(ids, vraw);
         const Keep keep = keep_of(ids, k0);
