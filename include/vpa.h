@@ -873,12 +873,15 @@ int vpa_release_shared_blocks(uint32_t* block_tables, int32_t block_table_stride
                               int32_t num_rows, void* stream);
 
 /*
- * unshare_rows - every row whose next token (positions[r]) falls inside a block
- * that others hold too takes a fresh block from the ring in its place, in index
+ * unshare_rows - every block that a row would write to and that others hold too,
+ * its next token's (number positions[r] / block_size) and those the row holds
+ * behind it, is replaced by a fresh one from the ring, rows and blocks in index
  * order; the last holder keeps the block. Needed after a row was cut back to
  * fewer tokens than it shares, before it is appended to. ok[r] = 0 for a row the
  * ring cannot serve, which must not be appended to; 1 otherwise. Pairs
- * copy_src / copy_dst [num_rows] and *copy_count as in vpa_fork_rows.
+ * copy_src / copy_dst [num_rows] and *copy_count, as in vpa_fork_rows, of the
+ * replaced blocks that hold some of the row's tokens (where positions[r] is
+ * inside a block).
  */
 int vpa_unshare_rows(uint32_t* block_tables, int32_t block_table_stride, uint32_t* row_blocks,
                      const uint32_t* positions, uint32_t* shared, int64_t num_blocks,

@@ -325,24 +325,26 @@ __global__ __launch_bounds__(kPageThreads) void release_shared_kernel(
 
 // ---- copies before a write --------------------------------------------------
 
-// Rows, in order, whose next token falls into a block that others hold too take a
-// fresh one and have the old one's contents copied. Such rows are rare (a row cut
-// back below the length it was forked at): found by all lanes, taken one by one.
+// Rows, in order, replace each block that they would write to and that others hold too:
+// the one that their next token falls into, whose contents are copied, and those they
+// still hold behind it. Such rows are rare (a row cut back below the length it was
+// forked at): found by all lanes, taken one by one.
 __global__ __launch_bounds__(kPageThreads) void unshare_rows_kernel(
     const PageState s, uint8_t* __restrict__ ok, uint32_t* __restrict__ copy_src,
     uint32_t* __restrict__ copy_dst, uint32_t* __restrict__ copy_count) {
   __shared__ uint32_t s_tmp[kPageThreads / 64];
   __shared__ uint32_t s_rows[kPageThreads];
   uint32_t head = s.ring_state[0], avail = s.ring_state[1], copies = 0;
+  auto shared_block = [&](uint32_t id) {
+    return id != 0 && (int64_t)id < s.num_blocks && s.shared[id] != 0;
+  };
   for (int base = 0; base < s.num_rows; base += kPageThreads) {
     const int r = base + threadIdx.x;
     bool want = false;
     if (r < s.num_rows) {
-      const uint32_t pos = s.positions[r], at = pos / (uint32_t)s.block_size;
-      if (pos % (uint32_t)s.block_size != 0 && at < min(s.row_blocks[r], (uint32_t)s.cols)) {
-        const uint32_t id = s.block_tables[(int64_t)r * s.cols + at];
-        want = id != 0 && (int64_t)id < s.num_blocks && s.shared[id] != 0;
-      }
+      const uint32_t have = min(s.row_blocks[r], (uint32_t)s.cols);
+      for (uint32_t at = s.positions[r] / (uint32_t)s.block_size; at < have && !want; ++at)
+        want = shared_block(s.block_tables[(int64_t)r * s.cols + at]);
       ok[r] = 1;
     }
     uint32_t total;
@@ -351,22 +353,28 @@ __global__ __launch_bounds__(kPageThreads) void unshare_rows_kernel(
     __syncthreads();
     if (threadIdx.x == 0) {
       for (uint32_t k = 0; k < total; ++k) {
-        const uint32_t row = s_rows[k], at = s.positions[row] / (uint32_t)s.block_size;
-        uint32_t* entry = &s.block_tables[(int64_t)row * s.cols + at];
-        const uint32_t id = *entry;
-        if (s.shared[id] == 0) continue;  // the rows before it have all taken copies
-        if (avail == 0) {
-          ok[row] = 0;
-          continue;
+        const uint32_t row = s_rows[k], pos = s.positions[row];
+        const uint32_t first = pos / (uint32_t)s.block_size;
+        const uint32_t have = min(s.row_blocks[row], (uint32_t)s.cols);
+        for (uint32_t at = first; at < have; ++at) {
+          uint32_t* entry = &s.block_tables[(int64_t)row * s.cols + at];
+          const uint32_t id = *entry;
+          if (!shared_block(id)) continue;  // (or the rows before it have all taken copies)
+          if (avail == 0) {
+            ok[row] = 0;
+            break;
+          }
+          const uint32_t fresh = s.ring[head % (uint32_t)s.ring_cap];
+          head = (head + 1) % (uint32_t)s.ring_cap;
+          --avail;
+          s.shared[id] -= 1;
+          *entry = fresh;
+          if (at == first && pos % (uint32_t)s.block_size != 0) {
+            copy_src[copies] = id;
+            copy_dst[copies] = fresh;
+            ++copies;
+          }
         }
-        const uint32_t fresh = s.ring[head % (uint32_t)s.ring_cap];
-        head = (head + 1) % (uint32_t)s.ring_cap;
-        --avail;
-        s.shared[id] -= 1;
-        *entry = fresh;
-        copy_src[copies] = id;
-        copy_dst[copies] = fresh;
-        ++copies;
       }
     }
     __syncthreads();
