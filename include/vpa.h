@@ -817,10 +817,10 @@ int vpa_paged_attention_block_scaled(
  * Blocks that several rows of the device block allocator hold (its state:
  * vpa_allocate_rows), with one more array:
  *   shared [num_blocks] u32   rows that hold a block besides the first
- * all zeros before the first fork. vpa_allocate_rows and
- * vpa_decode_step_metadata go on as they are (their blocks are fresh); rows
- * give blocks back with vpa_release_shared_blocks in place of
- * vpa_release_blocks. A shared block is full for all its holders, so nobody
+ * all zeros before the first fork. vpa_allocate_rows goes on as it is (its
+ * blocks are fresh); rows step with vpa_decode_step_metadata_shared and give
+ * blocks back with vpa_release_shared_blocks in place of
+ * vpa_decode_step_metadata and vpa_release_blocks. A shared block is full for all its holders, so nobody
  * writes to it, unless a row is cut back (vpa_unshare_rows); vpa_evict_kv_cache,
  * which rewrites a row's blocks, is not for rows that share any. Block 0 is not
  * counted. No counterparts in the reference, whose blocks have one owner.
@@ -859,6 +859,22 @@ int vpa_fork_rows(uint32_t* block_tables, int32_t block_table_stride, uint32_t* 
                   uint8_t* ok, uint32_t* copy_src, uint32_t* copy_dst, uint32_t* copy_count,
                   uint32_t* free_ring, uint32_t* free_ring_state, int32_t free_ring_capacity,
                   int32_t block_size, int32_t num_rows, void* stream);
+
+/*
+ * decode_step_metadata_shared - vpa_decode_step_metadata where blocks may have
+ * several holders: a row whose next token falls into a block that others hold
+ * too (one cut back that vpa_unshare_rows could not serve, or was not called
+ * for) stalls, like one without a block left, and goes on once the block is its
+ * own.
+ */
+int vpa_decode_step_metadata_shared(uint32_t* block_tables, int32_t block_table_stride,
+                                    uint32_t* row_blocks, uint32_t* positions,
+                                    const uint32_t* shared, int64_t num_blocks,
+                                    const uint8_t* finished, uint32_t* free_ring,
+                                    uint32_t* free_ring_state, int32_t free_ring_capacity,
+                                    int32_t block_size, int64_t* slot_mapping,
+                                    uint32_t* context_lens, uint32_t* status, int32_t num_rows,
+                                    void* stream);
 
 /*
  * release_shared_blocks - vpa_release_blocks where blocks may have several

@@ -835,14 +835,13 @@ int vpa_allocate_rows(uint32_t* block_tables, int32_t block_table_stride, uint32
                                              static_cast<hipStream_t>(stream)));
 }
 
-int vpa_decode_step_metadata(uint32_t* block_tables, int32_t block_table_stride,
-                             uint32_t* row_blocks, uint32_t* positions, const uint8_t* finished,
-                             uint32_t* free_ring, uint32_t* free_ring_state,
-                             int32_t free_ring_capacity, int32_t block_size,
-                             int64_t* slot_mapping, uint32_t* context_lens, uint32_t* status,
-                             int32_t num_rows, void* stream) {
-  clear_error();
-  const char* op = "decode_step_metadata";
+namespace {
+int decode_step(const char* op, uint32_t* block_tables, int32_t block_table_stride,
+                uint32_t* row_blocks, uint32_t* positions, const uint8_t* finished,
+                const uint32_t* shared, int64_t num_blocks, uint32_t* free_ring,
+                uint32_t* free_ring_state, int32_t free_ring_capacity, int32_t block_size,
+                int64_t* slot_mapping, uint32_t* context_lens, uint32_t* status,
+                int32_t num_rows, void* stream) {
   int rc = check_alloc_state(op, block_tables, block_table_stride, row_blocks, free_ring,
                              free_ring_state, free_ring_capacity, num_rows);
   if (rc != VPA_OK) return rc;
@@ -854,8 +853,39 @@ int vpa_decode_step_metadata(uint32_t* block_tables, int32_t block_table_stride,
   return hip_status(op, launch_decode_step_metadata(
                             block_tables, block_table_stride, row_blocks, positions, finished,
                             free_ring, free_ring_state, free_ring_capacity, block_size,
-                            slot_mapping, context_lens, status, num_rows,
+                            slot_mapping, context_lens, status, num_rows, shared, num_blocks,
                             static_cast<hipStream_t>(stream)));
+}
+}  // namespace
+
+int vpa_decode_step_metadata(uint32_t* block_tables, int32_t block_table_stride,
+                             uint32_t* row_blocks, uint32_t* positions, const uint8_t* finished,
+                             uint32_t* free_ring, uint32_t* free_ring_state,
+                             int32_t free_ring_capacity, int32_t block_size,
+                             int64_t* slot_mapping, uint32_t* context_lens, uint32_t* status,
+                             int32_t num_rows, void* stream) {
+  clear_error();
+  return decode_step("decode_step_metadata", block_tables, block_table_stride, row_blocks,
+                     positions, finished, nullptr, 0, free_ring, free_ring_state,
+                     free_ring_capacity, block_size, slot_mapping, context_lens, status, num_rows,
+                     stream);
+}
+
+int vpa_decode_step_metadata_shared(uint32_t* block_tables, int32_t block_table_stride,
+                                    uint32_t* row_blocks, uint32_t* positions,
+                                    const uint32_t* shared, int64_t num_blocks,
+                                    const uint8_t* finished, uint32_t* free_ring,
+                                    uint32_t* free_ring_state, int32_t free_ring_capacity,
+                                    int32_t block_size, int64_t* slot_mapping,
+                                    uint32_t* context_lens, uint32_t* status, int32_t num_rows,
+                                    void* stream) {
+  clear_error();
+  const char* op = "decode_step_metadata_shared";
+  if (shared == nullptr) return fail(VPA_ERR_INVALID_ARGUMENT, "%s: shared must be non-null", op);
+  if (num_blocks <= 0) return fail(VPA_ERR_INVALID_ARGUMENT, "%s: num_blocks must be > 0", op);
+  return decode_step(op, block_tables, block_table_stride, row_blocks, positions, finished, shared,
+                     num_blocks, free_ring, free_ring_state, free_ring_capacity, block_size,
+                     slot_mapping, context_lens, status, num_rows, stream);
 }
 
 int vpa_release_blocks(const uint32_t* block_tables, int32_t block_table_stride,

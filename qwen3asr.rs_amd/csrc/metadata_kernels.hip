@@ -60,12 +60,17 @@ __device__ __forceinline__ uint32_t block_exclusive_scan(uint32_t v, uint32_t* s
   return r;
 }
 
+// kShared: with rows that may share blocks (shared[b]: holders of block b besides the
+// first) a row whose next token falls into a block that others hold too stalls; one more
+// dependent load, which rows of their own do without.
+template <bool kShared>
 __global__ __launch_bounds__(kMetaThreads) void decode_step_metadata_kernel(
     uint32_t* __restrict__ block_tables, int32_t cols, uint32_t* __restrict__ row_blocks,
     uint32_t* __restrict__ positions, const uint8_t* __restrict__ finished,
     uint32_t* __restrict__ ring, uint32_t* __restrict__ ring_state, int32_t ring_cap,
     int32_t block_size, int64_t* __restrict__ slot_mapping, uint32_t* __restrict__ context_lens,
-    uint32_t* __restrict__ status, int32_t num_rows) {
+    uint32_t* __restrict__ status, int32_t num_rows, const uint32_t* __restrict__ shared,
+    int64_t num_blocks) {
   __shared__ uint32_t s_tmp[kMetaThreads / 64 + 1];
   const int tid = threadIdx.x;
   const uint32_t head = ring_state[0];
@@ -104,9 +109,12 @@ __global__ __launch_bounds__(kMetaThreads) void decode_step_metadata_kernel(
             ok = false;
           }
         }
+        const uint32_t bi = pos / (uint32_t)block_size;
+        const uint32_t blk = ok ? block_tables[(int64_t)r * cols + bi] : 0u;
+        if constexpr (kShared) {
+          if (!grow && blk != 0 && (int64_t)blk < num_blocks && shared[blk] != 0) ok = false;
+        }
         if (ok) {
-          const uint32_t bi = pos / (uint32_t)block_size;
-          const uint32_t blk = block_tables[(int64_t)r * cols + bi];
           slot = (int64_t)blk * block_size + pos % (uint32_t)block_size;
           ctx = pos + 1;
           positions[r] = pos + 1;
@@ -291,11 +299,16 @@ hipError_t launch_decode_step_metadata(uint32_t* block_tables, int32_t cols,
                                        uint32_t* ring_state, int32_t ring_cap,
                                        int32_t block_size, int64_t* slot_mapping,
                                        uint32_t* context_lens, uint32_t* status,
-                                       int32_t num_rows, hipStream_t stream) {
-  hipLaunchKernelGGL(decode_step_metadata_kernel, dim3(1), dim3(kMetaThreads), 0, stream,
-                     block_tables, cols, row_blocks, positions, finished, ring, ring_state,
-                     ring_cap, block_size, slot_mapping, context_lens, status, num_rows);
-  return hipGetLastError();
+                                       int32_t num_rows, const uint32_t* shared,
+                                       int64_t num_blocks, hipStream_t stream) {
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kMetaThreads), 0, stream, block_tables, cols,
+                       row_blocks, positions, finished, ring, ring_state, ring_cap, block_size,
+                       slot_mapping, context_lens, status, num_rows, shared, num_blocks);
+    return hipGetLastError();
+  };
+  return shared != nullptr ? go(decode_step_metadata_kernel<true>)
+                           : go(decode_step_metadata_kernel<false>);
 }
 
 hipError_t launch_release_blocks(const uint32_t* block_tables, int32_t cols,

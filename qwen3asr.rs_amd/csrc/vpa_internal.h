@@ -548,7 +548,9 @@ hipError_t launch_decode_step_metadata(uint32_t* block_tables, int32_t cols,
                                        uint32_t* ring_state, int32_t ring_cap,
                                        int32_t block_size, int64_t* slot_mapping,
                                        uint32_t* context_lens, uint32_t* status,
-                                       int32_t num_rows, hipStream_t stream);
+                                       int32_t num_rows,
+                                       const uint32_t* shared,  // null: no block is shared
+                                       int64_t num_blocks, hipStream_t stream);
 hipError_t launch_release_blocks(const uint32_t* block_tables, int32_t cols,
                                  uint32_t* row_blocks, const uint32_t* keep_blocks,
                                  uint32_t* ring, uint32_t* ring_state, int32_t ring_cap,

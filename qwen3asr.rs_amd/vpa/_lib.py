@@ -107,6 +107,8 @@ SIGNATURES = {
                                      _p, _i32, _i32, _i32, _p]),
     "vpa_release_shared_blocks": (ctypes.c_int, [_p, _i32, _p, _p, _i64, _p, _p, _p, _i32, _i32,
                                                  _p]),
+    "vpa_decode_step_metadata_shared": (ctypes.c_int, [
+        _p, _i32, _p, _p, _p, _i64, _p, _p, _p, _i32, _i32, _p, _p, _p, _i32, _p]),
     "vpa_unshare_rows": (ctypes.c_int, [_p, _i32, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i32,
                                         _i32, _i32, _p]),
     "vpa_compact_blocks_workspace_size": (_sz, [_i64]),

@@ -642,8 +642,19 @@ class DeviceBlockAllocator:
         return self.ok
 
     def step(self, finished: Optional[torch.Tensor] = None):
-        """One decode step: returns (slot_mapping, context_lens) device tensors."""
+        """One decode step: returns (slot_mapping, context_lens) device tensors. Where rows
+        may share blocks, one whose next token falls into a block that others hold stalls
+        (``trim`` found none to copy it to) until the block is its own."""
         ring, state, cap = self._common()
+        if self.shared is not None:
+            with _on_device_of(self.block_tables):
+                check(_lib.load().vpa_decode_step_metadata_shared(
+                    self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
+                    self.positions.data_ptr(), self.shared.data_ptr(), self.ring_capacity,
+                    _ptr(finished), ring, state, cap, self.block_size,
+                    self.slot_mapping.data_ptr(), self.context_lens.data_ptr(),
+                    self.status.data_ptr(), self.batch, _stream(self.block_tables)))
+            return self.slot_mapping, self.context_lens
         check(_lib.load().vpa_decode_step_metadata(
             self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
             self.positions.data_ptr(), _ptr(finished), ring, state, cap, self.block_size,
@@ -731,7 +742,8 @@ class DeviceBlockAllocator:
 
         Where rows share blocks, ``buffers`` (the caches, and scales, of all layers) are
         needed: a row cut back to inside a block that others hold takes a copy of it.
-        ``ok`` is then 0 for a row that found no block for one, which must not go on."""
+        ``ok`` is then 0 for a row that found no block for one: it stalls in the steps to
+        come until a ``trim`` finds one or the others gave theirs back."""
         if self.shared is not None:
             if buffers is None:
                 raise _err("rows may share blocks: trim needs the buffers to copy them in")
