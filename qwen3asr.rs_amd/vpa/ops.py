@@ -604,7 +604,8 @@ class DeviceBlockAllocator:
     every buffer on the device so a captured decode graph can run them.
 
     Rows may share blocks once ``fork`` has been called (or ``enable_sharing``, which
-    has to come before a graph with ``release`` or ``trim`` in it is captured):
+    has to come before a graph with ``step``, ``release`` or ``trim`` in it is captured
+    and is refused afterwards):
     ``shared`` then counts the rows that hold each block besides the first. What
     rewrites a row's blocks in place (``evict_kv_cache``) is not for rows that share
     any. ``buffers`` are lists of tensors, or ``BlockBuffers`` made of one once."""
@@ -628,6 +629,12 @@ class DeviceBlockAllocator:
         self.status = torch.zeros(3, dtype=torch.uint32, device=device)
         self.ok = torch.zeros(batch, dtype=torch.uint8, device=device)
         self.shared: Optional[torch.Tensor] = None
+        self._captured_alone = False  # a graph holds calls that do not know of shared blocks
+
+    def _alone(self) -> None:
+        """Ahead of a call that knows of no shared blocks."""
+        if self.block_tables.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._captured_alone = True
 
     def _common(self):
         return (self.free_ring.data_ptr(), self.free_ring_state.data_ptr(), self.ring_capacity)
@@ -655,6 +662,7 @@ class DeviceBlockAllocator:
                     self.slot_mapping.data_ptr(), self.context_lens.data_ptr(),
                     self.status.data_ptr(), self.batch, _stream(self.block_tables)))
             return self.slot_mapping, self.context_lens
+        self._alone()
         check(_lib.load().vpa_decode_step_metadata(
             self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
             self.positions.data_ptr(), _ptr(finished), ring, state, cap, self.block_size,
@@ -667,6 +675,9 @@ class DeviceBlockAllocator:
         if self.shared is None:
             if self.block_tables.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise _err("sharing has to be enabled before the graph is captured")
+            if self._captured_alone:
+                raise _err("a graph was captured whose step or release knows of no shared "
+                           "blocks: enable_sharing has to come before it")
             self.shared = torch.zeros(self.ring_capacity, dtype=torch.int32,
                                       device=self.block_tables.device).view(torch.uint32)
 
@@ -789,6 +800,7 @@ class DeviceBlockAllocator:
                     keep_blocks.contiguous().data_ptr(), ring, state, cap, self.batch,
                     _stream(self.block_tables)))
             return
+        self._alone()
         check(_lib.load().vpa_release_blocks(
             self.block_tables.data_ptr(), self.cols, self.row_blocks.data_ptr(),
             keep_blocks.contiguous().data_ptr(), ring, state, cap, self.batch,
