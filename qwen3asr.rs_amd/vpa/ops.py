@@ -791,6 +791,10 @@ class DeviceBlockAllocator:
     def release(self, keep_blocks: torch.Tensor) -> None:
         """Rows keep their first keep_blocks[r] blocks (u32 [batch]), the rest go back
         (a block that other rows hold: with its last holder)."""
+        if keep_blocks.dtype != torch.uint32 or keep_blocks.shape != (self.batch,):
+            raise _err(f"keep_blocks must be u32 [{self.batch}], got {keep_blocks.dtype} "
+                       f"{tuple(keep_blocks.shape)}")
+        _require_device(keep_blocks, self.block_tables)
         ring, state, cap = self._common()
         if self.shared is not None:
             with _on_device_of(self.block_tables):
