@@ -56,6 +56,7 @@ class DeviceDecodeStep:
                                                        self.max_context_len, device)
         self.scale = head_dim ** -0.5
         self._workspaces = {}
+        self._listed = True  # the step was begun with a work list
 
     def admit(self, prompt_lens: torch.Tensor) -> torch.Tensor:
         """Rows hold prompt_lens[r] tokens already written to the caches (u32
@@ -76,9 +77,10 @@ class DeviceDecodeStep:
         this step's slot_mapping / context_lens and the decode work list
         built (the caches of any layer give the geometry and cache type).
         Layers over a block-scaled cache need no work list: ``block_scaled``
-        leaves it out, for a step of such layers alone."""
+        leaves it out, for a step of such layers alone (others are refused)."""
         self.tokens.consume(self.allocator.slot_mapping)
         self.allocator.step(self.tokens.finished)
+        self._listed = not block_scaled
         if block_scaled:
             return
         ops.paged_attention_plan(self.allocator.context_lens, self.max_context_len, self.cols,
@@ -99,6 +101,9 @@ class DeviceDecodeStep:
                 self.allocator.context_lens, self.scale, max_context_len=self.max_context_len,
                 out=out, workspace=self._scaled_workspace(q, key_cache))
             return
+        if not self._listed:
+            raise ops._err("begin(block_scaled=True) made no work list: this layer's cache is "
+                           "not block-scaled")
         ops.reshape_and_cache(k, v, k_scale, v_scale, key_cache, value_cache,
                               self.allocator.slot_mapping)
         ops.paged_attention(q, k_scale, v_scale, key_cache, value_cache,
