@@ -1584,9 +1584,14 @@ int vpa_adjust_logits(void* logits, int64_t seq_stride, int64_t row_stride, int3
   if (logits == nullptr) return fail(VPA_ERR_INVALID_ARGUMENT, "%s: logits must be non-null", op);
   if (reinterpret_cast<uintptr_t>(logits) % (uintptr_t)dtype_bytes(dtype) != 0)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: misaligned logits", op);
-  // (rows are written: none may lie in another)
-  if ((rows_per_seq > 1 && row_stride < vocab) ||
-      (num_seqs > 1 && seq_stride < (rows_per_seq - 1) * row_stride + vocab))
+  // (rows are written: none may lie in another, whichever of the two dimensions is outside)
+  const bool seqs_outside =
+      (rows_per_seq == 1 || row_stride >= vocab) &&
+      (num_seqs == 1 || seq_stride >= (rows_per_seq - 1) * row_stride + vocab);
+  const bool rows_outside =
+      (num_seqs == 1 || seq_stride >= vocab) &&
+      (rows_per_seq == 1 || row_stride >= (num_seqs - 1) * seq_stride + vocab);
+  if (!seqs_outside && !rows_outside)
     return fail(VPA_ERR_INVALID_ARGUMENT, "%s: logits rows overlap: strides %lld and %lld", op,
                 (long long)seq_stride, (long long)row_stride);
   if ((bias_ids == nullptr) != (bias == nullptr))
