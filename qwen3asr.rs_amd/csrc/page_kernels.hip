@@ -6,8 +6,8 @@
 // allocator's other operations, whose blocks are fresh, need not know of it.
 //
 // All of it is moved bytes and whole numbers: the copy is bound by HBM (two
-// passes over the blocks: 165 MB in 112 buffers of 28 layers 28 us, 5.9 TB/s), the rest
-// by the latency of a few dependent loads (96 forks 4.3 + 3.6 us, their release 13; the
+// passes over the blocks: 165 MB in 112 buffers of 28 layers 29 us, 5.7 TB/s), the rest
+// by the latency of a few dependent loads (96 forks 4.7 + 3.7 us, their release 13; the
 // blocks of a pool of 1024 paired and renamed 6 + 4).
 
 #include "vpa_device.h"

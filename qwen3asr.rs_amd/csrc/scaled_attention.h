@@ -47,12 +47,13 @@
 // Bounds, with 16 query and 8 kv heads of 128 dims: a decode of 256 sequences of 800 to
 // 4096 tokens by HBM (77 us, 5.3 TB/s; a read-only kernel reaches as much); one of 1500
 // tokens by its two launches and their dependent loads (8.0 us, 6.0 + 2.4 on their own);
-// rows of prompts by the issue of vector instructions, about 460 beside 64 matrix
+// rows of prompts by the issue of vector instructions, about 470 beside 64 matrix
 // instructions for 32 rows and 64 keys (512 rows each of 64 prompts of 560 to 1600 tokens:
-// 341 us, 704 TFLOP/s; matrix units busy 31 % of the time, vector issue 70 %). There the
+// 347 us, 691 TFLOP/s; matrix units busy 31 % of the time, vector issue 71 %). There the
 // next operands' bytes are converted between the matrix instructions (1 to 5 % of a
 // prompt's time); without any conversion the same call takes 12 % less, without
-// exponentials 7 %, without loads 5 %. Not kept: 8 waves that split the keys (97 us for the
+// exponentials 7 %, without loads 5 %. A reference of V's scales per row costs such calls
+// 1 to 4 %, a decode nothing. Not kept: 8 waves that split the keys (97 us for the
 // 256 sequences).
 #pragma once
 
@@ -173,11 +174,12 @@ constexpr bool scaled_two_tiles() {
 
 // Waves per SIMD: O, Q and two tiles' bytes are what a wave holds. Two row tiles of head
 // dims 192 and 256 fill it alone, and share each conversion: 512 rows each of 32 prompts
-// of 1000 to 2000 tokens, head dim 256, 487 us, 714 with one tile. (Four row tiles of
-// head dim 128, alone too, are slower than two waves of two: 450 us for 340.)
+// of 1000 to 2000 tokens, calls of 192 / 256 dims, 450 / 512 us, 620 / 717 with one tile.
+// (Four row tiles of head dim 128, alone too, are slower than two waves of two: 450 us
+// for 340.) Head dim 64's two tiles fit three waves, in 168 registers.
 template <typename T, int D, int BS, int NQ>
 constexpr int scaled_waves_per_eu() {
-  if (D == 64 && NQ == 2 && BS > 8) return 3;  // (168 registers)
+  if (D == 64 && NQ == 2 && BS > 8) return 3;
   return D <= 128 || (D == 192 && NQ == 1 && !std::is_same_v<T, float>) ? 2 : 1;
 }
 

@@ -64,7 +64,7 @@ __device__ __forceinline__ void widen(const uint4& v, float (&f)[16 / sizeof(T)]
   }
 }
 
-// One byte scaled by `ratio` (a scale over a larger one).
+// Four bytes scaled by `ratio` (a scale over a larger one).
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
   const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
@@ -323,10 +323,14 @@ hipError_t launch_scaled_append(int dtype, const ScaledAppendArgs& a, const Cach
 // (64 times 200 rows over 2000 keys: 184, 173; 40 rows each, 1024 tiles: 61, 66), where
 // one tile alone is always split (a decode). Contexts of one step of 64 keys have nothing
 // to split (256 of them: 17 us, 8), and more than 256 rows go without (8000 keys, 128
-// rows: 19 us split, 24 not; a batch of 64 with 1024 rows each keeps its waves busy).
+// rows: 19 us split, 24 not; a batch of 64 with 1024 rows each keeps its waves busy). That
+// border is the batch's: one to four prompts of 1024 rows (512 positions) would gain by the
+// split over shorter contexts (one over 2000 keys 38 us, 23 split; over 6500 56, 54; four
+// over 4000 102, 89) and lose over long ones (four over 8000 177, 183; two over 6000 80, 81).
 // Waves with rows of their own are a workgroup each: four to one end at different keys
 // and leave the last one's without rows (64 times 400 rows: 68 us for 53; 512 rows each
-// of 32 prompts, head dim 256: 548, 496; never more than 2 % faster).
+// of 32 prompts, head dim 256: 548, 496, both of a build of their own; never more than 2 %
+// faster).
 // Keys: chunks over workgroups until an MI355X has one of four waves (split keys) per
 // compute unit or two waves (with rows of their own, which finish at different times) per
 // SIMD, of at least 256 keys; where the waves split the keys and there are enough
