@@ -793,7 +793,7 @@ size_t vpa_paged_attention_block_scaled_workspace_size(int32_t num_seqs, int32_t
  * vpa_chunked_prefill_paged_attention the caller's. Scales may be any finite
  * numbers, not only powers of two; those of blocks that a row does not see have
  * no part in its result. Of those it sees, a token counts as long as p_t
- * value_scales is above 2^-27 of the largest (probabilities are 16-bit numbers,
+ * value_scales is above 2^-32 of the largest (probabilities are 16-bit numbers,
  * for f32 queries pairs of them).
  * Any number of query heads per kv head, head_dim 64, 96, 128, 192 or 256,
  * block_size 8, 16 or 32. n_s and L_s are clamped to max_query_len and
@@ -820,10 +820,11 @@ int vpa_paged_attention_block_scaled(
  * all zeros before the first fork. vpa_allocate_rows goes on as it is (its
  * blocks are fresh); rows step with vpa_decode_step_metadata_shared and give
  * blocks back with vpa_release_shared_blocks in place of
- * vpa_decode_step_metadata and vpa_release_blocks. A shared block is full for all its holders, so nobody
- * writes to it, unless a row is cut back (vpa_unshare_rows); vpa_evict_kv_cache,
- * which rewrites a row's blocks, is not for rows that share any. Block 0 is not
- * counted. No counterparts in the reference, whose blocks have one owner.
+ * vpa_decode_step_metadata and vpa_release_blocks. A shared block is full for
+ * all its holders, so nobody writes to it, unless a row is cut back
+ * (vpa_unshare_rows); vpa_evict_kv_cache, which rewrites a row's blocks, is not
+ * for rows that share any. Block 0 is not counted. No counterparts in the
+ * reference, whose blocks have one owner.
  */
 
 /*

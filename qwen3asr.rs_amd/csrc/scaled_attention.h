@@ -13,9 +13,9 @@
 // 448; that largest one is part of the softmax scale and of the output. Every
 // product is exact as long as the ratio is at least 2^-5 (E4M3's least number,
 // 2^-9, stays normal in f16). Steps with smaller ratios or other scales multiply
-// the f32 scores and probabilities instead. V's reference is a row's own, at most 2^5
-// above the largest scale that it sees: blocks that it does not see, louder by any factor,
-// do not push its weights p_t vs_t / vrow out of f16's range.
+// the f32 scores and probabilities instead. V's reference is then the largest scale that
+// the row itself sees: blocks that it does not see, louder by any factor, do not push its
+// weights p_t vs_t / vrow out of f16's range.
 //
 // Work of a wave: 16 NQ rows (a row is a position and a query head of the kv
 // head; heads fastest, so any group size fills the rows) over 64 keys at a time
@@ -113,8 +113,8 @@ constexpr int kScaledWaves = 4;  // of a workgroup that splits the keys
 constexpr int kScaledKeys = 64;  // keys of a step
 constexpr float kScaledSlack = 8.f;
 constexpr int kScaledProbLog2 = 7;
-// How far above a row's own the wave's reference of V's scales may be taken for it: what the
-// conversion takes along exactly.
+// How far above a row's own the wave's reference of V's scales is taken for it where the
+// conversion takes the ratios along, exactly.
 constexpr float kScaledReach = 32.f;
 
 // Maximum / sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
@@ -294,9 +294,9 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, BS, NQ>()))) void s
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[q][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  // V's reference: the largest scale of all that the wave's steps held or, for a row whose own
-  // do not reach that far (kScaledReach), the largest that it has seen. Rows of a wave differ
-  // in it only where the wave is `apart`.
+  // V's reference: the largest scale that a row has seen or, where the conversion takes the
+  // ratio along, the largest of all that the wave's steps held. Rows of a wave differ in it
+  // only where the wave is `apart`.
   float vrow[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) vrow[q] = 1.50463277e-36f;  // 2^-119 (over 2^kScaledProbLog2 normal)
@@ -555,6 +555,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, BS, NQ>()))) void s
 #pragma unroll
           for (int q = 0; q < NQ; ++q) vref = fmaxf(vref, vrow[q]);
           vref = wave_max_dpp(vref);
+          const float reach = all_plain(sc.v, vref) ? kScaledReach : 1.f;
           bool off = false;
 #pragma unroll
           for (int q = 0; q < NQ; ++q) {
@@ -563,7 +564,7 @@ __attribute__((amdgpu_waves_per_eu(scaled_waves_per_eu<T, D, BS, NQ>()))) void s
               seen = fmaxf(seen, k0 + 16 * kg + 8 <= limit[q] ? fabsf(sc.v[1]) : 0.f);
             seen = fmaxf(vrow[q], max_rows(seen));
             // (a row that sees nothing at all takes any)
-            const float to = limit[q] < k_first || seen * kScaledReach >= vref ? vref : seen;
+            const float to = limit[q] < k_first || seen * reach >= vref ? vref : seen;
             fix[q] *= vrow[q] / to;
             vrow[q] = to;
             off = off || to != vref;

@@ -80,3 +80,33 @@ def test_odd_and_negative_scales_apart(device):
             p.vs[p.tables[0, 1::2]] *= np.float32(-(2.0 ** 23))
             louder(p, 1, 3, 5, -70)
             p.check()
+
+
+@pytest.mark.parametrize("bs", [8, 16, 32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_small_probabilities_beside_a_block_somewhat_louder(device, dtype, bs):
+    """Rows whose result is made of probabilities of 2^-28: they count by the scale that the
+    rows see, not by that of the next block, 24 times as large."""
+    p = Problem(device, 31, dtype, 2, 1, 64, bs, [2 * bs], rows=[2 * bs])
+    first, second = p.tables[0, :2]
+    p.q[:] = 1.0
+    p.kc[:] = 0xB8  # -1
+    p.kc[first, :, :, 0] = 0x38  # 1: the first token, the others 28.5 bits below it
+    p.ks[:] = 28.5 * np.log(2) / 2 / (64 * p.scale)
+    p.vc[:] = 0x7E  # 448, of the first token 0
+    p.vc[first, :, :, 0] = 0
+    p.vs[first], p.vs[second] = 1.0, 24.0
+    got = p.check()
+    assert (got[1:bs] > 0).all()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_prompts_over_scales_of_any_size(device, seed):
+    """Random scales of 2^-48 to 2^40 times odd numbers: every row by the largest that it sees,
+    beside rows that see a block or two more."""
+    rng = np.random.default_rng(seed)
+    lens, rows = rng.integers(0, 71, size=40), rng.integers(0, 90, size=40)
+    p = Problem(device, seed, torch.float32, 14, 2, 96, (8, 16)[seed % 2], lens, rows=rows,
+                any_scale=seed > 2, spread=20)
+    p.vs *= np.ldexp(1.0, rng.integers(-40, 41, size=p.vs.shape)).astype(np.float32)
+    p.check()
